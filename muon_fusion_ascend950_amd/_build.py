@@ -2,10 +2,10 @@
 
 Two shared objects land next to this file:
 
-* ``libmuon_polar.so`` — the HIP kernels and the C ABI of ``include/muon_polar.h``
-  (``hipcc --offload-arch=gfx950``; no torch dependency).
-* ``_C.so`` — the torch operator ``muon_ascend950::polar_step`` (g++ against the
-  torch headers), linked to ``libmuon_polar.so``.
+* ``libmuon_polar.so`` — the HIP kernels and the C ABI of ``include/muon_polar.h`` and
+  ``include/muon_train.h`` (``hipcc --offload-arch=gfx950``; no torch dependency).
+* ``_C.so`` — the torch operators ``muon_ascend950::*`` (g++ against the torch
+  headers), linked to ``libmuon_polar.so``.
 
 This mirrors the reference build (``setup.py:46-153``: an accelerator compiler
 turns the kernel source into an object, then a C++ extension links it), with
@@ -75,7 +75,7 @@ def build_hip_library(verbose: bool = True) -> Path:
     BUILD_DIR.mkdir(exist_ok=True)
     common = HIP_FLAGS + [f"-I{INCLUDE}", f"-I{CSRC}"]
     sources = ["polar_kernels.hip", "polar_stream.hip", "polar_norm.hip", "polar_noalloc.hip",
-               "polar_resident.hip", "polar_capi.cpp"]
+               "polar_resident.hip", "polar_capi.cpp", "train_norms.hip"]
     objects = [BUILD_DIR / (Path(src).stem + ".o") for src in sources]
     jobs = [[_hipcc(), "-x", "hip", "-c", str(CSRC / src), "-o", str(obj)] + common
             for src, obj in zip(sources, objects)]
@@ -100,7 +100,7 @@ def build_torch_binding(verbose: bool = True) -> Path:
     cxx = shutil.which("g++") or "g++"
     cmd = [
         cxx, "-O2", "-std=c++17", "-fPIC", "-shared",
-        str(CSRC / "muon_polar_step_binding.cpp"),
+        str(CSRC / "muon_polar_step_binding.cpp"), str(CSRC / "muon_train_binding.cpp"),
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
         f"-I{INCLUDE}", f"-I{ROCM / 'include'}",
         f"-I{sysconfig.get_paths()['include']}",

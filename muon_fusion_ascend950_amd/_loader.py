@@ -68,7 +68,24 @@ def load_library() -> None:
                               lr, weight_decay, lr_scale):
         return None
 
-    for name, fake in (("muon_ascend950::polar_step", fake_polar_step),
+    def fake_norms_forward(y, residual, post_weight, gate, scale, scale_value, pre_weight,
+                           gate_kind, rows_per_sequence, post_norm, pre_norm, eps, save):
+        rows = y.numel() // y.shape[-1]
+        return (residual.new_empty(y.shape), y.new_empty(y.shape if pre_norm else (0,)),
+                y.new_empty((rows if save else 0, 2), dtype=torch.float32))
+
+    def fake_norms_backward(y, residual, post_weight, gate, scale, scale_value, pre_weight,
+                            gate_kind, rows_per_sequence, post_norm, pre_norm, eps, stats,
+                            d_residual_out, d_normed, wanted):
+        def grad(t, bit):
+            return y.new_empty((0,)) if t is None or not wanted & bit else t.new_empty(t.shape)
+
+        return (y.new_empty(y.shape), residual.new_empty(y.shape), grad(post_weight, 1),
+                grad(gate, 2), grad(scale, 4), grad(pre_weight, 8))
+
+    for name, fake in (("muon_ascend950::norms_forward", fake_norms_forward),
+                       ("muon_ascend950::norms_backward", fake_norms_backward),
+                       ("muon_ascend950::polar_step", fake_polar_step),
                        ("muon_ascend950::polar_step_tall", fake_polar_step),
                        ("muon_ascend950::polar_express", fake_polar_express),
                        ("muon_ascend950::muon_update", fake_muon_update),

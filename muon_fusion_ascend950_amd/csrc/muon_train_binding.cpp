@@ -1,0 +1,201 @@
+// muon_train_binding.cpp — registers the operators of a training step around the Muon
+// update (include/muon_train.h) as torch operators of the muon_ascend950 library.  No
+// reference counterpart.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/library.h>
+
+#include "muon_train.h"
+
+namespace {
+
+using OptTensor = std::optional<at::Tensor>;
+
+int dtype_of(const at::Tensor &t, const char *what) {
+    TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, what,
+                " must be float32 or bfloat16");
+    return t.scalar_type() == at::kFloat ? MUON_TRAIN_F32 : MUON_TRAIN_BF16;
+}
+
+bool given(const OptTensor &t) { return t.has_value() && t->defined(); }
+
+hipStream_t stream_of(const at::Tensor &t) {
+    return c10::hip::getCurrentHIPStream(t.device().index()).stream();
+}
+
+// t [.., d] as rows: the tensor itself where its rows lie evenly apart and unbroken,
+// otherwise a contiguous copy.
+struct Rows {
+    at::Tensor t;
+    int64_t rows, ld;
+};
+Rows as_rows(const at::Tensor &t) {
+    const int64_t d = t.size(-1), rows = d > 0 ? t.numel() / d : 0;
+    if (t.is_contiguous()) return {t, rows, d};
+    at::Tensor r = t.reshape({rows, d});
+    if (d > 1 && r.stride(1) == 1 && r.stride(0) >= d) return {r, rows, r.stride(0)};
+    return {r.contiguous(), rows, d};
+}
+
+at::Tensor none(const at::Tensor &like) { return at::empty({0}, like.options()); }
+
+// ---------------------------------------------------------------------------- norms
+struct Norms {
+    muon_train_norms_args a{};
+    Rows y, residual;
+    at::Tensor post, pre, gate, scale;
+
+    Norms(const at::Tensor &y_, const at::Tensor &residual_, const OptTensor &post_weight,
+          const OptTensor &gate_, const OptTensor &scale_, double scale_value,
+          const OptTensor &pre_weight, int64_t gate_kind, int64_t rows_per_sequence,
+          bool post_norm, bool pre_norm, double eps) {
+        TORCH_CHECK(y_.device().is_cuda() && residual_.device() == y_.device(),
+                    "block_norms: y and residual must be on one ROCm (HIP) device");
+        TORCH_CHECK(y_.dim() >= 1 && y_.sizes() == residual_.sizes(),
+                    "block_norms: y and residual must have one shape");
+        a.d = y_.size(-1);
+        a.y_dtype = dtype_of(y_, "block_norms: y");
+        a.residual_dtype = dtype_of(residual_, "block_norms: residual");
+        y = as_rows(y_);
+        residual = as_rows(residual_);
+        a.rows = y.rows;
+        a.ld_y = y.ld;
+        a.ld_residual = residual.ld;
+        a.y = y.t.data_ptr();
+        a.residual = residual.t.data_ptr();
+        auto vector = [&](const OptTensor &t, int64_t numel, const char *what) {
+            TORCH_CHECK(t->device() == y_.device() && t->numel() == numel, "block_norms: ", what,
+                        " has the wrong device or size");
+            return t->contiguous();
+        };
+        if (given(post_weight)) {
+            post = vector(post_weight, a.d, "post_weight");
+            a.weight_dtype = dtype_of(post, "block_norms: post_weight");
+            a.post_weight = post.data_ptr();
+        }
+        if (given(pre_weight)) {
+            pre = vector(pre_weight, a.d, "pre_weight");
+            a.weight_dtype = dtype_of(pre, "block_norms: pre_weight");
+            a.pre_weight = pre.data_ptr();
+            TORCH_CHECK(!post.defined() || post.scalar_type() == pre.scalar_type(),
+                        "block_norms: post_weight and pre_weight must have one dtype");
+        }
+        a.gate_kind = static_cast<int>(gate_kind);
+        a.rows_per_sequence = rows_per_sequence;
+        if (gate_kind != MUON_TRAIN_GATE_NONE) {
+            TORCH_CHECK(given(gate_), "block_norms: gate is missing");
+            TORCH_CHECK(gate_kind != MUON_TRAIN_GATE_SEQUENCE || rows_per_sequence > 0,
+                        "block_norms: rows_per_sequence must be positive");
+            const int64_t numel = gate_kind == MUON_TRAIN_GATE_CHANNEL ? a.d
+                                  : gate_kind == MUON_TRAIN_GATE_SEQUENCE
+                                      ? a.rows / rows_per_sequence * a.d
+                                  : gate_kind == MUON_TRAIN_GATE_TOKEN ? a.rows
+                                                                       : a.rows * a.d;
+            gate = vector(gate_, numel, "gate");
+            a.gate_dtype = dtype_of(gate, "block_norms: gate");
+            a.gate = gate.data_ptr();
+        }
+        a.scale_value = scale_value;
+        if (given(scale_)) {
+            a.scale_kind = scale_->numel() == 1 ? MUON_TRAIN_SCALE_SCALAR : MUON_TRAIN_SCALE_VECTOR;
+            scale = vector(scale_, scale_->numel() == 1 ? 1 : a.d, "residual_scale");
+            TORCH_CHECK(scale.scalar_type() == at::kFloat,
+                        "block_norms: residual_scale must be float32");
+            a.scale = scale.data_ptr<float>();
+        }
+        a.post_norm = post_norm;
+        a.pre_norm = pre_norm;
+        a.eps = eps;
+    }
+};
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> NormsForward(
+    const at::Tensor &y, const at::Tensor &residual, const OptTensor &post_weight,
+    const OptTensor &gate, const OptTensor &scale, double scale_value, const OptTensor &pre_weight,
+    int64_t gate_kind, int64_t rows_per_sequence, bool post_norm, bool pre_norm, double eps,
+    bool save) {
+    const c10::OptionalDeviceGuard device_guard(y.device());
+    Norms n(y, residual, post_weight, gate, scale, scale_value, pre_weight, gate_kind,
+            rows_per_sequence, post_norm, pre_norm, eps);
+    at::Tensor out = at::empty(y.sizes(), residual.options());
+    at::Tensor normed = pre_norm ? at::empty(y.sizes(), y.options()) : none(y);
+    at::Tensor stats = at::empty({save ? n.a.rows : 0, 2}, y.options().dtype(at::kFloat));
+    n.a.residual_out = out.data_ptr();
+    if (pre_norm) n.a.normed = normed.data_ptr();
+    if (save) n.a.stats = stats.data_ptr<float>();
+    const int st = muon_train_norms_forward(&n.a, stream_of(y));
+    TORCH_CHECK(st == MUON_POLAR_OK, "block_norms: ", muon_polar_last_error());
+    return {out, normed, stats};
+}
+
+// wanted: bits of the gradients wanted (1 post_weight, 2 gate, 4 scale, 8 pre_weight); y's
+// and residual's are always formed.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> NormsBackward(
+    const at::Tensor &y, const at::Tensor &residual, const OptTensor &post_weight,
+    const OptTensor &gate, const OptTensor &scale, double scale_value, const OptTensor &pre_weight,
+    int64_t gate_kind, int64_t rows_per_sequence, bool post_norm, bool pre_norm, double eps,
+    const at::Tensor &stats, const OptTensor &d_residual_out, const OptTensor &d_normed,
+    int64_t wanted) {
+    const c10::OptionalDeviceGuard device_guard(y.device());
+    Norms n(y, residual, post_weight, gate, scale, scale_value, pre_weight, gate_kind,
+            rows_per_sequence, post_norm, pre_norm, eps);
+    TORCH_CHECK(stats.is_contiguous() && stats.scalar_type() == at::kFloat &&
+                    stats.numel() == 2 * n.a.rows,
+                "block_norms: stats of another forward pass");
+    n.a.stats = stats.data_ptr<float>();
+    at::Tensor dro, dno;
+    if (given(d_residual_out)) {
+        TORCH_CHECK(d_residual_out->sizes() == y.sizes() &&
+                        d_residual_out->scalar_type() == residual.scalar_type(),
+                    "block_norms: the gradient of residual_out has another shape or dtype");
+        dro = d_residual_out->contiguous();
+        n.a.d_residual_out = dro.data_ptr();
+    }
+    if (given(d_normed) && pre_norm) {
+        TORCH_CHECK(d_normed->sizes() == y.sizes() && d_normed->scalar_type() == y.scalar_type(),
+                    "block_norms: the gradient of normed has another shape or dtype");
+        dno = d_normed->contiguous();
+        n.a.d_normed = dno.data_ptr();
+    }
+    at::Tensor dy = at::empty(y.sizes(), y.options());
+    at::Tensor dr = at::empty(y.sizes(), residual.options());
+    auto grad = [&](const at::Tensor &t, int64_t bit) {
+        return (wanted & bit) && t.defined() ? at::empty(t.sizes(), t.options()) : none(y);
+    };
+    at::Tensor d_post = grad(n.post, 1), d_gate = grad(n.gate, 2), d_scale = grad(n.scale, 4),
+               d_pre = grad(n.pre, 8);
+    n.a.d_y = dy.data_ptr();
+    n.a.d_residual = dr.data_ptr();
+    if ((wanted & 1) && n.post.defined()) n.a.d_post_weight = d_post.data_ptr();
+    if ((wanted & 2) && n.gate.defined()) n.a.d_gate = d_gate.data_ptr();
+    if ((wanted & 4) && n.scale.defined()) n.a.d_scale = d_scale.data_ptr<float>();
+    if ((wanted & 8) && n.pre.defined()) n.a.d_pre_weight = d_pre.data_ptr();
+    size_t bytes = 0;
+    int st = muon_train_norms_workspace(&n.a, &bytes);
+    TORCH_CHECK(st == MUON_POLAR_OK, "block_norms: ", muon_polar_last_error());
+    at::Tensor workspace =
+        at::empty({static_cast<int64_t>(bytes)}, y.options().dtype(at::kByte));
+    st = muon_train_norms_backward(&n.a, workspace.data_ptr(), bytes, stream_of(y));
+    TORCH_CHECK(st == MUON_POLAR_OK, "block_norms: ", muon_polar_last_error());
+    return {dy, dr, d_post, d_gate, d_scale, d_pre};
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(muon_ascend950, m) {
+    m.def("norms_forward(Tensor y, Tensor residual, Tensor? post_weight, Tensor? gate, "
+          "Tensor? scale, float scale_value, Tensor? pre_weight, int gate_kind, "
+          "int rows_per_sequence, bool post_norm, bool pre_norm, float eps, bool save) -> "
+          "(Tensor, Tensor, Tensor)");
+    m.def("norms_backward(Tensor y, Tensor residual, Tensor? post_weight, Tensor? gate, "
+          "Tensor? scale, float scale_value, Tensor? pre_weight, int gate_kind, "
+          "int rows_per_sequence, bool post_norm, bool pre_norm, float eps, Tensor stats, "
+          "Tensor? d_residual_out, Tensor? d_normed, int wanted) -> "
+          "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+}
+
+TORCH_LIBRARY_IMPL(muon_ascend950, CUDA, m) {
+    m.impl("norms_forward", &NormsForward);
+    m.impl("norms_backward", &NormsBackward);
+}

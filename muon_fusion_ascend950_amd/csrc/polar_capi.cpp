@@ -1581,6 +1581,15 @@ void stage_extent(const StageLaunch &L, bool splits, muon_polar_stage_extent &e)
 
 }  // namespace
 
+// The operators of muon_train.h report through the same thread-local message.
+int muon_polar::report(int code, const char *msg) noexcept {
+    try {
+        return fail(code, msg);
+    } catch (...) {  // no memory for the message: the code says enough
+        return code;
+    }
+}
+
 extern "C" {
 
 int muon_polar_query(int64_t batch, int64_t m, int64_t n, muon_polar_shape_info *info) {

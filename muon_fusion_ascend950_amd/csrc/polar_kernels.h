@@ -188,4 +188,7 @@ hipError_t launch_resident(const ResidentArgs &g, int64_t batch, hipStream_t str
 constexpr size_t kNoAllocScratchBytes = size_t(192) << 20;
 hipError_t noalloc_scratch(int device, void **ptr);
 
+// Keeps `msg` for muon_polar_last_error() on this thread and returns `code`.
+int report(int code, const char *msg) noexcept;
+
 }  // namespace muon_polar

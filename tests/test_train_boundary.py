@@ -1,0 +1,128 @@
+"""Host side of the training-step operators, without a GPU: public names, refusals of wrong
+arguments, FakeTensor kernels, and the C ABI of include/muon_train.h (its exported set and
+its checks before any launch)."""
+
+from __future__ import annotations
+
+import ctypes
+import re
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import muon_fusion_ascend950_amd as mf
+from muon_fusion_ascend950_amd import capi, train
+
+ROOT = Path(__file__).resolve().parent.parent
+HEADER = ROOT / "include" / "muon_train.h"
+F32, B16 = torch.float32, torch.bfloat16
+
+
+def test_public_names():
+    assert mf.train is train
+    for name in train.__all__:
+        assert getattr(train, name).__doc__, name
+
+
+def test_header_declares_what_the_library_exports():
+    declared = set(re.findall(r"^int (muon_train_\w+)\s*\(", HEADER.read_text(), re.M))
+    out = subprocess.run(["nm", "-D", "--defined-only", str(capi.library_path())],
+                         capture_output=True, text=True, check=True).stdout
+    assert declared and declared == set(re.findall(r" T (muon_train_\w+)$", out, re.M))
+
+
+# ------------------------------------------------------------------------------- norms
+def _cuda(*shape, dtype=F32):
+    return torch.empty(shape, dtype=dtype, device="cuda")
+
+
+def _norms_ok(**change):
+    args = dict(y=_cuda(2, 3, 64, dtype=B16), residual=_cuda(2, 3, 64), post_weight=_cuda(64),
+                gate=_cuda(2, 1, 64, dtype=B16), residual_scale=_cuda(1), pre_weight=_cuda(64))
+    args.update(change)
+    return args
+
+
+def _norms(**args):
+    return train.block_norms(args.pop("y"), args.pop("residual"), **args)
+
+
+@pytest.mark.parametrize("change,error,message", [
+    (lambda: dict(y=[1.0]), TypeError, "torch.Tensor"),
+    (lambda: dict(y=torch.zeros(2, 3, 64)), ValueError, "ROCm GPU"),
+    (lambda: dict(y=_cuda(2, 3, 64, dtype=torch.float16)), TypeError, "float32 or torch.bfloat16"),
+    (lambda: dict(residual=_cuda(2, 64)), ValueError, "one shape"),
+    (lambda: dict(residual=torch.zeros(2, 3, 64)), ValueError, "cuda"),
+    (lambda: dict(y=_cuda(2, 16385), residual=_cuda(2, 16385)), ValueError, "16384"),
+    (lambda: dict(y=_cuda(2, 0), residual=_cuda(2, 0)), ValueError, "16384"),
+    (lambda: dict(y=_cuda(), residual=_cuda()), ValueError, "shape"),
+    (lambda: dict(post_weight=_cuda(63)), ValueError, "post_weight"),
+    (lambda: dict(pre_weight=_cuda(1, 64)), ValueError, "pre_weight"),
+    (lambda: dict(pre_weight=_cuda(64, dtype=B16)), TypeError, "one dtype"),
+    (lambda: dict(pre_norm=False), ValueError, "pre_norm"),
+    (lambda: dict(gate=_cuda(3, 1, 64)), ValueError, "gate"),
+    (lambda: dict(gate=_cuda(2, 3)), ValueError, "gate"),
+    (lambda: dict(gate=0.5), TypeError, "gate"),
+    (lambda: dict(residual_scale=_cuda(2)), ValueError, "residual_scale"),
+    (lambda: dict(residual_scale=_cuda(64, dtype=B16)), TypeError, "residual_scale"),
+    (lambda: dict(eps=-1.0), ValueError, "eps"),
+    (lambda: dict(eps=float("nan")), ValueError, "eps"),
+])
+def test_block_norms_refuses(change, error, message):
+    with FakeTensorMode():
+        with pytest.raises(error, match=message):
+            _norms(**_norms_ok(**change()))
+
+
+def test_block_norms_fake():
+    with FakeTensorMode():
+        args = _norms_ok()
+        out, h = _norms(**args)
+        assert out.shape == h.shape == (2, 3, 64) and (out.dtype, h.dtype) == (F32, B16)
+        args = _norms_ok(pre_weight=None, pre_norm=False)
+        assert _norms(**args)[1] is None
+        args = _norms_ok()
+        ops = torch.ops.muon_ascend950
+        common = (args["y"], args["residual"], args["post_weight"], args["gate"],
+                  args["residual_scale"], 1.0, args["pre_weight"], 2, 3, True, True, 1e-6)
+        stats = ops.norms_forward(*common, True)[2]
+        assert stats.shape == (6, 2) and stats.dtype == F32
+        grads = ops.norms_backward(*common, stats, None, args["y"], 2 | 4)
+        like = [args[n] for n in ("y", "residual", "gate", "residual_scale")]
+        got = [grads[0], grads[1], grads[3], grads[4]]
+        assert [(g.shape, g.dtype) for g in got] == [(t.shape, t.dtype) for t in like]
+        assert grads[2].numel() == grads[5].numel() == 0
+
+
+class NormsArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("rows", "d", "rows_per_sequence", "ld_y", "ld_residual")] + [
+        (n, ctypes.c_void_p) for n in ("y", "residual", "post_weight", "pre_weight", "gate", "scale")] + [
+        (n, ctypes.c_double) for n in ("scale_value", "eps")] + [
+        (n, ctypes.c_int) for n in ("y_dtype", "residual_dtype", "weight_dtype", "gate_dtype",
+                                    "gate_kind", "scale_kind", "post_norm", "pre_norm")] + [
+        (n, ctypes.c_void_p) for n in ("residual_out", "normed", "stats", "d_residual_out", "d_normed",
+                                       "d_y", "d_residual", "d_post_weight", "d_pre_weight",
+                                       "d_gate", "d_scale")]
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(rows=-1), "rows"), (dict(d=0), "d must"), (dict(d=16385), "d must"),
+    (dict(y_dtype=2), "dtypes"), (dict(gate_kind=5), "kind"), (dict(scale_kind=-1), "kind"),
+    (dict(gate_kind=2, rows_per_sequence=0, gate=4096), "rows_per_sequence"),
+    (dict(gate_kind=2, rows_per_sequence=3, gate=4096), "rows_per_sequence"),
+    (dict(gate_kind=1), "null"), (dict(scale_kind=1), "null"), (dict(y=None), "null"),
+    (dict(ld_y=7), "overlap"), (dict(residual_out=None), "null output"),
+    (dict(normed=None), "null output"),
+])
+def test_norms_entry_checks_before_any_launch(change, message):
+    lib = capi.load()
+    base = dict(rows=4, d=8, rows_per_sequence=4, ld_y=8, ld_residual=8, y=4096, residual=4096,
+                eps=1e-6, pre_norm=1, residual_out=4096, normed=4096)
+    args = NormsArgs(**{**base, **change})
+    assert lib.muon_train_norms_forward(ctypes.byref(args), None) == capi.ERR_INVALID_ARGUMENT
+    assert message in capi.last_error()
+    assert lib.muon_train_norms_forward(None, None) == capi.ERR_INVALID_ARGUMENT
+    assert lib.muon_train_norms_forward(ctypes.byref(NormsArgs(**{**base, "rows": 0})), None) == capi.OK
