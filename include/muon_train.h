@@ -3,6 +3,7 @@
  * (same library as muon_polar.h: libmuon_polar.so).
  *
  *   norms    the norms before and after a block, with its gate and residual scale
+ *   distill  the loss against a teacher's top logits
  *
  * All functions are asynchronous on the given HIP stream.  Pointers are device pointers
  * unless said otherwise; structs are read during the call only.  No function allocates
@@ -77,6 +78,38 @@ int muon_train_norms_forward(const muon_train_norms_args *args, hipStream_t stre
 int muon_train_norms_workspace(const muon_train_norms_args *args, size_t *bytes);
 int muon_train_norms_backward(const muon_train_norms_args *args, void *workspace,
                               size_t workspace_bytes, hipStream_t stream);
+
+/* ----------------------------------------------------------------- distill
+ * Of each row (a token with `vocab` student logits z and k teacher logits t at the
+ * indices i), in fp32:
+ *
+ *     p = softmax(t / τ) over the row's entries with 0 <= i < vocab (others are absent)
+ *     loss = (1 − λ)·τ²·Σ_j p_j·(log p_j − log softmax(z / τ)[i_j]) + λ·CE(z, label)
+ *     grad = g·[(1 − λ)·τ·(softmax(z / τ) − p) + λ·(softmax(z) − onehot(label))]
+ *
+ * with λ = label_weight.  A row whose entries are all absent or −inf has no first term, a
+ * row whose label is outside [0, vocab) no second.  An index that occurs twice counts
+ * twice.  `grad` may be `logits` itself (same address and row length); otherwise the two
+ * must not overlap. */
+typedef struct muon_train_distill_args {
+    int64_t rows, vocab, k; /* k: 1 to 1024 */
+    int64_t ld_logits, ld_grad; /* elements from row to row, >= vocab */
+    const void *logits;         /* [rows, vocab] */
+    const void *teacher_logits; /* [rows, k] */
+    const void *teacher_indices; /* [rows, k], int32 or int64 */
+    const int64_t *labels;      /* [rows], or null: no second term */
+    const float *grad_loss;     /* [rows], or null: grad_value for every row */
+    double temperature, label_weight, grad_value;
+    int logits_dtype, teacher_dtype, index_bytes; /* index_bytes: 4 or 8 */
+    float *loss;  /* [rows] */
+    float *stats; /* [rows, 4]: max z, 1 / Σ exp((z − max) / τ), 1 / Σ exp(z − max), 0 */
+    void *grad;   /* [rows, vocab], logits' dtype */
+} muon_train_distill_args;
+
+/* loss, and where they are not null stats and (in the same pass over the logits) grad. */
+int muon_train_distill_forward(const muon_train_distill_args *args, hipStream_t stream);
+/* grad from the stats of a forward pass. */
+int muon_train_distill_backward(const muon_train_distill_args *args, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -83,7 +83,24 @@ def load_library() -> None:
         return (y.new_empty(y.shape), residual.new_empty(y.shape), grad(post_weight, 1),
                 grad(gate, 2), grad(scale, 4), grad(pre_weight, 8))
 
-    for name, fake in (("muon_ascend950::norms_forward", fake_norms_forward),
+    def fake_distill_forward(logits, teacher_logits, teacher_indices, labels, temperature,
+                             label_weight, save):
+        rows = logits.numel() // logits.shape[-1]
+        return (logits.new_empty(logits.shape[:-1], dtype=torch.float32),
+                logits.new_empty((rows if save else 0, 4), dtype=torch.float32))
+
+    def fake_distill_backward(logits, teacher_logits, teacher_indices, labels, temperature,
+                              label_weight, stats, grad_loss):
+        return logits.new_empty(logits.shape)
+
+    def fake_distill_with_grad(logits, teacher_logits, teacher_indices, labels, temperature,
+                               label_weight, grad_loss, grad_value, grad):
+        return logits.new_empty(logits.shape[:-1], dtype=torch.float32)
+
+    for name, fake in (("muon_ascend950::distill_forward", fake_distill_forward),
+                       ("muon_ascend950::distill_backward", fake_distill_backward),
+                       ("muon_ascend950::distill_with_grad", fake_distill_with_grad),
+                       ("muon_ascend950::norms_forward", fake_norms_forward),
                        ("muon_ascend950::norms_backward", fake_norms_backward),
                        ("muon_ascend950::polar_step", fake_polar_step),
                        ("muon_ascend950::polar_step_tall", fake_polar_step),

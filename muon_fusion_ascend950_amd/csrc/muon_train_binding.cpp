@@ -181,6 +181,121 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
     return {dy, dr, d_post, d_gate, d_scale, d_pre};
 }
 
+// -------------------------------------------------------------------------- distill
+struct Distill {
+    muon_train_distill_args a{};
+    Rows logits;
+    at::Tensor teacher, indices, labels, grad_loss;
+
+    Distill(const at::Tensor &logits_, const at::Tensor &teacher_, const at::Tensor &indices_,
+            const OptTensor &labels_, double temperature, double label_weight) {
+        TORCH_CHECK(logits_.device().is_cuda(), "distill_topk: logits must be a ROCm (HIP) device tensor");
+        TORCH_CHECK(logits_.dim() >= 1 && teacher_.dim() == logits_.dim() &&
+                        teacher_.sizes() == indices_.sizes(),
+                    "distill_topk: logits [.., V], teacher_logits and teacher_indices [.., K]");
+        for (int64_t i = 0; i + 1 < logits_.dim(); ++i)
+            TORCH_CHECK(teacher_.size(i) == logits_.size(i),
+                        "distill_topk: logits and teacher_logits must have the same rows");
+        logits = as_rows(logits_);
+        a.rows = logits.rows;
+        a.vocab = logits_.size(-1);
+        a.k = teacher_.size(-1);
+        a.ld_logits = logits.ld;
+        a.logits_dtype = dtype_of(logits_, "distill_topk: logits");
+        a.logits = logits.t.data_ptr();
+        auto on_device = [&](const at::Tensor &t, const char *what) {
+            TORCH_CHECK(t.device() == logits_.device(), "distill_topk: ", what, " is on another device");
+            return t.contiguous();
+        };
+        teacher = on_device(teacher_, "teacher_logits");
+        a.teacher_dtype = dtype_of(teacher, "distill_topk: teacher_logits");
+        a.teacher_logits = teacher.data_ptr();
+        indices = on_device(indices_, "teacher_indices");
+        TORCH_CHECK(indices.scalar_type() == at::kInt || indices.scalar_type() == at::kLong,
+                    "distill_topk: teacher_indices must be int32 or int64");
+        a.index_bytes = indices.scalar_type() == at::kInt ? 4 : 8;
+        a.teacher_indices = indices.data_ptr();
+        if (given(labels_)) {
+            labels = on_device(*labels_, "labels");
+            TORCH_CHECK(labels.scalar_type() == at::kLong && labels.numel() == a.rows,
+                        "distill_topk: labels must be int64, one a row");
+            a.labels = labels.data_ptr<int64_t>();
+        }
+        a.temperature = temperature;
+        a.label_weight = label_weight;
+    }
+    void set_grad_loss(const OptTensor &t, double value) {
+        a.grad_value = value;
+        if (!given(t)) return;
+        TORCH_CHECK(t->device() == logits.t.device() && t->scalar_type() == at::kFloat &&
+                        t->numel() == a.rows,
+                    "distill_topk: grad_loss must be float32, one a row");
+        grad_loss = t->contiguous();
+        a.grad_loss = grad_loss.data_ptr<float>();
+    }
+    at::Tensor per_row(const at::Tensor &like) const {
+        return at::empty(like.sizes().slice(0, like.dim() - 1), like.options().dtype(at::kFloat));
+    }
+};
+
+std::tuple<at::Tensor, at::Tensor> DistillForward(const at::Tensor &logits,
+                                                  const at::Tensor &teacher_logits,
+                                                  const at::Tensor &teacher_indices,
+                                                  const OptTensor &labels, double temperature,
+                                                  double label_weight, bool save) {
+    const c10::OptionalDeviceGuard device_guard(logits.device());
+    Distill d(logits, teacher_logits, teacher_indices, labels, temperature, label_weight);
+    at::Tensor loss = d.per_row(logits);
+    at::Tensor stats = at::empty({save ? d.a.rows : 0, 4}, loss.options());
+    d.a.loss = loss.data_ptr<float>();
+    if (save) d.a.stats = stats.data_ptr<float>();
+    const int st = muon_train_distill_forward(&d.a, stream_of(logits));
+    TORCH_CHECK(st == MUON_POLAR_OK, "distill_topk: ", muon_polar_last_error());
+    return {loss, stats};
+}
+
+at::Tensor DistillBackward(const at::Tensor &logits, const at::Tensor &teacher_logits,
+                           const at::Tensor &teacher_indices, const OptTensor &labels,
+                           double temperature, double label_weight, const at::Tensor &stats,
+                           const at::Tensor &grad_loss) {
+    const c10::OptionalDeviceGuard device_guard(logits.device());
+    Distill d(logits, teacher_logits, teacher_indices, labels, temperature, label_weight);
+    TORCH_CHECK(stats.is_contiguous() && stats.scalar_type() == at::kFloat &&
+                    stats.numel() == 4 * d.a.rows,
+                "distill_topk: stats of another forward pass");
+    d.set_grad_loss(grad_loss, 0.0);
+    at::Tensor grad = at::empty(logits.sizes(), logits.options());
+    d.a.stats = stats.data_ptr<float>();
+    d.a.grad = grad.data_ptr();
+    d.a.ld_grad = d.a.vocab;
+    const int st = muon_train_distill_backward(&d.a, stream_of(logits));
+    TORCH_CHECK(st == MUON_POLAR_OK, "distill_topk: ", muon_polar_last_error());
+    return grad;
+}
+
+// Loss, and the gradient into `grad`, which may be logits itself.
+at::Tensor DistillWithGrad(const at::Tensor &logits, const at::Tensor &teacher_logits,
+                           const at::Tensor &teacher_indices, const OptTensor &labels,
+                           double temperature, double label_weight, const OptTensor &grad_loss,
+                           double grad_value, const at::Tensor &grad) {
+    const c10::OptionalDeviceGuard device_guard(logits.device());
+    Distill d(logits, teacher_logits, teacher_indices, labels, temperature, label_weight);
+    TORCH_CHECK(grad.sizes() == logits.sizes() && grad.scalar_type() == logits.scalar_type() &&
+                    grad.device() == logits.device(),
+                "distill_topk: out must have the shape, dtype and device of logits");
+    d.set_grad_loss(grad_loss, grad_value);
+    const Rows out = as_rows(grad);
+    TORCH_CHECK(grad.numel() == 0 || out.t.data_ptr() == grad.data_ptr(),
+                "distill_topk: the rows of out must lie evenly apart, each unbroken");
+    at::Tensor loss = d.per_row(logits);
+    d.a.loss = loss.data_ptr<float>();
+    d.a.grad = out.t.data_ptr();
+    d.a.ld_grad = out.ld;
+    const int st = muon_train_distill_forward(&d.a, stream_of(logits));
+    TORCH_CHECK(st == MUON_POLAR_OK, "distill_topk: ", muon_polar_last_error());
+    return loss;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(muon_ascend950, m) {
@@ -193,9 +308,20 @@ TORCH_LIBRARY_FRAGMENT(muon_ascend950, m) {
           "int rows_per_sequence, bool post_norm, bool pre_norm, float eps, Tensor stats, "
           "Tensor? d_residual_out, Tensor? d_normed, int wanted) -> "
           "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+    m.def("distill_forward(Tensor logits, Tensor teacher_logits, Tensor teacher_indices, "
+          "Tensor? labels, float temperature, float label_weight, bool save) -> (Tensor, Tensor)");
+    m.def("distill_backward(Tensor logits, Tensor teacher_logits, Tensor teacher_indices, "
+          "Tensor? labels, float temperature, float label_weight, Tensor stats, "
+          "Tensor grad_loss) -> Tensor");
+    m.def("distill_with_grad(Tensor logits, Tensor teacher_logits, Tensor teacher_indices, "
+          "Tensor? labels, float temperature, float label_weight, Tensor? grad_loss, "
+          "float grad_value, Tensor(a!) grad) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(muon_ascend950, CUDA, m) {
     m.impl("norms_forward", &NormsForward);
     m.impl("norms_backward", &NormsBackward);
+    m.impl("distill_forward", &DistillForward);
+    m.impl("distill_backward", &DistillBackward);
+    m.impl("distill_with_grad", &DistillWithGrad);
 }

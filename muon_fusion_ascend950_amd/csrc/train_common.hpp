@@ -219,17 +219,26 @@ struct BlockSum {
         sum(v);
         return v[0];
     }
-    __device__ __forceinline__ float max(float a) {
-        a = wave_max(a);
-        if constexpr (NW == 1) return a;
-        const int wave = threadIdx.x >> 6;
-        if ((threadIdx.x & 63) == 0) red[turn][wave * N] = a;
-        __syncthreads();
-        float t = red[turn][0];
+    template <int K>
+    __device__ __forceinline__ void max(float (&v)[K]) {
+        static_assert(K <= N, "room for K values a wave");
 #pragma unroll
-        for (int w = 1; w < NW; ++w) t = fmaxf(t, red[turn][w * N]);
+        for (int k = 0; k < K; ++k) v[k] = wave_max(v[k]);
+        if constexpr (NW == 1) return;
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) red[turn][wave * N + k] = v[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float t = red[turn][k];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) t = fmaxf(t, red[turn][w * N + k]);
+            v[k] = t;
+        }
         turn ^= 1;
-        return t;
     }
 };
 

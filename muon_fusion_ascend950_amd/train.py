@@ -1,6 +1,8 @@
 """Operators of a training step around the Muon update, on hand-written gfx950 kernels.
 
-* ``block_norms`` — the norms before and after a block, with its gate and residual scale.
+* ``block_norms`` — the norms before and after a block, with its gate and residual scale;
+* ``distill_topk``, ``distill_topk_with_grad`` — the loss against a teacher's top logits,
+  and loss and gradient in one pass.
 
 ``muon_update`` starts from the gradients of a model's matrices; these are pieces of the
 forward and backward pass that produce them.  All take ROCm GPU tensors of float32 or
@@ -17,7 +19,7 @@ from ._loader import load_library
 
 load_library()
 
-__all__ = ["block_norms"]
+__all__ = ["block_norms", "distill_topk", "distill_topk_with_grad"]
 
 _ops = torch.ops.muon_ascend950
 _DTYPES = (torch.float32, torch.bfloat16)
@@ -148,3 +150,122 @@ def block_norms(y: torch.Tensor, residual: torch.Tensor, *, post_weight=None, ga
                                         kind, per_sequence, bool(post_norm), bool(pre_norm),
                                         float(eps), False)
     return out, (normed if pre_norm else None)
+
+
+# -------------------------------------------------------------------------- distillation
+_MAX_TOP = 1024
+
+
+class _DistillTopk(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher_logits, teacher_indices, labels, temperature, label_weight):
+        loss, stats = _ops.distill_forward(logits, teacher_logits, teacher_indices, labels,
+                                           temperature, label_weight, True)
+        ctx.save_for_backward(logits, teacher_logits, teacher_indices, labels, stats)
+        ctx.options = temperature, label_weight
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_loss):
+        logits, teacher_logits, teacher_indices, labels, stats = ctx.saved_tensors
+        grad = _ops.distill_backward(logits, teacher_logits, teacher_indices, labels,
+                                     *ctx.options, stats, grad_loss)
+        return grad, None, None, None, None, None
+
+
+def _check_distill(logits, teacher_logits, teacher_indices, temperature, labels, label_weight):
+    """Checks the operands; returns (labels or None, temperature, label weight)."""
+    _check_tensor("logits", logits)
+    _check_tensor("teacher_logits", teacher_logits, logits.device)
+    _check_tensor("teacher_indices", teacher_indices, logits.device, (torch.int32, torch.int64))
+    if logits.ndim < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits must have shape [..., V], got {tuple(logits.shape)}")
+    if (teacher_logits.ndim != logits.ndim or teacher_logits.shape[:-1] != logits.shape[:-1]
+            or teacher_indices.shape != teacher_logits.shape):
+        raise ValueError(
+            f"teacher_logits and teacher_indices must have shape {tuple(logits.shape[:-1])} + (K,), "
+            f"got {tuple(teacher_logits.shape)} and {tuple(teacher_indices.shape)}")
+    if not 1 <= teacher_logits.shape[-1] <= _MAX_TOP:
+        raise ValueError(f"K must be 1 to {_MAX_TOP}, got {teacher_logits.shape[-1]}")
+    temperature, label_weight = float(temperature), float(label_weight)
+    if not 0.0 < temperature < 1e30:
+        raise ValueError(f"temperature must be positive, got {temperature}")
+    if not 0.0 <= label_weight <= 1.0:
+        raise ValueError(f"label_weight must be 0 to 1, got {label_weight}")
+    if labels is None:
+        if label_weight != 0.0:
+            raise ValueError("label_weight needs labels")
+    else:
+        _check_tensor("labels", labels, logits.device, (torch.int64,))
+        if labels.shape != logits.shape[:-1]:
+            raise ValueError(f"labels must have shape {tuple(logits.shape[:-1])}, "
+                             f"got {tuple(labels.shape)}")
+        if label_weight == 0.0:
+            labels = None
+    return labels, temperature, label_weight
+
+
+def distill_topk(logits: torch.Tensor, teacher_logits: torch.Tensor,
+                 teacher_indices: torch.Tensor, *, temperature: float = 1.0, labels=None,
+                 label_weight: float = 0.0) -> torch.Tensor:
+    """Loss of each row of student logits against a teacher's top logits::
+
+        p = softmax(teacher_logits / temperature)       # over the row's K entries
+        q = softmax(logits / temperature)               # over the vocabulary
+        loss = (1 - label_weight) * temperature**2 * sum(p * (log p - log q[teacher_indices]))
+               + label_weight * cross_entropy(logits, labels)
+
+    logits ``[..., V]``, teacher_logits ``[..., K]`` (K at most 1024) float32 or bfloat16;
+    teacher_indices ``[..., K]`` int32 or int64; labels ``[...]`` int64.  Returns float32
+    ``[...]``, differentiable with respect to ``logits``.
+
+    An entry whose index is outside ``[0, V)`` is absent (rows with fewer than K entries are
+    filled with -1), and an absent entry's logit is not looked at.  A row without entries,
+    or whose entries are all -inf, has no first term and no gradient from it; a label
+    outside ``[0, V)`` (such as -100) leaves its row without the second.
+    """
+    labels, temperature, label_weight = _check_distill(
+        logits, teacher_logits, teacher_indices, temperature, labels, label_weight)
+    if _wants_grad(logits):
+        return _DistillTopk.apply(logits, teacher_logits, teacher_indices, labels, temperature,
+                                  label_weight)
+    return _ops.distill_forward(logits, teacher_logits, teacher_indices, labels, temperature,
+                                label_weight, False)[0]
+
+
+@torch.no_grad()
+def distill_topk_with_grad(logits: torch.Tensor, teacher_logits: torch.Tensor,
+                           teacher_indices: torch.Tensor, *, grad_loss=1.0,
+                           temperature: float = 1.0, labels=None, label_weight: float = 0.0,
+                           out=None):
+    """``distill_topk`` and its gradient in one pass over the logits.
+
+    Returns ``(loss, grad)`` with ``grad`` the gradient of ``sum(grad_loss * loss)`` with
+    respect to ``logits``, in their dtype, for ``logits.backward(grad)`` further down.
+    grad_loss: a number or float32 ``[...]`` (0 for tokens that do not count).  ``out``
+    receives the gradient; it may be ``logits`` itself, which is then overwritten.
+    """
+    labels, temperature, label_weight = _check_distill(
+        logits, teacher_logits, teacher_indices, temperature, labels, label_weight)
+    weight, value = None, 1.0
+    if isinstance(grad_loss, torch.Tensor):
+        _check_tensor("grad_loss", grad_loss, logits.device, (torch.float32,))
+        if grad_loss.shape != logits.shape[:-1]:
+            raise ValueError(f"grad_loss must have shape {tuple(logits.shape[:-1])}, "
+                             f"got {tuple(grad_loss.shape)}")
+        weight = grad_loss
+    else:
+        value = float(grad_loss)
+    if out is None:
+        grad = torch.empty_like(logits, memory_format=torch.contiguous_format)
+    else:
+        _check_tensor("out", out, logits.device, (logits.dtype,))
+        if out.shape != logits.shape:
+            raise ValueError(f"out must have shape {tuple(logits.shape)}, got {tuple(out.shape)}")
+        grad = out
+    loss = _ops.distill_with_grad(logits, teacher_logits, teacher_indices, labels, temperature,
+                                  label_weight, weight, value, grad)
+    if out is not None and not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+    return loss, grad

@@ -126,3 +126,91 @@ def test_norms_entry_checks_before_any_launch(change, message):
     assert message in capi.last_error()
     assert lib.muon_train_norms_forward(None, None) == capi.ERR_INVALID_ARGUMENT
     assert lib.muon_train_norms_forward(ctypes.byref(NormsArgs(**{**base, "rows": 0})), None) == capi.OK
+
+
+# ------------------------------------------------------------------------ distillation
+def _distill_ok(**change):
+    args = dict(logits=_cuda(2, 3, 50, dtype=B16), teacher_logits=_cuda(2, 3, 4),
+                teacher_indices=_cuda(2, 3, 4, dtype=torch.int32), temperature=2.0,
+                labels=_cuda(2, 3, dtype=torch.int64), label_weight=0.5)
+    args.update(change)
+    return [args.pop(n) for n in ("logits", "teacher_logits", "teacher_indices")], args
+
+
+@pytest.mark.parametrize("change,error,message", [
+    (lambda: dict(logits=1.0), TypeError, "torch.Tensor"),
+    (lambda: dict(logits=torch.zeros(2, 3, 50)), ValueError, "ROCm GPU"),
+    (lambda: dict(logits=_cuda(2, 3, 50, dtype=torch.float16)), TypeError, "logits"),
+    (lambda: dict(logits=_cuda(2, 3, 0)), ValueError, "logits"),
+    (lambda: dict(logits=_cuda(6, 50)), ValueError, "teacher_logits"),
+    (lambda: dict(logits=_cuda(2, 4, 50)), ValueError, "teacher_logits"),
+    (lambda: dict(teacher_indices=_cuda(2, 3, 5, dtype=torch.int32)), ValueError, "teacher_indices"),
+    (lambda: dict(teacher_indices=_cuda(2, 3, 4)), TypeError, "teacher_indices"),
+    (lambda: dict(teacher_logits=_cuda(2, 3, 1025), teacher_indices=_cuda(2, 3, 1025, dtype=torch.int32)),
+     ValueError, "1024"),
+    (lambda: dict(teacher_logits=_cuda(2, 3, 0), teacher_indices=_cuda(2, 3, 0, dtype=torch.int32)),
+     ValueError, "1024"),
+    (lambda: dict(temperature=0.0), ValueError, "temperature"),
+    (lambda: dict(temperature=float("nan")), ValueError, "temperature"),
+    (lambda: dict(temperature=float("inf")), ValueError, "temperature"),
+    (lambda: dict(label_weight=1.5), ValueError, "label_weight"),
+    (lambda: dict(labels=None), ValueError, "labels"),
+    (lambda: dict(labels=_cuda(2, dtype=torch.int64)), ValueError, "labels"),
+    (lambda: dict(labels=_cuda(2, 3, dtype=torch.int32)), TypeError, "labels"),
+])
+def test_distill_refuses(change, error, message):
+    with FakeTensorMode():
+        for call in (train.distill_topk, train.distill_topk_with_grad):
+            args, kw = _distill_ok(**change())
+            with pytest.raises(error, match=message):
+                call(*args, **kw)
+
+
+def test_distill_with_grad_refuses_and_fake():
+    with FakeTensorMode():
+        args, kw = _distill_ok()
+        with pytest.raises(ValueError, match="grad_loss"):
+            train.distill_topk_with_grad(*args, grad_loss=_cuda(6), **kw)
+        with pytest.raises(TypeError, match="grad_loss"):
+            train.distill_topk_with_grad(*args, grad_loss=_cuda(2, 3, dtype=B16), **kw)
+        with pytest.raises(TypeError, match="out"):
+            train.distill_topk_with_grad(*args, out=_cuda(2, 3, 50), **kw)
+        with pytest.raises(ValueError, match="out"):
+            train.distill_topk_with_grad(*args, out=_cuda(6, 50, dtype=B16), **kw)
+        loss, grad = train.distill_topk_with_grad(*args, **kw)
+        assert (loss.shape, loss.dtype) == ((2, 3), F32)
+        assert (grad.shape, grad.dtype) == ((2, 3, 50), B16)
+        args[0].requires_grad_(True)
+        loss = train.distill_topk(*args, **kw)
+        assert (loss.shape, loss.dtype, loss.requires_grad) == ((2, 3), F32, True)
+
+
+class DistillArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("rows", "vocab", "k", "ld_logits", "ld_grad")] + [
+        (n, ctypes.c_void_p) for n in ("logits", "teacher_logits", "teacher_indices", "labels", "grad_loss")] + [
+        (n, ctypes.c_double) for n in ("temperature", "label_weight", "grad_value")] + [
+        (n, ctypes.c_int) for n in ("logits_dtype", "teacher_dtype", "index_bytes")] + [
+        (n, ctypes.c_void_p) for n in ("loss", "stats", "grad")]
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(rows=-1), "rows"), (dict(vocab=0), "vocab"), (dict(vocab=1 << 31), "vocab"),
+    (dict(k=0), "k must"), (dict(k=1025), "k must"), (dict(logits_dtype=7), "dtypes"),
+    (dict(index_bytes=2), "indices"), (dict(temperature=-1.0), "temperature"),
+    (dict(label_weight=2.0), "label_weight"), (dict(logits=None), "null"),
+    (dict(ld_logits=9), "overlap"), (dict(ld_grad=9), "overlap"),
+    (dict(grad=(1 << 20) + 4), "overlap"), (dict(grad=1 << 20, ld_grad=11), "overlap"),
+    (dict(loss=None), "null output"),
+])
+def test_distill_entry_checks_before_any_launch(change, message):
+    lib = capi.load()
+    base = dict(rows=4, vocab=10, k=3, ld_logits=10, ld_grad=10, logits=1 << 20,
+                teacher_logits=1 << 21, teacher_indices=1 << 22, temperature=1.0, index_bytes=4,
+                loss=1 << 23, grad=1 << 24)
+    args = DistillArgs(**{**base, **change})
+    assert lib.muon_train_distill_forward(ctypes.byref(args), None) == capi.ERR_INVALID_ARGUMENT
+    assert message in capi.last_error()
+    no_stats = DistillArgs(**base)
+    assert lib.muon_train_distill_backward(ctypes.byref(no_stats), None) == capi.ERR_INVALID_ARGUMENT
+    assert lib.muon_train_distill_forward(None, None) == capi.ERR_INVALID_ARGUMENT
+    assert lib.muon_train_distill_forward(ctypes.byref(DistillArgs(**{**base, "rows": 0})), None) == capi.OK
