@@ -4,6 +4,7 @@
  *
  *   norms    the norms before and after a block, with its gate and residual scale
  *   distill  the loss against a teacher's top logits
+ *   fp8      products in 8-bit floating point with a scale for each block of 128
  *
  * All functions are asynchronous on the given HIP stream.  Pointers are device pointers
  * unless said otherwise; structs are read during the call only.  No function allocates
@@ -110,6 +111,49 @@ typedef struct muon_train_distill_args {
 int muon_train_distill_forward(const muon_train_distill_args *args, hipStream_t stream);
 /* grad from the stats of a forward pass. */
 int muon_train_distill_backward(const muon_train_distill_args *args, hipStream_t stream);
+
+/* --------------------------------------------------------------------- fp8
+ * A matrix [rows, cols] held as e4m3 values (OCP, no infinities, largest 448) and one fp32
+ * scale for each block of block_rows x 128 elements, block_rows 1 (activations and
+ * gradients) or 128 (weights):
+ *
+ *     s = max(amax·(1/448), 2^-126)       amax: largest |x| of the block
+ *     value = round_to_nearest_even_e4m3(x·(1/s))
+ *
+ * in fp32 (1/448 the nearest fp32).  A block with an infinity or a NaN has no finite
+ * element back.  The rows of values lie `ld` bytes apart, a multiple of 128 at least cols,
+ * and are zero past cols.  Scale (i, j), of row block i and column block j, is at
+ * scales[i·scale_row + j·scale_col]. */
+typedef struct muon_train_fp8_quantize_args {
+    int64_t rows, cols, ld_x; /* elements from row to row of x (>= cols) */
+    const void *x;
+    int x_dtype, block_rows;
+    void *values;    /* [rows, roundup(cols, 128)], or null */
+    float *scales;   /* block_rows 1: [ceil(cols / 128)][rows] (scale_row 1);
+                        block_rows 128: [ceil(rows / 128)][ceil(cols / 128)] */
+    void *values_t;  /* of the transposed matrix: [cols, roundup(rows, 128)], or null */
+    float *scales_t; /* block_rows 1: [ceil(rows / 128)][cols]; block_rows 128: the
+                        transposed matrix's scales are the same ones, scales with scale_row
+                        and scale_col changed over (scales_t unused, scales written) */
+} muon_train_fp8_quantize_args;
+int muon_train_fp8_quantize(const muon_train_fp8_quantize_args *args, hipStream_t stream);
+
+/* c[m][n] = Σ_blocks a_scale·b_scale·Σ_{k in block} a[m][k]·b[n][k], both operands with k
+ * running along their rows: products of values and their sums in fp32, rounded once. */
+typedef struct muon_train_fp8_operand {
+    const void *values; /* [rows, k], 16-byte aligned */
+    const float *scales;
+    int64_t ld, scale_row, scale_col;
+    int block_rows; /* 1 (scale_row must be 1) or 128 */
+} muon_train_fp8_operand;
+typedef struct muon_train_fp8_matmul_args {
+    int64_t m, n, k; /* k a multiple of 128 (values padded with zeros); 0: c is zeros */
+    muon_train_fp8_operand a, b;
+    void *c; /* [m, n] */
+    int64_t ldc;
+    int c_dtype;
+} muon_train_fp8_matmul_args;
+int muon_train_fp8_matmul(const muon_train_fp8_matmul_args *args, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -97,7 +97,43 @@ def load_library() -> None:
                                label_weight, grad_loss, grad_value, grad):
         return logits.new_empty(logits.shape[:-1], dtype=torch.float32)
 
-    for name, fake in (("muon_ascend950::distill_forward", fake_distill_forward),
+    def held(like, rows, cols, block_rows):
+        kb = -(-cols // 128)
+        scales = (like.new_empty((kb, rows), dtype=torch.float32).t() if block_rows == 1 else
+                  like.new_empty((-(-rows // 128), kb), dtype=torch.float32))
+        return like.new_empty((rows, kb * 128), dtype=torch.float8_e4m3fn), scales
+
+    def fake_quantize_fp8(x, block_rows):
+        return held(x, x.shape[0], x.shape[1], block_rows)
+
+    def fake_fp8_matmul(a, a_scales, b, b_scales, dtype):
+        return a.new_empty((a.shape[0], b.shape[0]), dtype=dtype)
+
+    def fake_fp8_linear(x, values, scales):
+        return x.new_empty((*x.shape[:-1], values.shape[0]))
+
+    def fake_fp8_linear_forward(x, weight, save):
+        n, k = weight.shape
+        none = x.new_empty((0,)), x.new_empty((0,))
+        xt = held(x, k, x.numel() // k, 1) if save & 1 else none
+        wt = held(x, k, n, 128) if save & 2 else none
+        if save & 2:  # a view of the weight's own scales
+            wt = wt[0], wt[1].new_empty(wt[1].shape[::-1]).t()
+        return (x.new_empty((*x.shape[:-1], n)), *xt, *wt)
+
+    def fake_fp8_linear_backward(dy, xt_values, xt_scales, wt_values, wt_scales, weight_dtype,
+                                 wanted):
+        dx = dy.new_empty((*dy.shape[:-1], wt_values.shape[0]) if wanted & 1 else (0,))
+        dw = dy.new_empty((dy.shape[-1], xt_values.shape[0]) if wanted & 2 else (0,),
+                          dtype=weight_dtype if wanted & 2 else dy.dtype)
+        return dx, dw
+
+    for name, fake in (("muon_ascend950::quantize_fp8", fake_quantize_fp8),
+                       ("muon_ascend950::fp8_matmul", fake_fp8_matmul),
+                       ("muon_ascend950::fp8_linear", fake_fp8_linear),
+                       ("muon_ascend950::fp8_linear_forward", fake_fp8_linear_forward),
+                       ("muon_ascend950::fp8_linear_backward", fake_fp8_linear_backward),
+                       ("muon_ascend950::distill_forward", fake_distill_forward),
                        ("muon_ascend950::distill_backward", fake_distill_backward),
                        ("muon_ascend950::distill_with_grad", fake_distill_with_grad),
                        ("muon_ascend950::norms_forward", fake_norms_forward),

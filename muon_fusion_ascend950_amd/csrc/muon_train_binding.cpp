@@ -296,6 +296,177 @@ at::Tensor DistillWithGrad(const at::Tensor &logits, const at::Tensor &teacher_l
     return loss;
 }
 
+// ------------------------------------------------------------------------------ fp8
+constexpr int64_t kBlock = 128;
+int64_t blocks(int64_t n) { return (n + kBlock - 1) / kBlock; }
+
+// A matrix held as e4m3 values [rows, blocks(cols) * 128] and scales
+// [rows or blocks(rows), blocks(cols)].
+struct Held {
+    at::Tensor values, scales;
+};
+Held empty_held(const at::Tensor &like, int64_t rows, int64_t cols, int64_t block_rows) {
+    const auto f32 = like.options().dtype(at::kFloat);
+    Held h;
+    h.values = at::empty({rows, blocks(cols) * kBlock}, like.options().dtype(at::kFloat8_e4m3fn));
+    h.scales = block_rows == 1 ? at::empty({blocks(cols), rows}, f32).t()
+                               : at::empty({blocks(rows), blocks(cols)}, f32);
+    return h;
+}
+
+// x as held values, and the transposed x, as wanted.
+void quantize(const at::Tensor &x, int64_t block_rows, Held *plain, Held *turned) {
+    TORCH_CHECK(x.device().is_cuda() && x.dim() == 2, "fp8: a matrix on a ROCm (HIP) device is needed");
+    const Rows r = as_rows(x);
+    const int64_t rows = x.size(0), cols = x.size(1);
+    muon_train_fp8_quantize_args a{};
+    a.rows = rows;
+    a.cols = cols;
+    a.ld_x = r.ld;
+    a.x = r.t.data_ptr();
+    a.x_dtype = dtype_of(x, "fp8: a matrix to quantise");
+    a.block_rows = static_cast<int>(block_rows);
+    if (plain || (block_rows != 1 && turned)) {
+        Held h = empty_held(x, plain ? rows : 0, cols, block_rows);
+        if (!plain) h.scales = at::empty({blocks(rows), blocks(cols)}, h.scales.options());
+        if (plain) a.values = h.values.data_ptr();
+        a.scales = h.scales.data_ptr<float>();
+        if (plain) *plain = h;
+        if (turned && block_rows != 1) turned->scales = h.scales.t();
+    }
+    if (turned) {
+        if (block_rows == 1) {
+            *turned = empty_held(x, cols, rows, 1);
+            a.scales_t = turned->scales.data_ptr<float>();
+        } else {
+            turned->values = at::empty({cols, blocks(rows) * kBlock},
+                                       x.options().dtype(at::kFloat8_e4m3fn));
+        }
+        a.values_t = turned->values.data_ptr();
+    }
+    const int st = muon_train_fp8_quantize(&a, stream_of(x));
+    TORCH_CHECK(st == MUON_POLAR_OK, "fp8: ", muon_polar_last_error());
+}
+
+muon_train_fp8_operand operand(Held &h, const at::Tensor &like) {
+    TORCH_CHECK(h.values.device() == like.device() && h.scales.device() == like.device(),
+                "fp8: operands must be on one device");
+    TORCH_CHECK(h.values.dim() == 2 && h.values.scalar_type() == at::kFloat8_e4m3fn &&
+                    h.values.size(1) % kBlock == 0,
+                "fp8: values must be float8_e4m3fn [rows, a multiple of 128]");
+    const int64_t rows = h.values.size(0), kb = h.values.size(1) / kBlock;
+    TORCH_CHECK(h.scales.dim() == 2 && h.scales.scalar_type() == at::kFloat &&
+                    h.scales.size(1) == kb &&
+                    (h.scales.size(0) == rows || h.scales.size(0) == blocks(rows)),
+                "fp8: scales must be float32 [rows or ceil(rows / 128), cols / 128]");
+    if (h.values.stride(1) != 1 || h.values.stride(0) % 16 != 0 ||
+        h.values.stride(0) < h.values.size(1) ||
+        reinterpret_cast<uintptr_t>(h.values.data_ptr()) % 16 != 0)
+        h.values = h.values.clone(at::MemoryFormat::Contiguous);
+    muon_train_fp8_operand o{};
+    o.block_rows = h.scales.size(0) == rows ? 1 : static_cast<int>(kBlock);
+    if (o.block_rows == 1 && rows > 1 && (h.scales.stride(0) != 1 || h.scales.stride(1) < rows))
+        h.scales = h.scales.t().contiguous().t();
+    o.values = h.values.data_ptr();
+    o.scales = h.scales.data_ptr<float>();
+    o.ld = h.values.stride(0);
+    o.scale_row = o.block_rows == 1 ? 1 : h.scales.stride(0);
+    o.scale_col = h.scales.stride(1);
+    return o;
+}
+
+// c [m, n] = a · bᵀ
+void matmul(Held a, Held b, at::Tensor &c) {
+    muon_train_fp8_matmul_args g{};
+    g.a = operand(a, c);
+    g.b = operand(b, c);
+    TORCH_CHECK(a.values.size(1) == b.values.size(1), "fp8: operands of different width");
+    g.m = c.size(0);
+    g.n = c.size(1);
+    g.k = a.values.size(1);
+    TORCH_CHECK(g.m == a.values.size(0) && g.n == b.values.size(0), "fp8: result of another shape");
+    g.c = c.data_ptr();
+    g.ldc = g.n;
+    g.c_dtype = dtype_of(c, "fp8: the result");
+    const int st = muon_train_fp8_matmul(&g, stream_of(c));
+    TORCH_CHECK(st == MUON_POLAR_OK, "fp8: ", muon_polar_last_error());
+}
+
+std::tuple<at::Tensor, at::Tensor> QuantizeFp8(const at::Tensor &x, int64_t block_rows) {
+    const c10::OptionalDeviceGuard device_guard(x.device());
+    Held h;
+    quantize(x, block_rows, &h, nullptr);
+    return {h.values, h.scales};
+}
+
+at::Tensor Fp8Matmul(const at::Tensor &a, const at::Tensor &a_scales, const at::Tensor &b,
+                     const at::Tensor &b_scales, at::ScalarType dtype) {
+    const c10::OptionalDeviceGuard device_guard(a.device());
+    at::Tensor c = at::empty({a.size(0), b.size(0)}, a.options().dtype(dtype));
+    matmul({a, a_scales}, {b, b_scales}, c);
+    return c;
+}
+
+at::Tensor as_matrix(const at::Tensor &x) {
+    return x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+}
+at::Tensor result_like(const at::Tensor &x, int64_t n) {
+    auto sizes = x.sizes().vec();
+    sizes.back() = n;
+    return at::empty(sizes, x.options());
+}
+
+// y = x · wᵀ on a held weight.
+at::Tensor Fp8Linear(const at::Tensor &x, const at::Tensor &values, const at::Tensor &scales) {
+    const c10::OptionalDeviceGuard device_guard(x.device());
+    Held h;
+    quantize(as_matrix(x), 1, &h, nullptr);
+    at::Tensor y = result_like(x, values.size(0));
+    at::Tensor y2 = y.view({h.values.size(0), values.size(0)});
+    matmul(h, {values, scales}, y2);
+    return y;
+}
+
+// y = x · weightᵀ, and what the backward pass needs: the transposed x along the tokens
+// (save & 1, for the weight's gradient) and the transposed weight (save & 2, for x's).
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> Fp8LinearForward(
+    const at::Tensor &x, const at::Tensor &weight, int64_t save) {
+    const c10::OptionalDeviceGuard device_guard(x.device());
+    Held xq, xt, wq, wt;
+    quantize(as_matrix(x), 1, &xq, (save & 1) ? &xt : nullptr);
+    quantize(weight, kBlock, &wq, (save & 2) ? &wt : nullptr);
+    at::Tensor y = result_like(x, weight.size(0));
+    at::Tensor y2 = y.view({xq.values.size(0), weight.size(0)});
+    matmul(xq, wq, y2);
+    for (Held *h : {&xt, &wt})
+        if (!h->values.defined()) h->values = h->scales = none(x);
+    return {y, xt.values, xt.scales, wt.values, wt.scales};
+}
+
+// Gradients of x (with the saved transposed weight) and of the weight (with the saved
+// transposed x), as wanted (1: x, 2: weight).
+std::tuple<at::Tensor, at::Tensor> Fp8LinearBackward(const at::Tensor &dy, const at::Tensor &xt_values,
+                                                     const at::Tensor &xt_scales,
+                                                     const at::Tensor &wt_values,
+                                                     const at::Tensor &wt_scales,
+                                                     at::ScalarType weight_dtype, int64_t wanted) {
+    const c10::OptionalDeviceGuard device_guard(dy.device());
+    Held g, gt;
+    const at::Tensor dy2 = as_matrix(dy);
+    quantize(dy2, 1, (wanted & 1) ? &g : nullptr, (wanted & 2) ? &gt : nullptr);
+    at::Tensor dx = none(dy), dw = none(dy);
+    if (wanted & 1) {
+        dx = result_like(dy, wt_values.size(0));
+        at::Tensor dx2 = dx.view({dy2.size(0), wt_values.size(0)});
+        matmul(g, {wt_values, wt_scales}, dx2);
+    }
+    if (wanted & 2) {
+        dw = at::empty({dy2.size(1), xt_values.size(0)}, dy.options().dtype(weight_dtype));
+        matmul(gt, {xt_values, xt_scales}, dw);
+    }
+    return {dx, dw};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(muon_ascend950, m) {
@@ -316,6 +487,14 @@ TORCH_LIBRARY_FRAGMENT(muon_ascend950, m) {
     m.def("distill_with_grad(Tensor logits, Tensor teacher_logits, Tensor teacher_indices, "
           "Tensor? labels, float temperature, float label_weight, Tensor? grad_loss, "
           "float grad_value, Tensor(a!) grad) -> Tensor");
+    m.def("quantize_fp8(Tensor x, int block_rows) -> (Tensor, Tensor)");
+    m.def("fp8_matmul(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales, ScalarType dtype) -> "
+          "Tensor");
+    m.def("fp8_linear(Tensor x, Tensor values, Tensor scales) -> Tensor");
+    m.def("fp8_linear_forward(Tensor x, Tensor weight, int save) -> "
+          "(Tensor, Tensor, Tensor, Tensor, Tensor)");
+    m.def("fp8_linear_backward(Tensor dy, Tensor xt_values, Tensor xt_scales, Tensor wt_values, "
+          "Tensor wt_scales, ScalarType weight_dtype, int wanted) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(muon_ascend950, CUDA, m) {
@@ -324,4 +503,9 @@ TORCH_LIBRARY_IMPL(muon_ascend950, CUDA, m) {
     m.impl("distill_forward", &DistillForward);
     m.impl("distill_backward", &DistillBackward);
     m.impl("distill_with_grad", &DistillWithGrad);
+    m.impl("quantize_fp8", &QuantizeFp8);
+    m.impl("fp8_matmul", &Fp8Matmul);
+    m.impl("fp8_linear", &Fp8Linear);
+    m.impl("fp8_linear_forward", &Fp8LinearForward);
+    m.impl("fp8_linear_backward", &Fp8LinearBackward);
 }

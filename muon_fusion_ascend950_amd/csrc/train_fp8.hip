@@ -1,0 +1,501 @@
+// train_fp8.hip — e4m3 values with a scale for each block of 128, and products of matrices
+// held so (include/muon_train.h; the formulas are there).
+#include "train_common.hpp"
+
+namespace muon_train {
+
+namespace {
+
+using muon_polar::f32x4;
+using muon_polar::u32x2;
+using i32x8 = int32_t __attribute__((ext_vector_type(8)));
+using muon_polar::i32x4;
+
+constexpr int kBlock = 128;
+
+// ------------------------------------------------------------------------- quantising
+// One workgroup takes a tile of 128 x 128 elements: thread t the rows 8·(t / 16) .. + 7 and
+// the columns 8·(t % 16) .. + 7.  Magnitudes are compared as integers, which orders NaN
+// above the infinities and those above all numbers, so that either reaches the scale.
+constexpr int kQuantThreads = 256;
+constexpr int kTilePitch = kBlock + 16;  // bytes from column to column of the turned tile
+
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+template <int kCtrl>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
+    return __builtin_amdgcn_update_dpp(v, v, kCtrl, 0xf, 0xf, false);
+}
+// Over the 16 lanes of a row of the wave.
+__device__ __forceinline__ uint32_t row_umax(uint32_t v) {
+    v = umax(v, dpp_u32<kQuadXor1>(v));
+    v = umax(v, dpp_u32<kQuadXor2>(v));
+    v = umax(v, dpp_u32<kRowHalfMirror>(v));
+    return umax(v, dpp_u32<kRowMirror>(v));
+}
+__device__ __forceinline__ float scale_of(uint32_t amax) {
+    const float s = __uint_as_float(amax) * (1.0f / 448.0f);
+    return s >= 0x1p-126f || s != s ? s : 0x1p-126f;
+}
+// Eight values as e4m3, in order.
+__device__ __forceinline__ u32x2 to_fp8(const float (&f)[8], const float (&inv)[8]) {
+    int lo = 0, hi = 0;
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0] * inv[0], f[1] * inv[1], lo, false);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[2] * inv[2], f[3] * inv[3], lo, true);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[4] * inv[4], f[5] * inv[5], hi, false);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[6] * inv[6], f[7] * inv[7], hi, true);
+    return u32x2{uint32_t(lo), uint32_t(hi)};
+}
+
+using QuantArgs = muon_train_fp8_quantize_args;
+
+template <class T, int kRows>
+__global__ __launch_bounds__(kQuantThreads) void quantize_kernel(QuantArgs a, int col_tiles) {
+    using Raw = typename T::Raw;
+    __shared__ uint32_t col_max[4][kBlock];
+    __shared__ uint8_t turned[kBlock * kTilePitch];
+    const int tid = threadIdx.x, wave = tid >> 6;
+    const int64_t tile_r = blockIdx.x / col_tiles, tile_c = blockIdx.x % col_tiles;
+    const int64_t row0 = tile_r * kBlock + 8 * (tid >> 4), col0 = tile_c * kBlock + 8 * (tid & 15);
+    const int64_t padded_cols = int64_t(col_tiles) * kBlock;
+    const int64_t padded_rows = (a.rows + kBlock - 1) / kBlock * kBlock;
+    const int64_t left = a.cols - col0;
+    const int valid = left < 0 ? 0 : left > 8 ? 8 : int(left);
+
+    float x[8][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        Piece<T> p;
+        if (row0 + i < a.rows)
+            p.load(static_cast<const Raw *>(a.x) + (row0 + i) * a.ld_x + col0, valid);
+        else
+            p.zero();
+        p.get(x[i]);
+    }
+    float inv[8];
+    if constexpr (kRows == 1) {
+        if (a.values) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m = umax(m, magnitude(x[i][e]));
+                const float s = scale_of(row_umax(m)), r = 1.0f / s;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) inv[e] = r;
+                if (row0 + i < a.rows) {
+                    const u32x2 q = to_fp8(x[i], inv);
+                    __builtin_memcpy(static_cast<uint8_t *>(a.values) + (row0 + i) * padded_cols + col0, &q, 8);
+                    if ((tid & 15) == 0) a.scales[tile_c * a.rows + row0 + i] = s;
+                }
+            }
+        }
+        if (!a.values_t) return;
+    }
+    // magnitudes of the columns (of the whole tile: blocks of 128 rows)
+    uint32_t cm[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = umax(m, magnitude(x[i][e]));
+        m = umax(m, __shfl_xor(m, 16));
+        cm[e] = umax(m, __shfl_xor(m, 32));
+    }
+    if constexpr (kRows == kBlock) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = umax(m, cm[e]);
+        m = row_umax(m);
+        if ((tid & 63) == 0) col_max[wave][0] = m;
+        __syncthreads();
+        m = umax(umax(col_max[0][0], col_max[1][0]), umax(col_max[2][0], col_max[3][0]));
+        const float s = scale_of(m), r = 1.0f / s;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) inv[e] = r;
+        if (tid == 0) a.scales[tile_r * col_tiles + tile_c] = s;
+        if (a.values) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (row0 + i < a.rows) {
+                    const u32x2 q = to_fp8(x[i], inv);
+                    __builtin_memcpy(static_cast<uint8_t *>(a.values) + (row0 + i) * padded_cols + col0, &q, 8);
+                }
+        }
+        if (!a.values_t) return;
+    } else {
+        if ((tid & 63) < 16) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) col_max[wave][8 * (tid & 15) + e] = cm[e];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int c = 8 * (tid & 15) + e;
+            const uint32_t m = umax(umax(col_max[0][c], col_max[1][c]), umax(col_max[2][c], col_max[3][c]));
+            const float s = scale_of(m);
+            inv[e] = 1.0f / s;
+            if ((tid >> 4) == 0 && col0 + e < a.cols) a.scales_t[tile_r * a.cols + col0 + e] = s;
+        }
+    }
+    // the tile turned: eight rows of a column are eight bytes in a line
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float f[8], r[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = x[i][e], r[i] = inv[e];
+        const u32x2 q = to_fp8(f, r);
+        *reinterpret_cast<u32x2 *>(turned + (8 * (tid & 15) + e) * kTilePitch + 8 * (tid >> 4)) = q;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int pass = 0; pass < 4; ++pass) {
+        const int c = 32 * pass + (tid >> 3), b = 16 * (tid & 7);
+        const int64_t col = tile_c * kBlock + c;
+        if (col < a.cols)
+            *reinterpret_cast<u32x4 *>(static_cast<uint8_t *>(a.values_t) + col * padded_rows +
+                                       tile_r * kBlock + b) =
+                *reinterpret_cast<const u32x4 *>(turned + c * kTilePitch + b);
+    }
+    // The check of store-data hazards reads the code in address order, past the program's
+    // end: two wait states keep it from pairing the last store with the block laid out there.
+    asm volatile("s_nop 1");
+}
+
+// -------------------------------------------------------------------------- products
+// v_mfma_f32_16x16x128_f8f6f4 on e4m3 values: lane l supplies 32 consecutive values (k-part
+// l / 16 of the 128) of row l % 16 of A and of column l % 16 of B, and receives
+// D[4·(l / 16) + j][l % 16], j = 0 .. 3.
+__device__ __forceinline__ f32x4 mfma_fp8(i32x8 a, i32x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+}
+
+using MatmulArgs = muon_train_fp8_matmul_args;
+
+// The fp8 MFMAs do not keep 32 bits of the products they add: measured against 64 bits,
+// results are off by 1.5e-5 to 2.7e-5 of their 2-norm, in chains of 16x16x32 as in single
+// 16x16x128 instructions.  Beside bf16's rounding (2^-9) that is nothing, and results that
+// leave as bf16 take them.  Results kept in fp32 (kExact) take the bf16 MFMA on the same
+// values, which bf16 holds exactly: 1e-7, at half the rate.
+using bf16x2 = __bf16 __attribute__((ext_vector_type(2)));
+using muon_polar::bf16x8;
+__device__ __forceinline__ bf16x8 to_bf16(uint32_t lo, uint32_t hi) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
+    const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
+    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// 16 rows of 128 K-values of an operand as a lane holds them.
+template <bool kExact>
+struct Frag {
+    i32x8 v;
+    __device__ __forceinline__ void set(i32x8 x) { v = x; }
+};
+template <>
+struct Frag<true> {
+    bf16x8 v[4];
+    __device__ __forceinline__ void set(i32x8 x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = to_bf16(x[2 * i], x[2 * i + 1]);
+    }
+};
+__device__ __forceinline__ f32x4 multiply(const Frag<false> &a, const Frag<false> &b) {
+    return mfma_fp8(a.v, b.v, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+}
+__device__ __forceinline__ f32x4 multiply(const Frag<true> &a, const Frag<true> &b) {
+    f32x4 t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t = muon_polar::mfma_16x16x32(a.v[i], b.v[i], t);
+    return t;
+}
+
+// 4 B per lane from rsrc + voffset into LDS at lds_base (wave-uniform) + 4·lane (see
+// dma_16B for the wait state).
+__device__ __forceinline__ void dma_4B(muon_polar::i32x4 rsrc, uint32_t lds_base, uint32_t voffset) {
+    asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
+                 :
+                 : "v"(voffset), "s"(rsrc), "{m0}"(__builtin_amdgcn_readfirstlane(lds_base))
+                 : "memory");
+}
+
+// Four consecutive results of a row, the first `count` of them inside the matrix.
+__device__ __forceinline__ void store4(void *c, int64_t at, int count, int dtype, f32x4 v) {
+    if (dtype == MUON_TRAIN_BF16) {
+        uint16_t *p = static_cast<uint16_t *>(c) + at;
+        const u32x2 w{f32_to_bf16_bits(v[0]) | uint32_t(f32_to_bf16_bits(v[1])) << 16,
+                      f32_to_bf16_bits(v[2]) | uint32_t(f32_to_bf16_bits(v[3])) << 16};
+        if (count >= 4) {
+            __builtin_memcpy(p, &w, 8);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+                if (e < count) p[e] = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
+        }
+    } else {
+        float *p = static_cast<float *>(c) + at;
+        if (count >= 4) {
+            __builtin_memcpy(p, &v, 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+                if (e < count) p[e] = v[e];
+        }
+    }
+}
+
+// Tile of a launch: workgroup w runs on XCD w % 8, and each XCD takes a run of tiles next
+// to each other (columns of kGroup row tiles, walked column by column), which share operand
+// panels in its L2.
+constexpr int kGroup = 8;
+__device__ __forceinline__ void tile_of(int w, int tiles_m, int tiles_n, int &tm, int &tn) {
+    const int total = tiles_m * tiles_n, each = total / 8, more = total % 8;
+    const int xcd = w % 8, first = xcd * each + (xcd < more ? xcd : more);
+    const int t = first + w / 8;
+    const int group = t / (kGroup * tiles_n), in = t % (kGroup * tiles_n);
+    const int high = tiles_m - group * kGroup < kGroup ? tiles_m - group * kGroup : kGroup;
+    tm = group * kGroup + in % high;
+    tn = in / high;
+}
+
+// A tile of BM x BN outputs, waves of WM x WN.  K runs in steps of one block of 128: the
+// step's panels (rows of 128 bytes) and scales come to LDS by DMA, D steps in a ring, so
+// that step k + D - 1 streams in while step k is multiplied.  A row's 16-byte chunk c lies
+// at place c ^ ((row >> 1) & 7): the 16 rows of a fragment read meet 16 different places of
+// the 256-byte bank window.
+//
+// The operand b, whose rows are output columns, is the MFMA's A side: a lane then holds
+// four consecutive columns of one output row, and a's scale is one number a lane.  Each
+// step's product starts from zero and is added to the fp32 sums times a_scale·b_scale: four
+// fused multiply-adds a lane beside each MFMA (16 against its 32 clocks).
+template <int BM, int BN, int WM, int WN, int D>
+struct Geometry {
+    static constexpr int kWaves = (BM / WM) * (BN / WN), kThreads = 64 * kWaves;
+    static constexpr int kPanels = (BM + BN) * kBlock;  // bytes of a step
+    static constexpr int kSlot = kPanels + (BM + BN) * 4;
+    static constexpr int kLoads = kPanels / 1024 / kWaves;  // 1 KiB DMA instructions of a wave
+    static constexpr int kScaleLoads = (BM + BN) / 64;      // 256 B ones of the workgroup
+    static_assert(kPanels % (1024 * kWaves) == 0 && BM % 64 == 0 && BN % 64 == 0, "whole DMA blocks");
+    static_assert(kScaleLoads <= kWaves, "one scale load a wave");
+    static_assert((D - 1) * (kLoads + 1) <= 63, "vmcnt range");
+    static_assert(D * kSlot <= 160 * 1024, "LDS");
+};
+
+template <int BM, int BN, int WM, int WN, int D, bool kExact, bool kRowB>
+__global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmul_kernel(
+    MatmulArgs g, int tiles_m, int tiles_n) {
+    using Geo = Geometry<BM, BN, WM, WN, D>;
+    constexpr int SM = WM / 16, SN = WN / 16, kLoads = Geo::kLoads;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[D * Geo::kSlot];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+    int tm, tn;
+    tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+    const int64_t m0 = int64_t(tm) * BM, n0 = int64_t(tn) * BN;
+    const int rows_m = g.m - m0 < BM ? int(g.m - m0) : BM;
+    const int rows_n = g.n - n0 < BN ? int(g.n - n0) : BN;
+    const int steps = static_cast<int>(g.k / kBlock);
+
+    // DMA: instruction d of this wave moves rows 8·(wave·kLoads + d) .. + 7 of the step's
+    // BM + BN panel rows; rows outside the matrices read as zeros.
+    const auto rs_a = muon_polar::make_buffer_rsrc(static_cast<const uint8_t *>(g.a.values) + m0 * g.a.ld,
+                                                   static_cast<uint32_t>(rows_m * g.a.ld));
+    const auto rs_b = muon_polar::make_buffer_rsrc(static_cast<const uint8_t *>(g.b.values) + n0 * g.b.ld,
+                                                   static_cast<uint32_t>(rows_n * g.b.ld));
+    uint32_t off[kLoads];
+#pragma unroll
+    for (int d = 0; d < kLoads; ++d) {
+        const int row = 8 * (wave * kLoads + d) + (lane >> 3);
+        const int chunk = (lane & 7) ^ ((row >> 1) & 7);
+        const bool is_a = row < BM;
+        const int at = is_a ? row : row - BM;
+        off[d] = at < (is_a ? rows_m : rows_n)
+                     ? static_cast<uint32_t>(at * (is_a ? g.a.ld : g.b.ld) + 16 * chunk)
+                     : muon_polar::kOob;
+    }
+    // scales: 64 rows' worth of the step's BM + BN, one each (rows past the end: the last's)
+    const int sblock = wave % Geo::kScaleLoads;
+    const bool scale_a = sblock * 64 < BM;
+    const muon_train_fp8_operand &so = scale_a ? g.a : g.b;
+    const int srow = (scale_a ? sblock * 64 : sblock * 64 - BM) + lane;
+    const int64_t sfirst = scale_a ? m0 : n0;
+    const int slast = (scale_a ? rows_m : rows_n) - 1;
+    const int64_t sat = sfirst + (srow < slast ? srow : slast);
+    const uint32_t soff = static_cast<uint32_t>(
+        4 * ((so.block_rows == 1 ? sat : sat / kBlock) - (so.block_rows == 1 ? sfirst : sfirst / kBlock)) *
+        so.scale_row);
+    const float *sbase = so.scales + (so.block_rows == 1 ? sfirst : sfirst / kBlock) * so.scale_row;
+    const int64_t sstep = so.scale_col;
+
+    const uint32_t lds0 = muon_polar::lds_addr(smem);
+    auto issue = [&](int d, int step, int slot) {
+        const uint32_t base = lds0 + slot * Geo::kSlot;
+        if (d < kLoads) {
+            const int row0 = 8 * (wave * kLoads + d);
+            const uint32_t at = step < steps ? off[d] + step * kBlock : muon_polar::kOob;
+            // a row outside the matrix stays outside: kOob + k is past every buffer
+            muon_polar::dma_16B(row0 < BM ? rs_a : rs_b, base + row0 * kBlock, at);
+        } else {
+            const int s = step < steps ? step : steps - 1;
+            const auto rs = muon_polar::make_buffer_rsrc(sbase + s * sstep, 0x7ffffffcu);
+            dma_4B(rs, base + Geo::kPanels + sblock * 256, soff);
+        }
+    };
+
+    const int wm = (wave % (BM / WM)) * WM, wn = (wave / (BM / WM)) * WN;
+    const int r = lane & 15, part = lane >> 4;
+    const int lane_at = r * kBlock + (((2 * part) ^ ((r >> 1) & 7)) << 4);
+    auto fragment = [&](const uint8_t *panel) {
+        const i32x4 lo = *reinterpret_cast<const i32x4 *>(panel + lane_at);
+        const i32x4 hi = *reinterpret_cast<const i32x4 *>(panel + (lane_at ^ 16));
+        Frag<kExact> f;
+        f.set(i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+        return f;
+    };
+
+    f32x4 acc[SM][SN] = {};
+    if (steps > 0) {
+        for (int s = 0; s < D - 1; ++s)
+#pragma unroll
+            for (int d = 0; d <= kLoads; ++d) issue(d, s, s);
+    }
+    int slot = 0;
+    for (int k = 0; k < steps; ++k) {
+        muon_polar::wait_vm_barrier<(D - 2) * (kLoads + 1)>();
+        const int next = slot == 0 ? D - 1 : slot - 1;  // the slot that step k - 1 left
+        const uint8_t *base = smem + slot * Geo::kSlot;
+        const float *scale_m = reinterpret_cast<const float *>(base + Geo::kPanels) + wm + r;
+        const float *scale_n = reinterpret_cast<const float *>(base + Geo::kPanels) + BM + wn;
+        Frag<kExact> fb[SN];
+        f32x4 sn[SN];
+#pragma unroll
+        for (int j = 0; j < SN; ++j) {
+            fb[j] = fragment(base + (BM + wn + 16 * j) * kBlock);
+            if constexpr (kRowB) sn[j] = *reinterpret_cast<const f32x4 *>(scale_n + 16 * j + 4 * part);
+        }
+        const float sb = kRowB ? 1.0f : scale_n[0];
+#pragma unroll
+        for (int i = 0; i < SM; ++i) {
+            const Frag<kExact> fa = fragment(base + (wm + 16 * i) * kBlock);
+            const float sm = scale_m[16 * i] * sb;
+#pragma unroll
+            for (int j = 0; j < SN; ++j) {
+                const f32x4 t = multiply(fb[j], fa);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    acc[i][j][e] = fmaf(t[e], kRowB ? sm * sn[j][e] : sm, acc[i][j][e]);
+            }
+#pragma unroll
+            for (int d = i * (kLoads + 1) / SM; d < (i + 1) * (kLoads + 1) / SM; ++d)
+                issue(d, k + D - 1, next);
+        }
+        slot = slot + 1 == D ? 0 : slot + 1;
+    }
+    muon_polar::wait_vm<0>();  // no DMA into LDS outlives the workgroup
+
+#pragma unroll
+    for (int i = 0; i < SM; ++i) {
+        const int64_t m = m0 + wm + 16 * i + r;
+        if (m >= g.m) continue;
+#pragma unroll
+        for (int j = 0; j < SN; ++j) {
+            const int64_t n = n0 + wn + 16 * j + 4 * part;
+            if (n < g.n) store4(g.c, m * g.ldc + n, g.n - n < 4 ? int(g.n - n) : 4, g.c_dtype, acc[i][j]);
+        }
+    }
+}
+
+// Tiles by how many of them there are: 256 x 256 where they occupy most compute units,
+// 128 x 128 where those do, else 64 x 64.
+template <int BM, int BN, int WM, int WN, int D>
+void launch_tiles(const MatmulArgs &g, hipStream_t stream) {
+    using Geo = Geometry<BM, BN, WM, WN, D>;
+    const int tm = static_cast<int>((g.m + BM - 1) / BM), tn = static_cast<int>((g.n + BN - 1) / BN);
+    const dim3 grid(static_cast<uint32_t>(tm) * static_cast<uint32_t>(tn));
+    const bool exact = g.c_dtype == MUON_TRAIN_F32, row_b = g.b.block_rows == 1;
+    auto go = [&](auto e, auto r) {
+        matmul_kernel<BM, BN, WM, WN, D, decltype(e)::value, decltype(r)::value>
+            <<<grid, Geo::kThreads, 0, stream>>>(g, tm, tn);
+    };
+    using std::bool_constant;
+    if (exact && row_b) go(bool_constant<true>{}, bool_constant<true>{});
+    else if (exact) go(bool_constant<true>{}, bool_constant<false>{});
+    else if (row_b) go(bool_constant<false>{}, bool_constant<true>{});
+    else go(bool_constant<false>{}, bool_constant<false>{});
+}
+
+bool dtype_ok(int t) { return t == MUON_TRAIN_F32 || t == MUON_TRAIN_BF16; }
+
+constexpr int64_t kMaxExtent = int64_t(1) << 30;
+
+int check(const muon_train_fp8_operand &o, int64_t k) {
+    if (!o.values || !o.scales) return invalid("fp8: null pointer");
+    if (reinterpret_cast<uintptr_t>(o.values) % 16 != 0 || o.ld % 16 != 0)
+        return invalid("fp8: values must be 16-byte aligned, row by row");
+    if (o.ld < k) return invalid("fp8: rows of values must not overlap");
+    // the rows of a tile are reached by 31-bit offsets
+    if (o.ld > (1 << 22)) return invalid("fp8: rows of values lie too far apart");
+    if (o.block_rows != 1 && o.block_rows != kBlock) return invalid("fp8: block_rows must be 1 or 128");
+    if (o.block_rows == 1 && o.scale_row != 1)
+        return invalid("fp8: scales of single rows must lie next to each other");
+    return MUON_POLAR_OK;
+}
+
+}  // namespace
+
+}  // namespace muon_train
+
+using namespace muon_train;
+
+extern "C" int muon_train_fp8_quantize(const muon_train_fp8_quantize_args *args, hipStream_t stream) {
+    if (!args) return invalid("fp8: args is null");
+    const QuantArgs a = *args;
+    if (a.rows < 0 || a.cols < 0 || a.rows > kMaxExtent || a.cols > kMaxExtent)
+        return invalid("fp8: rows and cols must be 0 to 2^30");
+    if (!dtype_ok(a.x_dtype)) return invalid("fp8: dtype must be float32 or bfloat16");
+    if (a.block_rows != 1 && a.block_rows != kBlock) return invalid("fp8: block_rows must be 1 or 128");
+    if (a.rows == 0 || a.cols == 0) return MUON_POLAR_OK;
+    if (!a.x || (!a.values && !a.values_t)) return invalid("fp8: null pointer");
+    if ((a.values || a.block_rows == kBlock) && !a.scales) return invalid("fp8: null pointer");
+    if (a.values_t && a.block_rows == 1 && !a.scales_t) return invalid("fp8: null pointer");
+    if (a.ld_x < a.cols) return invalid("fp8: rows of x must not overlap");
+    if (reinterpret_cast<uintptr_t>(a.values) % 16 != 0 || reinterpret_cast<uintptr_t>(a.values_t) % 16 != 0)
+        return invalid("fp8: values must be 16-byte aligned");
+    const int64_t tr = (a.rows + kBlock - 1) / kBlock, tc = (a.cols + kBlock - 1) / kBlock;
+    if (tr * tc > INT32_MAX) return invalid("fp8: matrix too large");
+    const dim3 grid(static_cast<uint32_t>(tr * tc));
+    const int t = static_cast<int>(tc);
+    if (a.x_dtype == MUON_TRAIN_BF16) {
+        if (a.block_rows == 1) quantize_kernel<Bf16, 1><<<grid, kQuantThreads, 0, stream>>>(a, t);
+        else quantize_kernel<Bf16, kBlock><<<grid, kQuantThreads, 0, stream>>>(a, t);
+    } else {
+        if (a.block_rows == 1) quantize_kernel<F32, 1><<<grid, kQuantThreads, 0, stream>>>(a, t);
+        else quantize_kernel<F32, kBlock><<<grid, kQuantThreads, 0, stream>>>(a, t);
+    }
+    return launched("fp8_quantize");
+}
+
+extern "C" int muon_train_fp8_matmul(const muon_train_fp8_matmul_args *args, hipStream_t stream) {
+    if (!args) return invalid("fp8: args is null");
+    const MatmulArgs g = *args;
+    if (g.m < 0 || g.n < 0 || g.k < 0 || g.m > kMaxExtent || g.n > kMaxExtent || g.k > kMaxExtent)
+        return invalid("fp8: m, n and k must be 0 to 2^30");
+    if (g.k % kBlock != 0) return invalid("fp8: k must be a multiple of 128");
+    if (!dtype_ok(g.c_dtype)) return invalid("fp8: dtype must be float32 or bfloat16");
+    if (g.m == 0 || g.n == 0) return MUON_POLAR_OK;
+    if (!g.c) return invalid("fp8: null pointer");
+    if (g.ldc < g.n) return invalid("fp8: rows of c must not overlap");
+    if (g.k > 0) {
+        int st = check(g.a, g.k);
+        if (st == MUON_POLAR_OK) st = check(g.b, g.k);
+        if (st != MUON_POLAR_OK) return st;
+    }
+    const int cus = compute_units();
+    if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "fp8: no device");
+    auto tiles = [&](int64_t t) { return ((g.m + t - 1) / t) * ((g.n + t - 1) / t); };
+    if (tiles(64) > INT32_MAX) return invalid("fp8: matrix too large");
+    if (2 * tiles(256) >= cus) launch_tiles<256, 256, 128, 64, 2>(g, stream);
+    else if (2 * tiles(128) >= cus) launch_tiles<128, 128, 64, 64, 2>(g, stream);
+    else launch_tiles<64, 64, 32, 32, 4>(g, stream);
+    return launched("fp8_matmul");
+}

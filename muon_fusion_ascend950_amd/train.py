@@ -2,7 +2,9 @@
 
 * ``block_norms`` — the norms before and after a block, with its gate and residual scale;
 * ``distill_topk``, ``distill_topk_with_grad`` — the loss against a teacher's top logits,
-  and loss and gradient in one pass.
+  and loss and gradient in one pass;
+* ``fp8_linear``, ``fp8_matmul``, ``quantize_fp8``, ``Fp8Blocks`` — products in 8-bit
+  floating point (e4m3) with a scale for each block of 128.
 
 ``muon_update`` starts from the gradients of a model's matrices; these are pieces of the
 forward and backward pass that produce them.  All take ROCm GPU tensors of float32 or
@@ -19,7 +21,8 @@ from ._loader import load_library
 
 load_library()
 
-__all__ = ["block_norms", "distill_topk", "distill_topk_with_grad"]
+__all__ = ["Fp8Blocks", "block_norms", "distill_topk", "distill_topk_with_grad", "fp8_linear",
+           "fp8_matmul", "quantize_fp8"]
 
 _ops = torch.ops.muon_ascend950
 _DTYPES = (torch.float32, torch.bfloat16)
@@ -269,3 +272,139 @@ def distill_topk_with_grad(logits: torch.Tensor, teacher_logits: torch.Tensor,
     if out is not None and not out.is_inference():
         torch.autograd.graph.increment_version(out)
     return loss, grad
+
+
+# ---------------------------------------------------------------------------------- fp8
+_BLOCK = 128
+
+
+def _blocks(n: int) -> int:
+    return -(-n // _BLOCK)
+
+
+class Fp8Blocks:
+    """A matrix as 8-bit values with a float32 scale for each block of 1 x 128 or 128 x 128.
+
+    values: ``float8_e4m3fn [rows, cols rounded up to a multiple of 128]``, zero past
+    ``cols`` (values of ``cols`` columns are padded here, by a copy); scales: float32
+    ``[rows, ceil(cols / 128)]`` or ``[ceil(rows / 128), ceil(cols / 128)]``; shape:
+    ``(rows, cols)``, by default that of ``values``.  Element (i, j) stands for
+    ``values[i, j] * scales[i or i // 128, j // 128]``.
+    """
+
+    __slots__ = ("values", "scales", "shape")
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor, shape=None):
+        _check_tensor("values", values, dtypes=(torch.float8_e4m3fn,))
+        _check_tensor("scales", scales, values.device, (torch.float32,))
+        if values.ndim != 2:
+            raise ValueError(f"values must be a matrix, got shape {tuple(values.shape)}")
+        rows, cols = tuple(values.shape) if shape is None else tuple(shape)
+        if cols < 1:
+            raise ValueError("a matrix must have columns")
+        padded = _blocks(cols) * _BLOCK
+        if rows != values.shape[0] or values.shape[1] not in (cols, padded):
+            raise ValueError(f"values of shape {tuple(values.shape)} do not hold a matrix of shape "
+                             f"{(rows, cols)}")
+        if tuple(scales.shape) not in ((rows, _blocks(cols)), (_blocks(rows), _blocks(cols))):
+            raise ValueError(f"scales must have shape {(rows, _blocks(cols))} or "
+                             f"{(_blocks(rows), _blocks(cols))}, got {tuple(scales.shape)}")
+        if values.shape[1] != padded:
+            whole = torch.zeros(rows, padded, dtype=torch.uint8, device=values.device)
+            whole[:, :cols] = values.view(torch.uint8)
+            values = whole.view(torch.float8_e4m3fn)
+        self.values, self.scales, self.shape = values, scales, (rows, cols)
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        """The matrix that the values and scales stand for."""
+        rows, cols = self.shape
+        scales = self.scales
+        if scales.shape[0] != rows:
+            scales = scales.repeat_interleave(_BLOCK, dim=0)[:rows]
+        wide = scales.repeat_interleave(_BLOCK, dim=1)
+        return (self.values.float() * wide)[:, :cols].to(dtype)
+
+
+def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> Fp8Blocks:
+    """``x`` ``[rows, cols]`` (float32 or bfloat16) in blocks of ``block_rows`` x 128, 1 for
+    activations and gradients or 128 for weights::
+
+        scale = max(amax(|block|) * (1 / 448), 2**-126)
+        values = (block * (1 / scale)).to(float8_e4m3fn)
+
+    A block that holds an infinity or a NaN has none but NaN back.
+    """
+    _check_tensor("x", x)
+    if x.ndim != 2 or x.shape[1] < 1:
+        raise ValueError(f"x must have shape [rows, cols], got {tuple(x.shape)}")
+    if block_rows not in (1, _BLOCK):
+        raise ValueError(f"block_rows must be 1 or {_BLOCK}, got {block_rows}")
+    values, scales = _ops.quantize_fp8(x.detach(), block_rows)
+    return Fp8Blocks(values, scales, x.shape)
+
+
+def _check_blocks(name, b) -> None:
+    if not isinstance(b, Fp8Blocks):
+        raise TypeError(f"{name} must be Fp8Blocks")
+
+
+def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``a @ b.T`` of matrices ``[M, K]`` and ``[N, K]``, summed in float32 and rounded once to
+    ``dtype`` (float32 or bfloat16).  No gradient: see ``fp8_linear``."""
+    _check_blocks("a", a)
+    _check_blocks("b", b)
+    if a.shape[1] != b.shape[1]:
+        raise ValueError(f"a and b must have one width, got {a.shape} and {b.shape}")
+    if a.values.device != b.values.device:
+        raise ValueError(f"b must be on {a.values.device}, got {b.values.device}")
+    if dtype not in _DTYPES:
+        raise TypeError(f"dtype must be torch.float32 or torch.bfloat16, got {dtype}")
+    return _ops.fp8_matmul(a.values, a.scales, b.values, b.scales, dtype)
+
+
+class _Fp8Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight):
+        need_x, need_w = ctx.needs_input_grad
+        y, *saved = _ops.fp8_linear_forward(x, weight, need_w | need_x << 1)
+        ctx.save_for_backward(*saved)
+        ctx.weight_dtype = weight.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        need_x, need_w = ctx.needs_input_grad
+        dx, dw = _ops.fp8_linear_backward(dy, *ctx.saved_tensors, ctx.weight_dtype,
+                                          need_x | need_w << 1)
+        return dx if need_x else None, dw if need_w else None
+
+
+def fp8_linear(x: torch.Tensor, weight) -> torch.Tensor:
+    """``x @ weight.T`` in 8-bit floating point: x ``[..., K]`` quantised in blocks of 1 x 128,
+    the weight ``[N, K]`` in blocks of 128 x 128; the result has x's dtype.
+
+    weight: a float32 or bfloat16 matrix (training: quantised in this call, and with the
+    gradients dx = dy @ weight and dweight = dy.T @ x, whose products are in 8 bits too, dy
+    and x quantised in blocks of 128 along the axis that each product sums over), or
+    ``Fp8Blocks`` (serving: no gradient).
+    """
+    _check_tensor("x", x)
+    if x.ndim < 1:
+        raise ValueError("x must have shape [..., K]")
+    if isinstance(weight, Fp8Blocks):
+        if weight.values.device != x.device:
+            raise ValueError(f"weight must be on {x.device}, got {weight.values.device}")
+        if weight.shape[1] != x.shape[-1]:
+            raise ValueError(f"x must have {weight.shape[1]} columns, got shape {tuple(x.shape)}")
+        if _wants_grad(x):
+            raise ValueError("a quantised weight has no gradient: pass the float32 or bfloat16 one")
+        return _ops.fp8_linear(x, weight.values, weight.scales)
+    _check_tensor("weight", weight, x.device)
+    if weight.ndim != 2 or weight.shape[1] != x.shape[-1]:
+        raise ValueError(f"weight must have shape [N, {x.shape[-1]}], got {tuple(weight.shape)}")
+    if 0 in weight.shape:
+        raise ValueError("weight's dimensions must be positive")
+    if _wants_grad(x, weight):
+        return _Fp8Linear.apply(x, weight)
+    return _ops.fp8_linear_forward(x, weight, 0)[0]

@@ -214,3 +214,122 @@ def test_distill_entry_checks_before_any_launch(change, message):
     assert lib.muon_train_distill_backward(ctypes.byref(no_stats), None) == capi.ERR_INVALID_ARGUMENT
     assert lib.muon_train_distill_forward(None, None) == capi.ERR_INVALID_ARGUMENT
     assert lib.muon_train_distill_forward(ctypes.byref(DistillArgs(**{**base, "rows": 0})), None) == capi.OK
+
+
+# ---------------------------------------------------------------------------------- fp8
+F8 = torch.float8_e4m3fn
+
+
+def test_fp8_blocks_refuses():
+    with FakeTensorMode():
+        ok = _cuda(200, 384, dtype=F8), _cuda(2, 3)
+        assert train.Fp8Blocks(*ok).shape == (200, 384)
+        assert train.Fp8Blocks(*ok, (200, 300)).shape == (200, 300)
+        assert train.Fp8Blocks(ok[0], _cuda(200, 3)).shape == (200, 384)
+        for bad, error in ((dict(values=_cuda(200, 384)), TypeError),
+                           (dict(values=torch.zeros(200, 384).to(F8)), ValueError),
+                           (dict(values=_cuda(384, dtype=F8)), ValueError),
+                           (dict(values=_cuda(200, 0, dtype=F8)), ValueError),
+                           (dict(scales=_cuda(2, 3, dtype=B16)), TypeError),
+                           (dict(scales=_cuda(3, 3)), ValueError),
+                           (dict(scales=_cuda(2, 4)), ValueError),
+                           (dict(shape=(199, 384)), ValueError),
+                           (dict(shape=(200, 200)), ValueError)):
+            args = dict(values=ok[0], scales=ok[1])
+            args.update(bad)
+            with pytest.raises(error):
+                train.Fp8Blocks(**args)
+
+
+def test_fp8_calls_refuse_and_fake():
+    with FakeTensorMode():
+        x, w = _cuda(2, 3, 300, dtype=B16), _cuda(130, 300)
+        q = train.quantize_fp8(w, 128)
+        assert q.values.shape == (130, 384) and q.scales.shape == (2, 3) and q.shape == (130, 300)
+        r = train.quantize_fp8(w)
+        assert r.scales.shape == (130, 3) and r.scales.stride() == (1, 130)
+        for call, error, message in (
+                (lambda: train.quantize_fp8(_cuda(3)), ValueError, "shape"),
+                (lambda: train.quantize_fp8(_cuda(3, 0)), ValueError, "shape"),
+                (lambda: train.quantize_fp8(w, 64), ValueError, "block_rows"),
+                (lambda: train.quantize_fp8(_cuda(3, 4, dtype=torch.float16)), TypeError, "x must"),
+                (lambda: train.quantize_fp8(torch.zeros(3, 4)), ValueError, "ROCm GPU"),
+                (lambda: train.fp8_matmul(w, q), TypeError, "Fp8Blocks"),
+                (lambda: train.fp8_matmul(q, train.quantize_fp8(_cuda(9, 301))), ValueError, "width"),
+                (lambda: train.fp8_matmul(q, r, torch.float16), TypeError, "dtype"),
+                (lambda: train.fp8_linear(3.0, w), TypeError, "x must"),
+                (lambda: train.fp8_linear(_cuda(), w), ValueError, "shape"),
+                (lambda: train.fp8_linear(x, _cuda(130, 301)), ValueError, "weight"),
+                (lambda: train.fp8_linear(x, _cuda(0, 300)), ValueError, "positive"),
+                (lambda: train.fp8_linear(x, w.half()), TypeError, "weight"),
+                (lambda: train.fp8_linear(_cuda(2, 301), q), ValueError, "columns"),
+                (lambda: train.fp8_linear(_cuda(2, 300).requires_grad_(True), q), ValueError, "gradient")):
+            with pytest.raises(error, match=message):
+                call()
+        assert train.fp8_matmul(r, q).shape == (130, 130)
+        y = train.fp8_linear(x, q)
+        assert y.shape == (2, 3, 130) and y.dtype == B16
+        y = train.fp8_linear(x, w.requires_grad_(True))
+        assert y.shape == (2, 3, 130) and y.requires_grad
+        ops = torch.ops.muon_ascend950
+        _, *saved = ops.fp8_linear_forward(x, w, 3)
+        assert saved[0].shape == (300, 128) and saved[2].shape == (300, 256)
+        dx, dw = ops.fp8_linear_backward(y, *saved, F32, 3)
+        assert dx.shape == x.shape and dx.dtype == B16 and dw.shape == w.shape and dw.dtype == F32
+
+
+class QuantizeArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("rows", "cols", "ld_x")] + [("x", ctypes.c_void_p)] + [
+        (n, ctypes.c_int) for n in ("x_dtype", "block_rows")] + [
+        (n, ctypes.c_void_p) for n in ("values", "scales", "values_t", "scales_t")]
+
+
+class Operand(ctypes.Structure):
+    _fields_ = [("values", ctypes.c_void_p), ("scales", ctypes.c_void_p)] + [
+        (n, ctypes.c_int64) for n in ("ld", "scale_row", "scale_col")] + [("block_rows", ctypes.c_int)]
+
+
+class MatmulArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("m", "n", "k")] + [("a", Operand), ("b", Operand),
+                ("c", ctypes.c_void_p), ("ldc", ctypes.c_int64), ("c_dtype", ctypes.c_int)]
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(rows=-1), "rows"), (dict(cols=1 << 31), "cols"), (dict(x_dtype=3), "dtype"),
+    (dict(block_rows=64), "block_rows"), (dict(x=None), "null"), (dict(values=None), "null"),
+    (dict(scales=None), "null"), (dict(values_t=4096), "null"), (dict(ld_x=9), "overlap"),
+    (dict(values=4100), "aligned"), (dict(rows=1 << 30, cols=1 << 30, ld_x=1 << 30), "too large"),
+])
+def test_quantize_entry_checks_before_any_launch(change, message):
+    lib = capi.load()
+    base = dict(rows=4, cols=10, ld_x=10, x=4096, block_rows=1, values=4096, scales=4096)
+    args = QuantizeArgs(**{**base, **change})
+    assert lib.muon_train_fp8_quantize(ctypes.byref(args), None) == capi.ERR_INVALID_ARGUMENT
+    assert message in capi.last_error()
+    assert lib.muon_train_fp8_quantize(None, None) == capi.ERR_INVALID_ARGUMENT
+    for empty in ("rows", "cols"):
+        args = QuantizeArgs(**{**base, empty: 0})
+        assert lib.muon_train_fp8_quantize(ctypes.byref(args), None) == capi.OK
+
+
+@pytest.mark.parametrize("change,operand,message", [
+    (dict(m=-1), {}, "m, n and k"), (dict(k=100), {}, "multiple of 128"), (dict(c=None), {}, "null"),
+    (dict(c_dtype=2), {}, "dtype"), (dict(ldc=7), {}, "overlap"), ({}, dict(values=None), "null"),
+    ({}, dict(scales=None), "null"), ({}, dict(values=4104), "aligned"), ({}, dict(ld=264), "aligned"),
+    ({}, dict(ld=128), "overlap"), ({}, dict(ld=1 << 23), "far apart"),
+    ({}, dict(block_rows=2), "block_rows"), ({}, dict(scale_row=2), "next to each other"),
+    (dict(m=1 << 30, n=1 << 30, ldc=1 << 30), {}, None),
+])
+def test_matmul_entry_checks_before_any_launch(change, operand, message):
+    lib = capi.load()
+    good = dict(values=4096, scales=4096, ld=256, scale_row=1, scale_col=4, block_rows=1)
+    base = dict(m=4, n=8, k=256, c=4096, ldc=8)
+    args = MatmulArgs(**{**base, **change}, a=Operand(**{**good, **operand}), b=Operand(**good))
+    status = lib.muon_train_fp8_matmul(ctypes.byref(args), None)
+    if message is None:  # too large, or no device to say for
+        assert status in (capi.ERR_INVALID_ARGUMENT, capi.ERR_HIP)
+    else:
+        assert status == capi.ERR_INVALID_ARGUMENT and message in capi.last_error()
+    for empty in ("m", "n"):
+        args = MatmulArgs(**{**base, empty: 0}, a=Operand(**good), b=Operand(**good))
+        assert lib.muon_train_fp8_matmul(ctypes.byref(args), None) == capi.OK

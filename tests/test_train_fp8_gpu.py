@@ -1,0 +1,267 @@
+"""quantize_fp8, fp8_matmul and fp8_linear on the GPU: the held values and scales bit for bit
+against the definition in torch on the CPU, the products against 64 bits, forward and both
+gradients, at sizes from one row, column or block to ragged ones past many tiles.
+
+Tolerances: products of held values are exact in float32 up to a sum of K of them, scaled
+by s_a * s_b (one rounding each): F32_SUM on the 2-norm, whose terms cancel."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import muon_fusion_ascend950_amd as mf
+from tests.train_checks import F32_SUM, check, randn
+
+pytestmark = pytest.mark.gpu
+F32, B16, F8 = torch.float32, torch.bfloat16, torch.float8_e4m3fn
+
+
+def held(x, rows):
+    """(values as bytes [R, C padded], scales) by the definition, on the CPU."""
+    x = x.detach().float().cpu()
+    r, c = x.shape
+    rp, cp = -(-r // rows) * rows, -(-c // 128) * 128
+    blocks = torch.nn.functional.pad(x, (0, cp - c, 0, rp - r)).view(rp // rows, rows, cp // 128, 128)
+    amax = blocks.abs().amax(dim=(1, 3))
+    scales = amax * torch.tensor(1 / 448, dtype=F32)
+    scales = torch.where(scales < 2.0 ** -126, torch.tensor(2.0 ** -126), scales)
+    inverse = torch.ones(()) / scales
+    values = (blocks * inverse[:, None, :, None]).to(F8)
+    return values.view(rp, cp)[:r].view(torch.uint8), scales
+
+
+def value(x, rows):
+    """What the held matrix stands for, in 64 bits."""
+    q, s = held(x, rows)
+    s = s.double().repeat_interleave(rows, 0)[: q.shape[0]].repeat_interleave(128, 1)
+    return (q.view(F8).double() * s)[:, : x.shape[1]]
+
+
+def spread(gen, r, c, dtype=F32):
+    """Rows and columns of sizes orders of magnitude apart."""
+    return (randn(gen, r, c) * torch.exp(randn(gen, r, 1)) * torch.exp(2 * randn(gen, 1, c))).to(dtype)
+
+
+@pytest.mark.parametrize("r,c", [(1, 1), (1, 128), (3, 130), (128, 128), (129, 257), (500, 77), (40, 2051)])
+@pytest.mark.parametrize("dtype", [F32, B16], ids=str)
+@pytest.mark.parametrize("rows", [1, 128])
+def test_quantize_bits(r, c, dtype, rows):
+    x = spread(torch.Generator().manual_seed(r + c), r, c, dtype)
+    got = mf.train.quantize_fp8(x.cuda(), rows)
+    values, scales = held(x, rows)
+    assert got.shape == (r, c) and got.values.shape == values.shape
+    assert torch.equal(got.scales.cpu(), scales)
+    assert torch.equal(got.values.view(torch.uint8).cpu(), values)
+    assert torch.equal(got.dequantize().cpu().double(), value(x, rows).float().double())
+
+
+@pytest.mark.parametrize("rows", [1, 128])
+def test_quantize_extremes(rows):
+    x = torch.zeros(256, 512)
+    x[0, 128:256] = 1e-42  # subnormal
+    x[128, 0] = 3.4e38
+    x[128, 300] = -1e-30
+    x[5, 384:] = torch.linspace(-448, 448, 128)  # every rounding of the grid
+    x[6, 384:] = torch.linspace(-1, 1, 128) * 2.0 ** -9
+    got, (values, scales) = mf.train.quantize_fp8(x.cuda(), rows), held(x, rows)
+    assert torch.equal(got.scales.cpu(), scales)
+    assert torch.equal(got.values.view(torch.uint8).cpu() & 0x7f, values & 0x7f)
+    x[1, 3] = math.inf
+    x[200, 400] = math.nan
+    back = mf.train.quantize_fp8(x.cuda(), rows).dequantize().cpu()
+    assert back[1, :128].isnan().all() and back[200, 384:].isnan().all()
+    ok = torch.ones(256, 512, dtype=torch.bool)
+    ok[(slice(0, 128) if rows == 128 else 1), :128] = False
+    ok[(slice(128, 256) if rows == 128 else 200), 384:] = False
+    assert back[ok].isfinite().all()
+
+
+def test_quantize_strides():
+    gen = torch.Generator().manual_seed(0)
+    x = spread(gen, 300, 411)
+    for view in (x[7:200:2, 5:301], x.t(), x[:1].expand(40, 411), x[:, :1]):
+        g = x.cuda()
+        on_gpu = torch.as_strided(g, view.shape, view.stride(), view.storage_offset())
+        got, (values, scales) = mf.train.quantize_fp8(on_gpu), held(view, 1)
+        assert torch.equal(got.scales.cpu(), scales)
+        assert torch.equal(got.values.view(torch.uint8).cpu(), values)
+
+
+SIZES = [(1, 1, 1), (1, 16, 128), (1, 300, 1000), (2, 5, 129), (16, 64, 256), (17, 130, 640),
+         (64, 513, 384), (127, 128, 128), (128, 129, 4096), (150, 2050, 1000), (257, 255, 2050),
+         (300, 31, 14336), (1000, 777, 520), (1, 4099, 300), (33, 1, 77), (512, 768, 1024)]
+
+
+@pytest.mark.parametrize("m,n,k", SIZES, ids=str)
+@pytest.mark.parametrize("a_rows,b_rows", [(1, 128), (1, 1), (128, 128)])
+def test_products(m, n, k, a_rows, b_rows):
+    gen = torch.Generator().manual_seed(m + n + k)
+    a, b = spread(gen, m, k), spread(gen, n, k)
+    qa, qb = mf.train.quantize_fp8(a.cuda(), a_rows), mf.train.quantize_fp8(b.cuda(), b_rows)
+    want = value(a, a_rows) @ value(b, b_rows).t()
+    got = mf.train.fp8_matmul(qa, qb, F32)
+    assert got.shape == (m, n) and got.dtype == F32
+    check(got, want, F32_SUM)
+    low = mf.train.fp8_matmul(qa, qb)
+    assert low.dtype == B16
+    check(low, want, F32_SUM)
+    assert torch.equal(got, mf.train.fp8_matmul(qa, qb, F32))
+
+
+def test_products_of_many_tiles():
+    gen = torch.Generator().manual_seed(9)
+    a, b = randn(gen, 2100, 900), randn(gen, 1900, 900)
+    want = (value(a, 1).cuda() @ value(b, 128).cuda().t())
+    qa, qb = mf.train.quantize_fp8(a.cuda()), mf.train.quantize_fp8(b.cuda(), 128)
+    check(mf.train.fp8_matmul(qa, qb, F32), want, F32_SUM)
+    check(mf.train.fp8_matmul(qb, qa, F32), want.t(), F32_SUM)
+
+
+def test_exact_sums():
+    """Small whole numbers with scales of one: every sum is exact, so every bit is known."""
+    gen = torch.Generator().manual_seed(2)
+    for m, n, k in ((70, 90, 300), (1, 257, 5000), (300, 520, 1100), (1030, 1290, 640)):
+        a = torch.randint(-8, 9, (m, k), generator=gen).float()
+        b = torch.randint(-8, 9, (n, k), generator=gen).float()
+        qa = mf.train.Fp8Blocks(a.to(F8).cuda(), torch.ones(m, -(-k // 128), device="cuda"))
+        qb = mf.train.Fp8Blocks(b.to(F8).cuda(), torch.ones(-(-n // 128), -(-k // 128), device="cuda"))
+        assert torch.equal(mf.train.fp8_matmul(qa, qb, F32).cpu(), a @ b.t())
+
+
+def test_each_block_has_its_scale():
+    """One element of a in each block of 128, scales that are powers of two of their place:
+    the product of one block with ones, exactly."""
+    m, n, k = 200, 300, 5 * 128
+    for b_rows in (1, 128):
+        sa = 2.0 ** ((torch.arange(m)[:, None] * 3 + torch.arange(5)) % 11 - 5).float()
+        nb = n if b_rows == 1 else -(-n // 128)
+        sb = 2.0 ** ((torch.arange(nb)[:, None] * 5 + 2 * torch.arange(5)) % 7 - 3).float()
+        a = torch.zeros(m, k)
+        for block in range(5):
+            a[:, block * 128 + (torch.arange(m).argmax() * 0 + 31 * block) % 128] = 1.0 + block
+        b = torch.ones(n, k)
+        qa = mf.train.Fp8Blocks(a.to(F8).cuda(), sa.cuda())
+        qb = mf.train.Fp8Blocks(b.to(F8).cuda(), sb.cuda())
+        full = sb.repeat_interleave(b_rows, 0)[:n]
+        want = (sa * torch.arange(1.0, 6.0)) @ full.t()
+        assert torch.equal(mf.train.fp8_matmul(qa, qb, F32).cpu(), want)
+
+
+def test_rows_of_nan_and_padding():
+    """A NaN stays in its row; bytes past a matrix's own columns are no part of it."""
+    gen = torch.Generator().manual_seed(3)
+    a, b = randn(gen, 40, 300), randn(gen, 70, 300)
+    clean = mf.train.fp8_matmul(mf.train.quantize_fp8(a.cuda()), mf.train.quantize_fp8(b.cuda(), 128))
+    a[11, 200] = math.nan
+    got = mf.train.fp8_matmul(mf.train.quantize_fp8(a.cuda()), mf.train.quantize_fp8(b.cuda(), 128))
+    rows = [i for i in range(40) if i != 11]
+    assert got[11].isnan().all() and torch.equal(got[rows], clean[rows])
+    wide = torch.full((70, 384), 0x7f, dtype=torch.uint8, device="cuda")  # NaN past column 300
+    qb = mf.train.quantize_fp8(b.cuda(), 128)
+    wide[:, :300] = qb.values.view(torch.uint8)[:, :300]
+    cut = mf.train.Fp8Blocks(wide[:, :300].view(F8), qb.scales)
+    got = mf.train.fp8_matmul(mf.train.quantize_fp8(a.cuda()), cut)
+    assert torch.equal(got[rows], clean[rows])
+
+
+def test_operands_of_other_layouts():
+    gen = torch.Generator().manual_seed(4)
+    a, b = mf.train.quantize_fp8(randn(gen, 50, 500).cuda()), mf.train.quantize_fp8(randn(gen, 300, 500).cuda(), 128)
+    want = mf.train.fp8_matmul(a, b)
+    rows = mf.train.Fp8Blocks(a.values, a.scales.contiguous(), a.shape)
+    wide = torch.zeros(50, 527, dtype=torch.uint8, device="cuda")
+    wide[:, 3:515] = a.values.view(torch.uint8)
+    shifted = mf.train.Fp8Blocks(wide[:, 3:515].view(F8), a.scales, a.shape)
+    turned = mf.train.Fp8Blocks(b.values, b.scales.t().contiguous().t(), b.shape)
+    for x, y in ((rows, b), (shifted, b), (a, turned)):
+        assert torch.equal(mf.train.fp8_matmul(x, y), want)
+
+
+LINEAR = [((1,), 128, 128), ((1, 1), 300, 260), ((3, 50), 130, 1000), ((5, 7), 513, 77),
+          ((333,), 768, 2050), ((2, 260), 640, 384), ((1200,), 520, 650)]
+
+
+@pytest.mark.parametrize("lead,n,k", LINEAR, ids=str)
+@pytest.mark.parametrize("dtype,weight_dtype", [(F32, F32), (B16, F32), (B16, B16)], ids=str)
+def test_linear_and_gradients(lead, n, k, dtype, weight_dtype):
+    gen = torch.Generator().manual_seed(n + k)
+    t = math.prod(lead)
+    x, w = spread(gen, t, k, dtype), (randn(gen, n, k) / math.sqrt(k)).to(weight_dtype)
+    dy = spread(gen, t, n, dtype)
+    xg = x.view(*lead, k).cuda().requires_grad_(True)
+    wg = w.cuda().requires_grad_(True)
+    y = mf.train.fp8_linear(xg, wg)
+    assert y.shape == (*lead, n) and y.dtype == dtype
+    check(y.view(t, n), value(x, 1) @ value(w, 128).t(), F32_SUM, "y")
+    with torch.no_grad():
+        assert torch.equal(mf.train.fp8_linear(xg, wg), y)
+        assert torch.equal(mf.train.fp8_linear(xg, mf.train.quantize_fp8(wg, 128)), y)
+    dx, dw = torch.autograd.grad(y, (xg, wg), dy.view(*lead, n).cuda())
+    assert dx.shape == xg.shape and dx.dtype == dtype and dw.shape == w.shape and dw.dtype == weight_dtype
+    check(dx.view(t, k), value(dy, 1) @ value(w, 128), F32_SUM, "dx")
+    check(dw, value(dy.t(), 1) @ value(x.t(), 1).t(), F32_SUM, "dw")
+
+
+def test_only_some_gradients_wanted():
+    gen = torch.Generator().manual_seed(6)
+    x, w, dy = spread(gen, 70, 300).cuda(), randn(gen, 140, 300).cuda(), randn(gen, 70, 140).cuda()
+    both = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    dx, dw = torch.autograd.grad(mf.train.fp8_linear(*both), both, dy)
+    a = x.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(mf.train.fp8_linear(a, w), a, dy)[0], dx)
+    b = w.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(mf.train.fp8_linear(x, b), b, dy.t().contiguous().t())[0], dw)
+
+
+def test_no_tokens():
+    x = torch.empty(0, 3, 256, device="cuda", requires_grad=True)
+    w = torch.randn(100, 256, device="cuda", requires_grad=True)
+    y = mf.train.fp8_linear(x, w)
+    y.sum().backward()
+    assert y.shape == (0, 3, 100) and x.grad.shape == x.shape
+    assert torch.equal(w.grad, torch.zeros_like(w))
+
+
+def test_gradients_against_differences():
+    """The product is linear in each operand but for its rounding to 8 bits, 2^-4 of a value
+    at most: along the gradient itself the change over a step of the operand's own size is
+    the slope to within that."""
+    gen = torch.Generator().manual_seed(8)
+    x, w = randn(gen, 200, 384).cuda(), randn(gen, 256, 384).cuda()
+    dy = randn(gen, 200, 256).cuda()
+    xg, wg = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    dx, dw = torch.autograd.grad(mf.train.fp8_linear(xg, wg), (xg, wg), dy)
+
+    def total(a, b):
+        with torch.no_grad():
+            return (mf.train.fp8_linear(a, b).double() * dy.double()).sum()
+
+    for g, at in ((dx, lambda d: total(x + d, w)), (dw, lambda d: total(x, w + d))):
+        way = g / g.square().mean().sqrt()
+        slope = (g.double() * way.double()).sum()
+        assert abs((at(way) - at(-way)) / 2 - slope) <= 2.0 ** -4 * slope
+
+
+def test_another_stream_and_a_graph():
+    gen = torch.Generator().manual_seed(7)
+    x, w = randn(gen, 200, 640, dtype=B16).cuda(), mf.train.quantize_fp8(randn(gen, 512, 640).cuda(), 128)
+    want = mf.train.fp8_linear(x, w)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = mf.train.fp8_linear(x, w)
+    torch.cuda.current_stream().wait_stream(stream)
+    assert torch.equal(got, want)
+    for rows in (1, 200):
+        held_x = x[:rows].clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = mf.train.fp8_linear(held_x, w)
+        for _ in range(3):
+            held_x.copy_(randn(gen, rows, 640, dtype=B16))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, mf.train.fp8_linear(held_x, w))
