@@ -63,6 +63,12 @@ def _run(cmd: list[str], verbose: bool) -> None:
             print("\n".join(lines), flush=True)
 
 
+def _run_all(jobs: list[list[str]], verbose: bool) -> None:
+    with concurrent.futures.ThreadPoolExecutor(max_workers=len(jobs)) as pool:
+        for fut in [pool.submit(_run, cmd, verbose) for cmd in jobs]:
+            fut.result()
+
+
 def _torch_paths() -> tuple[list[str], Path]:
     import torch  # noqa: WPS433 (build-time only)
 
@@ -80,9 +86,7 @@ def build_hip_library(verbose: bool = True) -> Path:
     objects = [BUILD_DIR / (Path(src).stem + ".o") for src in sources]
     jobs = [[_hipcc(), "-x", "hip", "-c", str(CSRC / src), "-o", str(obj)] + common
             for src, obj in zip(sources, objects)]
-    with concurrent.futures.ThreadPoolExecutor(max_workers=len(jobs)) as pool:
-        for fut in [pool.submit(_run, cmd, verbose) for cmd in jobs]:
-            fut.result()
+    _run_all(jobs, verbose)
     out = PKG_DIR / "libmuon_polar.so"
     tmp = out.with_suffix(".so.tmp")
     _run([_hipcc(), "-shared", "-fPIC", f"--offload-arch={ARCH}"] + [str(o) for o in objects]
@@ -99,15 +103,16 @@ def build_torch_binding(verbose: bool = True) -> Path:
     out = PKG_DIR / "_C.so"
     tmp = out.with_suffix(".so.tmp")
     cxx = shutil.which("g++") or "g++"
+    flags = ["-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             f"-D_GLIBCXX_USE_CXX11_ABI={abi}", f"-I{INCLUDE}", f"-I{ROCM / 'include'}",
+             f"-I{sysconfig.get_paths()['include']}"] + [f"-I{p}" for p in incs]
+    BUILD_DIR.mkdir(exist_ok=True)
+    sources = ["muon_polar_step_binding.cpp", "muon_train_binding.cpp"]
+    objects = [BUILD_DIR / (Path(src).stem + ".o") for src in sources]
+    _run_all([[cxx, "-c", str(CSRC / src), "-o", str(obj)] + flags
+              for src, obj in zip(sources, objects)], verbose)
     cmd = [
-        cxx, "-O2", "-std=c++17", "-fPIC", "-shared",
-        str(CSRC / "muon_polar_step_binding.cpp"), str(CSRC / "muon_train_binding.cpp"),
-        "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-        f"-I{INCLUDE}", f"-I{ROCM / 'include'}",
-        f"-I{sysconfig.get_paths()['include']}",
-    ]
-    cmd += [f"-I{p}" for p in incs]
-    cmd += [
+        cxx, "-shared", *(str(o) for o in objects),
         f"-L{PKG_DIR}", "-lmuon_polar",
         f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip",
         f"-L{ROCM / 'lib'}", "-lamdhip64",
