@@ -103,7 +103,8 @@ typedef struct muon_train_distill_args {
     double temperature, label_weight, grad_value;
     int logits_dtype, teacher_dtype, index_bytes; /* index_bytes: 4 or 8 */
     float *loss;  /* [rows] */
-    float *stats; /* [rows, 4]: max z, 1 / Σ exp((z − max) / τ), 1 / Σ exp(z − max), 0 */
+    float *stats; /* [rows, 4]: max z, 1 / Σ exp((z − max) / τ), 1 / Σ exp(z − max) (labels),
+                     1 / Σ exp((t − max t) / τ) (0 without entries) */
     void *grad;   /* [rows, vocab], logits' dtype */
 } muon_train_distill_args;
 

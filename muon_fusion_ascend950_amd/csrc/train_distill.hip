@@ -1,11 +1,12 @@
 // train_distill.hip — the loss against a teacher's top logits, its gradient, and both in
 // one pass (include/muon_train.h; the formulas are there).
 //
-// One workgroup a row.  The row is loaded into registers whole (up to 256 KiB: 1024
-// threads with 16 pieces of 16 bytes each), its maximum and its sum of exponentials are
-// taken from there, and the gradient is written from there: the logits cross memory once
-// in and once out, which is what bounds the pass.  Of a longer row the threads take the
-// rest with a running maximum and sum, and read it again for the gradient.
+// Loss and gradient in one pass: one workgroup a row, which it loads into registers whole
+// (up to 256 KiB: 1024 threads with 16 pieces of 16 bytes each); maximum and sum of
+// exponentials are taken from there, and the gradient is written from there: the logits
+// cross memory once in and once out, which is what bounds the pass.  Of a longer row the
+// threads take the rest with a running maximum and sum, and read it again for the gradient.
+// Loss alone, and the gradient from a forward pass's stats, hold no row: it streams by.
 //
 // The gradient is the softmax everywhere but at the teacher's indices and the label.  All
 // of the row is written as softmax first; then, past a barrier, each entry overwrites its
@@ -88,227 +89,378 @@ __device__ __forceinline__ int64_t load_index(const Args &a, int64_t i) {
 // their share of a sum whose largest term is 1 does).
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-enum { kLoss = 0, kLossAndGrad = 1, kGradFromStats = 2 };
+// The teacher's entries of one row, kTops in each of NT threads, and the label.
+template <int NT, bool kHard>
+struct Targets {
+    static constexpr int kTops = kMaxTop / NT;
+    float t[kTops], zk[kTops], pe[kTops];  // logits of teacher and student, exp of the former
+    int index[kTops];
+    int label = -1;
+    float z_label = 0.0f;
 
-// NT threads a row, R chunks of it in each thread's registers.  kHard: with labels.
-template <class T, int NT, int R, int MODE, bool kHard>
-__global__ __launch_bounds__(NT) void distill_kernel(Args a) {
+    // Loads; returns the largest of the thread's teacher logits.
+    template <class Raw>
+    __device__ __forceinline__ float load(const Args &a, int64_t row, const Raw *z) {
+        float top = kNegInf;
+#pragma unroll
+        for (int j = 0; j < kTops; ++j) {
+            const int e = j * NT + threadIdx.x;
+            index[j] = -1;
+            t[j] = kNegInf;
+            zk[j] = 0.0f;
+            if (e < a.k) {
+                const int64_t i = load_index(a, row * a.k + e);
+                if (i >= 0 && i < a.vocab) {
+                    index[j] = static_cast<int>(i);
+                    t[j] = load_any(a.teacher_logits, row * a.k + e, a.teacher_dtype);
+                    zk[j] = to_f32(z[i]);
+                }
+                top = fmaxf(top, t[j]);
+            }
+        }
+        if constexpr (kHard) {
+            const int64_t y = a.labels[row];
+            label = y >= 0 && y < a.vocab ? static_cast<int>(y) : -1;
+            if (label >= 0) z_label = to_f32(z[label]);
+        }
+        return top;
+    }
+    // The thread's share of Σ exp((t − t_max) / τ); c = log2(e) / τ.
+    __device__ __forceinline__ float weigh(float t_max, float c) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kTops; ++j) {
+            pe[j] = index[j] >= 0 && t_max > kNegInf ? exp2_hw((t[j] - t_max) * c) : 0.0f;
+            if (index[j] >= 0 && t[j] != t[j]) pe[j] = t[j];
+            sum += pe[j];
+        }
+        return sum;
+    }
+    // The thread's share of τ²·Σ p·(log p − log q): the differences of logits are scaled by
+    // τ alone, so that neither overflows where the loss does not.
+    __device__ __forceinline__ float divergence(float tau, float t_max, float t_sum, float z_max,
+                                                float z_sum) const {
+        const bool taught = t_sum != 0.0f;
+        const float inv = taught ? 1.0f / t_sum : 0.0f;
+        const float logs = tau * (logf(z_sum) - (taught ? logf(t_sum) : 0.0f));
+        float kl = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kTops; ++j) {
+            const float p = pe[j] * inv;
+            if (p != 0.0f) kl += p * (tau * (((t[j] - t_max) - (zk[j] - z_max)) + logs));
+        }
+        return kl;
+    }
+};
+
+// One chunk's arithmetic at a time.
+__device__ __forceinline__ void chunk_done() { __builtin_amdgcn_sched_barrier(0); }
+// Makes the compiler forget what it knows of held chunks: it would keep what one pass over
+// them works out (fp32 values, exponentials: twice the registers of bf16 chunks) for the
+// next, and spill.
+template <int R, class C>
+__device__ __forceinline__ void forget(C *held) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) asm volatile("" : "+v"(held[r].v));
+}
+
+// Largest logit and sums of exponentials of a part of a row, taken piece by piece: the sums
+// are relative to the largest so far (to 0 while that is −inf, so that −inf adds nothing
+// and a NaN stays one).
+template <bool kHard>
+struct Running {
+    float top = kNegInf, sum = 0.0f, hard = 0.0f;
+    __device__ __forceinline__ static float against(float top) { return top == kNegInf ? 0.0f : top; }
+    __device__ __forceinline__ void rebase(float m, float c) {
+        const float d = top - against(m);
+        sum *= exp2_hw(d * c);
+        if constexpr (kHard) hard *= exp2_hw(d * kLog2e);
+        top = m;
+    }
+    template <int N>
+    __device__ __forceinline__ void add(const float (&f)[N], float c) {
+        const float ref = against(top);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            sum += exp2_hw((f[i] - ref) * c);
+            if constexpr (kHard) hard += exp2_hw((f[i] - ref) * kLog2e);
+        }
+    }
+};
+
+// Takes kAhead chunks of a thread into its running sums.  Every kernel takes a row's chunks
+// in the same groups and order, so the loss has the same bits with and without a gradient.
+constexpr int kAhead = 4;
+template <class C, bool kHard>
+__device__ __forceinline__ void take(Running<kHard> &run, C *x, float c) {
+    float m = run.top;
+#pragma unroll
+    for (int r = 0; r < kAhead; ++r) {
+        float f[C::kElems];
+        x[r].get(f);
+#pragma unroll
+        for (int i = 0; i < C::kElems; ++i) m = fmaxf(m, f[i]);
+        chunk_done();
+    }
+    forget<kAhead>(x);
+    run.rebase(m, c);
+#pragma unroll
+    for (int r = 0; r < kAhead; ++r) {
+        float f[C::kElems];
+        x[r].get(f);
+        run.add(f, c);
+        chunk_done();
+    }
+}
+
+// What the gradient needs of a row: softmax(z / τ) times f_soft plus softmax(z) times f_hard.
+template <bool kHard>
+struct Slope {
+    float z_max, c, f_soft, f_hard;
+    __device__ __forceinline__ float operator()(float x) const {
+        float d = f_soft * exp2_hw((x - z_max) * c);
+        if constexpr (kHard) d = fmaf(f_hard, exp2_hw((x - z_max) * kLog2e), d);
+        return d;
+    }
+};
+
+// Past a barrier behind the whole row's softmax: the elements of the entries in [lo, hi).
+template <class T, int NT, bool kHard>
+__device__ __forceinline__ void overwrite_entries(const Args &a, const Targets<NT, kHard> &y,
+                                                  const Slope<kHard> &slope, float g, float soft,
+                                                  float inv_teacher, typename T::Raw *out, int lo,
+                                                  int hi, int *entry_at, float *entry_amount) {
+    const int k = static_cast<int>(a.k), tid = threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < y.kTops; ++j) {
+        const int e = j * NT + tid;
+        if (e < k) {
+            entry_at[e] = y.index[j];
+            entry_amount[e] = soft * (y.pe[j] * inv_teacher);
+        }
+    }
+    if (kHard && tid == 0) {
+        entry_at[k] = y.label;
+        entry_amount[k] = y.label >= 0 ? float(a.label_weight) : 0.0f;
+    }
+    __syncthreads();
+    const int entries = k + (kHard ? 1 : 0);
+    auto overwrite = [&](int at, float x) {
+        float amount = 0.0f;
+#pragma unroll 8
+        for (int e = 0; e < entries; ++e) amount += entry_at[e] == at ? entry_amount[e] : 0.0f;
+        const float d = slope(x) - g * amount;
+        if constexpr (sizeof(typename T::Raw) == 2)
+            out[at] = f32_to_bf16_bits(d);
+        else
+            out[at] = d;
+    };
+#pragma unroll
+    for (int j = 0; j < y.kTops; ++j)
+        if (y.index[j] >= lo && y.index[j] < hi) overwrite(y.index[j], y.zk[j]);
+    if (kHard && tid == NT - 1 && y.label >= lo && y.label < hi) overwrite(y.label, y.z_label);
+}
+
+template <bool kHard>
+__device__ __forceinline__ void write_row(const Args &a, int64_t row, float kl, float z_max,
+                                          float z_sum, float z_hard, float t_sum, int label,
+                                          float z_label) {
+    const float lam = kHard ? float(a.label_weight) : 0.0f;
+    float loss = (1.0f - lam) * kl;
+    if (kHard && label >= 0) loss += lam * (logf(z_hard) - (z_label - z_max));
+    a.loss[row] = loss;
+    if (a.stats) {
+        a.stats[4 * row] = z_max;
+        a.stats[4 * row + 1] = 1.0f / z_sum;
+        a.stats[4 * row + 2] = kHard ? 1.0f / z_hard : 0.0f;
+        a.stats[4 * row + 3] = t_sum != 0.0f ? 1.0f / t_sum : 0.0f;
+    }
+}
+
+// Calls f(r, offset of the stripe, offset in it, elements of the chunk inside the row) for
+// the R stripes of NT chunks from `at` on; of a stripe that lies inside whole, without a
+// mask.
+template <int NT, int R, int E, class F>
+__device__ __forceinline__ void over_chunks(int at, int end, F &&f) {
+    const uint32_t own = threadIdx.x * E;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int base = at + r * NT * E;
+        if (base + NT * E <= end)
+            f(r, base, own, E);
+        else
+            f(r, base, own, end - (base + static_cast<int>(own)));
+    }
+}
+// Loss alone: the row streams by, kAhead chunks of each thread in flight.
+template <class T, int NT, bool kHard>
+__global__ __launch_bounds__(NT) void distill_loss_kernel(Args a) {
+    using C = Chunk<T>;
+    constexpr int E = C::kElems, NW = NT / 64, kStep = kAhead * NT * E;
+    __shared__ float red[2][NW * 3];
+    BlockSum<NW, 3> block(red);
+    const int64_t row = blockIdx.x;
+    const int vocab = static_cast<int>(a.vocab);
+    const auto *z = static_cast<const typename T::Raw *>(a.logits) + row * a.ld_logits;
+    const float tau = float(a.temperature), c = kLog2e / tau;
+
+    C next[kAhead];
+    auto fetch = [&](int at) {
+        over_chunks<NT, kAhead, E>(at, vocab, [&](int r, int base, uint32_t own, int valid) {
+            next[r].load((z + base) + own, valid);
+        });
+    };
+    fetch(0);
+    Targets<NT, kHard> y;
+    float top[2];
+    top[1] = y.load(a, row, z);
+    Running<kHard> run;
+    for (int at = 0; at < vocab; at += kStep) {
+        C now[kAhead];
+#pragma unroll
+        for (int r = 0; r < kAhead; ++r) now[r] = next[r];
+        if (at + kStep < vocab) fetch(at + kStep);
+        take(run, now, c);
+    }
+    top[0] = run.top;
+    block.max(top);
+    run.rebase(top[0], c);
+    float sum[3] = {run.sum, y.weigh(top[1], c), run.hard};
+    block.sum(sum);
+    const float kl = block.sum(y.divergence(tau, top[1], sum[1], top[0], sum[0]));
+    if (threadIdx.x == 0)
+        write_row<kHard>(a, row, kl, top[0], sum[0], sum[2], sum[1], y.label, y.z_label);
+}
+
+// Loss and gradient: NT threads hold R chunks each of the row in registers, 16 waves a
+// compute unit whatever NT is.
+template <class T, int NT, int R, bool kHard>
+__global__ __launch_bounds__(NT, 4) void distill_both_kernel(Args a) {
     using Raw = typename T::Raw;
     using C = Chunk<T>;
-    constexpr int E = C::kElems, NW = NT / 64, kTops = kMaxTop / NT;
+    constexpr int E = C::kElems, NW = NT / 64, kHeld = R * NT * E;
     __shared__ float red[2][NW * 3];
     __shared__ int entry_at[kMaxTop + 1];
     __shared__ float entry_amount[kMaxTop + 1];
     BlockSum<NW, 3> block(red);
-    const int tid = threadIdx.x;
     const int64_t row = blockIdx.x;
-    const int vocab = static_cast<int>(a.vocab), k = static_cast<int>(a.k);
+    const int vocab = static_cast<int>(a.vocab);
     const Raw *z = static_cast<const Raw *>(a.logits) + row * a.ld_logits;
     const float tau = float(a.temperature), lam = kHard ? float(a.label_weight) : 0.0f;
     const float c = kLog2e / tau;  // exponents in powers of two
 
-    C zr[R];
+    C held[R];
+    over_chunks<NT, R, E>(0, vocab, [&](int r, int base, uint32_t own, int valid) {
+        held[r].load((z + base) + own, valid);
+    });
+    Targets<NT, kHard> y;
+    float top[2];
+    top[1] = y.load(a, row, z);
+    Running<kHard> run;
+    static_assert(R % kAhead == 0, "whole groups");
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int at = (r * NT + tid) * E;
-        zr[r].load(z + at, vocab - at);
+    for (int r = 0; r < R; r += kAhead) take(run, held + r, c);
+    for (int at = kHeld; at < vocab; at += kAhead * NT * E) {  // what registers do not hold
+        C x[kAhead];
+        over_chunks<NT, kAhead, E>(at, vocab, [&](int r, int base, uint32_t own, int valid) {
+            x[r].load((z + base) + own, valid);
+        });
+        take(run, x, c);
     }
-    constexpr int kHeld = R * NT * E;  // elements of the row that registers hold
-
-    // the teacher's entries of this thread, and the student's logits there
-    float t[kTops], zk[kTops];
-    int index[kTops];
-    float top[2] = {kNegInf, kNegInf};  // of z, of t
-#pragma unroll
-    for (int j = 0; j < kTops; ++j) {
-        const int e = j * NT + tid;
-        index[j] = -1;
-        t[j] = kNegInf;
-        zk[j] = 0.0f;
-        if (e < k) {
-            const int64_t i = load_index(a, row * k + e);
-            if (i >= 0 && i < a.vocab) {
-                index[j] = static_cast<int>(i);
-                t[j] = load_any(a.teacher_logits, row * k + e, a.teacher_dtype);
-                zk[j] = to_f32(z[i]);
-            }
-            top[1] = fmaxf(top[1], t[j]);
-        }
-    }
-    int64_t label = -1;
-    float z_label = 0.0f;
-    if constexpr (kHard) {
-        label = a.labels[row];
-        if (label < 0 || label >= a.vocab) label = -1;
-        if (label >= 0) z_label = to_f32(z[label]);
-    }
-
-    // maxima; of the part past the registers a running sum too
-    float run_max = kNegInf, run_sum = 0.0f, run_hard = 0.0f;
-    if constexpr (MODE != kGradFromStats) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float f[E];
-            zr[r].get(f);
-#pragma unroll
-            for (int i = 0; i < E; ++i) top[0] = fmaxf(top[0], f[i]);
-        }
-        for (int at = kHeld + tid * E; at < vocab; at += NT * E) {
-            C x;
-            float f[E];
-            x.load(z + at, vocab - at);
-            x.get(f);
-            float m = run_max;
-#pragma unroll
-            for (int i = 0; i < E; ++i) m = fmaxf(m, f[i]);
-            if (m > run_max) {
-                run_sum *= exp2_hw((run_max - m) * c);
-                if constexpr (kHard) run_hard *= exp2_hw((run_max - m) * kLog2e);
-                run_max = m;
-            }
-            if (run_max > kNegInf) {
-#pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    run_sum += exp2_hw((f[i] - run_max) * c);
-                    if constexpr (kHard) run_hard += exp2_hw((f[i] - run_max) * kLog2e);
-                }
-            } else {  // −inf so far, or a NaN, which the maximum passes over
-#pragma unroll
-                for (int i = 0; i < E; ++i) run_sum += f[i] != f[i] ? f[i] : 0.0f;
-            }
-        }
-        top[0] = fmaxf(top[0], run_max);
-    }
+    top[0] = run.top;
     block.max(top);
-    const float t_max = top[1];
-    float z_max = top[0];
-
-    float sum[3] = {0.0f, 0.0f, 0.0f};  // of the student at τ, of the teacher, of the student at 1
-    float pe[kTops];
-#pragma unroll
-    for (int j = 0; j < kTops; ++j) {
-        pe[j] = index[j] >= 0 && t_max > kNegInf ? exp2_hw((t[j] - t_max) * c) : 0.0f;
-        if (index[j] >= 0 && t[j] != t[j]) pe[j] = t[j];
-        sum[1] += pe[j];
-    }
-    if constexpr (MODE != kGradFromStats) {
-        if (run_max > kNegInf) {
-            sum[0] = run_sum * exp2_hw((run_max - z_max) * c);
-            if constexpr (kHard) sum[2] = run_hard * exp2_hw((run_max - z_max) * kLog2e);
-        } else {
-            sum[0] = run_sum;
-            if constexpr (kHard) sum[2] = run_sum;
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float f[E];
-            zr[r].get(f);
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                sum[0] += exp2_hw((f[i] - z_max) * c);
-                if constexpr (kHard) sum[2] += exp2_hw((f[i] - z_max) * kLog2e);
-            }
-        }
-    }
+    run.rebase(top[0], c);
+    float sum[3] = {run.sum, y.weigh(top[1], c), run.hard};
+    forget<R>(held);
     block.sum(sum);
-    float inv_sum, inv_hard = 0.0f;
-    if constexpr (MODE == kGradFromStats) {
-        z_max = a.stats[4 * row];
-        inv_sum = a.stats[4 * row + 1];
-        inv_hard = a.stats[4 * row + 2];
-    } else {
-        inv_sum = 1.0f / sum[0];
-        if constexpr (kHard) inv_hard = 1.0f / sum[2];
-    }
-    const bool taught = sum[1] != 0.0f;
-    const float inv_teacher = taught ? 1.0f / sum[1] : 0.0f;
+    const float kl = block.sum(y.divergence(tau, top[1], sum[1], top[0], sum[0]));
+    if (threadIdx.x == 0)
+        write_row<kHard>(a, row, kl, top[0], sum[0], sum[2], sum[1], y.label, y.z_label);
 
-    if constexpr (MODE != kGradFromStats) {
-        // τ²·p·(log p − log q), the differences of logits scaled by τ alone: neither overflows
-        // where the loss does not
-        const float logs = tau * (logf(sum[0]) - (taught ? logf(sum[1]) : 0.0f));
-        float kl[1] = {0.0f};
+    const bool taught = sum[1] != 0.0f;
+    const float g = a.grad_loss ? a.grad_loss[row] : float(a.grad_value);
+    const float soft = taught ? (1.0f - lam) * tau : 0.0f;
+    const Slope<kHard> slope{top[0], c, g * soft * (1.0f / sum[0]),
+                             kHard && y.label >= 0 ? g * lam * (1.0f / sum[2]) : 0.0f};
+    Raw *out = static_cast<Raw *>(a.grad) + row * a.ld_grad;
+    over_chunks<NT, R, E>(0, vocab, [&](int r, int base, uint32_t own, int valid) {
+        float f[E];
+        held[r].get(f);
 #pragma unroll
-        for (int j = 0; j < kTops; ++j) {
-            const float p = pe[j] * inv_teacher;
-            if (p != 0.0f)
-                kl[0] += p * (tau * (((t[j] - t_max) - (zk[j] - z_max)) + logs));
-        }
-        block.sum(kl);
-        if (tid == 0) {
-            float loss = (1.0f - lam) * kl[0];
-            if constexpr (kHard)
-                if (label >= 0) loss += lam * (logf(sum[2]) - (z_label - z_max));
-            a.loss[row] = loss;
-            if (a.stats) {
-                a.stats[4 * row] = z_max;
-                a.stats[4 * row + 1] = inv_sum;
-                a.stats[4 * row + 2] = inv_hard;
-                a.stats[4 * row + 3] = 0.0f;
-            }
-        }
+        for (int i = 0; i < E; ++i) f[i] = slope(f[i]);
+        C x;
+        x.set(f);
+        x.store((out + base) + own, valid);
+        chunk_done();
+    });
+    for (int at = kHeld + threadIdx.x * E; at < vocab; at += NT * E) {
+        C x;
+        float f[E];
+        x.load(z + at, vocab - at);
+        x.get(f);
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[i] = slope(f[i]);
+        x.set(f);
+        x.store(out + at, vocab - at);
     }
-    if constexpr (MODE != kLoss) {
-        const float g = a.grad_loss ? a.grad_loss[row] : float(a.grad_value);
-        const float soft = taught ? (1.0f - lam) * tau : 0.0f;
-        const float f_soft = g * soft * inv_sum, f_hard = label >= 0 ? g * lam * inv_hard : 0.0f;
-        auto softmax = [&](float x) {
-            float d = f_soft * exp2_hw((x - z_max) * c);
-            if constexpr (kHard) d = fmaf(f_hard, exp2_hw((x - z_max) * kLog2e), d);
-            return d;
-        };
-        Raw *out = static_cast<Raw *>(a.grad) + row * a.ld_grad;
+    overwrite_entries<T, NT, kHard>(a, y, slope, g, soft, taught ? 1.0f / sum[1] : 0.0f, out, 0,
+                                    vocab, entry_at, entry_amount);
+}
+
+// Gradient from a forward pass's stats: no sums over the row, which streams by; blockIdx.y
+// takes the columns [y·width, (y + 1)·width).
+constexpr int kGradThreads = 256;
+template <class T, bool kHard>
+__global__ __launch_bounds__(kGradThreads) void distill_grad_kernel(Args a, int width) {
+    using Raw = typename T::Raw;
+    using C = Chunk<T>;
+    constexpr int NT = kGradThreads, E = C::kElems, NW = NT / 64, kStep = kAhead * NT * E;
+    __shared__ float red[2][NW];
+    __shared__ int entry_at[kMaxTop + 1];
+    __shared__ float entry_amount[kMaxTop + 1];
+    BlockSum<NW, 1> block(red);
+    const int64_t row = blockIdx.x;
+    const int lo = blockIdx.y * width;
+    const int hi = width < a.vocab - lo ? lo + width : static_cast<int>(a.vocab);
+    const Raw *z = static_cast<const Raw *>(a.logits) + row * a.ld_logits;
+    Raw *out = static_cast<Raw *>(a.grad) + row * a.ld_grad;
+    const float tau = float(a.temperature), lam = kHard ? float(a.label_weight) : 0.0f;
+    const float c = kLog2e / tau;
+
+    C next[kAhead];
+    auto fetch = [&](int at) {
+        over_chunks<NT, kAhead, E>(at, hi, [&](int r, int base, uint32_t own, int valid) {
+            next[r].load((z + base) + own, valid);
+        });
+    };
+    fetch(lo);
+    Targets<NT, kHard> y;
+    float t_max[1] = {y.load(a, row, z)};
+    block.max(t_max);
+    y.weigh(t_max[0], c);
+    const float inv_teacher = a.stats[4 * row + 3];
+    const bool taught = inv_teacher != 0.0f;
+    const float g = a.grad_loss ? a.grad_loss[row] : float(a.grad_value);
+    const float soft = taught ? (1.0f - lam) * tau : 0.0f;
+    const Slope<kHard> slope{a.stats[4 * row], c, g * soft * a.stats[4 * row + 1],
+                             kHard && y.label >= 0 ? g * lam * a.stats[4 * row + 2] : 0.0f};
+    for (int at = lo; at < hi; at += kStep) {
+        C now[kAhead];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int at = (r * NT + tid) * E;
+        for (int r = 0; r < kAhead; ++r) now[r] = next[r];
+        if (at + kStep < hi) fetch(at + kStep);
+        over_chunks<NT, kAhead, E>(at, hi, [&](int r, int base, uint32_t own, int valid) {
             float f[E];
-            zr[r].get(f);
+            now[r].get(f);
 #pragma unroll
-            for (int i = 0; i < E; ++i) f[i] = softmax(f[i]);
-            zr[r].set(f);
-            zr[r].store(out + at, vocab - at);
-        }
-        for (int at = kHeld + tid * E; at < vocab; at += NT * E) {
-            C x;
-            float f[E];
-            x.load(z + at, vocab - at);
-            x.get(f);
-#pragma unroll
-            for (int i = 0; i < E; ++i) f[i] = softmax(f[i]);
-            x.set(f);
-            x.store(out + at, vocab - at);
-        }
-        // what the entries take away, then their elements once more
-#pragma unroll
-        for (int j = 0; j < kTops; ++j) {
-            const int e = j * NT + tid;
-            if (e < k) {
-                entry_at[e] = index[j];
-                entry_amount[e] = soft * (pe[j] * inv_teacher);
-            }
-        }
-        if (tid == 0) {
-            entry_at[k] = static_cast<int>(label);
-            entry_amount[k] = label >= 0 ? lam : 0.0f;
-        }
-        __syncthreads();
-        const int entries = k + (kHard ? 1 : 0);
-        auto overwrite = [&](int at, float x) {
-            float amount = 0.0f;
-#pragma unroll 8
-            for (int e = 0; e < entries; ++e) amount += entry_at[e] == at ? entry_amount[e] : 0.0f;
-            const float d = softmax(x) - g * amount;
-            if constexpr (E == 8)
-                out[at] = f32_to_bf16_bits(d);
-            else
-                out[at] = d;
-        };
-#pragma unroll
-        for (int j = 0; j < kTops; ++j)
-            if (index[j] >= 0) overwrite(index[j], zk[j]);
-        if constexpr (kHard)
-            if (tid == NT - 1 && label >= 0) overwrite(static_cast<int>(label), z_label);
+            for (int i = 0; i < E; ++i) f[i] = slope(f[i]);
+            now[r].set(f);
+            now[r].store((out + base) + own, valid);
+            chunk_done();
+        });
     }
+    overwrite_entries<T, NT, kHard>(a, y, slope, g, soft, inv_teacher, out, lo, hi,
+                                    entry_at, entry_amount);
 }
 
 int check(const Args *a) {
@@ -341,31 +493,66 @@ int check(const Args *a) {
     return MUON_POLAR_OK;
 }
 
-// Threads and register chunks by the row's bytes: the fewest chunks that hold it, 256
-// threads up to 32 KiB and 1024 beyond.
-template <class T, int MODE, bool kHard>
-void launch(const Args &a, hipStream_t stream) {
-    const int64_t bytes = a.vocab * int64_t(sizeof(typename T::Raw));
+using std::integral_constant;
+
+// Threads of a row: rows that fill the card take as few as hold them with up to 16 chunks
+// each, so that several workgroups share a compute unit and one's loads and stores run
+// beside another's sums; fewer rows take 1024 threads, and the row arrives sooner.
+int row_threads(const Args &a, int64_t chunks, int cus) {
+    const bool many = a.rows >= 2 * int64_t(cus);
+    if (chunks <= 256 * 4 || (many && chunks <= 256 * 16)) return 256;
+    return many && chunks <= 512 * 16 ? 512 : 1024;
+}
+template <class T>
+int64_t row_chunks(const Args &a) {
+    return (a.vocab * int64_t(sizeof(typename T::Raw)) + 15) / 16;
+}
+
+template <class T, bool kHard>
+void launch_loss(const Args &a, int cus, hipStream_t stream) {
     const dim3 grid(static_cast<uint32_t>(a.rows));
-    auto go = [&](auto nt, auto r) {
-        distill_kernel<T, decltype(nt)::value, decltype(r)::value, MODE, kHard>
-            <<<grid, decltype(nt)::value, 0, stream>>>(a);
+    const int nt = row_threads(a, row_chunks<T>(a), cus);
+    if (nt == 256) distill_loss_kernel<T, 256, kHard><<<grid, nt, 0, stream>>>(a);
+    else if (nt == 512) distill_loss_kernel<T, 512, kHard><<<grid, nt, 0, stream>>>(a);
+    else distill_loss_kernel<T, 1024, kHard><<<grid, nt, 0, stream>>>(a);
+}
+template <class T, bool kHard>
+void launch_both(const Args &a, int cus, hipStream_t stream) {
+    const int64_t chunks = row_chunks<T>(a);
+    const int nt = row_threads(a, chunks, cus);
+    const dim3 grid(static_cast<uint32_t>(a.rows));
+    auto go = [&](auto threads, auto r) {
+        distill_both_kernel<T, decltype(threads)::value, decltype(r)::value, kHard>
+            <<<grid, nt, 0, stream>>>(a);
     };
-    using std::integral_constant;
-    if (bytes <= 256 * 2 * 16) go(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-    else if (bytes <= 256 * 8 * 16) go(integral_constant<int, 256>{}, integral_constant<int, 8>{});
-    else if (bytes <= 1024 * 4 * 16) go(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
-    else if (bytes <= 1024 * 8 * 16) go(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
+    if (nt == 256 && chunks <= 256 * 4) go(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+    else if (nt == 256 && chunks <= 256 * 8) go(integral_constant<int, 256>{}, integral_constant<int, 8>{});
+    else if (nt == 256) go(integral_constant<int, 256>{}, integral_constant<int, 16>{});
+    else if (nt == 512) go(integral_constant<int, 512>{}, integral_constant<int, 16>{});
+    else if (chunks <= 1024 * 8) go(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
     else go(integral_constant<int, 1024>{}, integral_constant<int, 16>{});
 }
-template <int MODE>
-void launch(const Args &a, hipStream_t stream) {
-    const bool hard = a.labels != nullptr;
-    if (a.logits_dtype == MUON_TRAIN_BF16)
-        hard ? launch<Bf16, MODE, true>(a, stream) : launch<Bf16, MODE, false>(a, stream);
-    else
-        hard ? launch<F32, MODE, true>(a, stream) : launch<F32, MODE, false>(a, stream);
+// Gradient alone: rows are cut where there are too few to fill the card, into parts of 16
+// KiB at least.
+template <class T, bool kHard>
+void launch_grad(const Args &a, int cus, hipStream_t stream) {
+    const int64_t least = 16384 / int64_t(sizeof(typename T::Raw));
+    int64_t parts = (8 * int64_t(cus) + a.rows - 1) / a.rows;
+    const int64_t most = (a.vocab + least - 1) / least;
+    parts = parts < most ? parts : most;
+    int64_t width = (a.vocab + parts - 1) / parts;
+    width = (width + 7) / 8 * 8;  // parts begin where 16-byte chunks do
+    const dim3 grid(static_cast<uint32_t>(a.rows), static_cast<uint32_t>((a.vocab + width - 1) / width));
+    distill_grad_kernel<T, kHard><<<grid, kGradThreads, 0, stream>>>(a, static_cast<int>(width));
 }
+#define MUON_TRAIN_LAUNCH(which)                                                              \
+    do {                                                                                      \
+        const bool hard = args->labels != nullptr;                                            \
+        if (args->logits_dtype == MUON_TRAIN_BF16)                                            \
+            hard ? which<Bf16, true>(*args, cus, stream) : which<Bf16, false>(*args, cus, stream); \
+        else                                                                                  \
+            hard ? which<F32, true>(*args, cus, stream) : which<F32, false>(*args, cus, stream);   \
+    } while (0)
 
 }  // namespace
 
@@ -377,10 +564,12 @@ extern "C" int muon_train_distill_forward(const muon_train_distill_args *args, h
     const int st = check(args);
     if (st != MUON_POLAR_OK || args->rows == 0) return st;
     if (!args->loss) return invalid("distill: null output");
+    const int cus = compute_units();
+    if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "distill: no device");
     if (args->grad)
-        launch<kLossAndGrad>(*args, stream);
+        MUON_TRAIN_LAUNCH(launch_both);
     else
-        launch<kLoss>(*args, stream);
+        MUON_TRAIN_LAUNCH(launch_loss);
     return launched("distill_forward");
 }
 
@@ -388,6 +577,8 @@ extern "C" int muon_train_distill_backward(const muon_train_distill_args *args, 
     const int st = check(args);
     if (st != MUON_POLAR_OK || args->rows == 0) return st;
     if (!args->grad || !args->stats) return invalid("distill: null output");
-    launch<kGradFromStats>(*args, stream);
+    const int cus = compute_units();
+    if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "distill: no device");
+    MUON_TRAIN_LAUNCH(launch_grad);
     return launched("distill_backward");
 }
