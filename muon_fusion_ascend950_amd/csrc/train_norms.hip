@@ -26,6 +26,13 @@ namespace {
 
 using Args = muon_train_norms_args;
 
+// Over a wave, in a fixed order; the same in every lane.
+__device__ __forceinline__ double wave_total(double v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
+    return v;
+}
+
 __device__ __forceinline__ int clamp8(int64_t n) { return n < 0 ? 0 : n > 8 ? 8 : int(n); }
 
 // NT threads take a row, V pieces of 8 columns each: thread t has the pieces t, t + NT, ..
@@ -117,8 +124,8 @@ __global__ __launch_bounds__(NT) void norms_forward_kernel(Args a) {
     }
 }
 
-// The column sums a workgroup of the backward pass leaves, [groups][sums][d] fp32, then
-// one word a group for a scalar scale's gradient.
+// What a workgroup of the backward pass leaves: one fp64 word for a scalar scale's gradient
+// [groups], then its column sums [groups][sums][d] fp32.
 enum { kSumPost = 0, kSumPre = 1, kSumScale = 2 };
 
 struct BackwardPlan {
@@ -129,17 +136,29 @@ struct BackwardPlan {
     size_t bytes;              // workspace
 };
 
-template <class TY, class TR, int NT, int V>
-__global__ __launch_bounds__(NT) void norms_backward_kernel(Args a, BackwardPlan plan, float *part,
-                                                            float *part_scale) {
+// kGeneral: a gate of y's shape or a scale vector, whose rows and columns have values of
+// their own; without, the gate that rows share is folded into post_weight, a token's is one
+// number (it leaves the row's sum Σ dn·n, taken before it, as the gate's own gradient), and
+// the scale is one number.
+//
+// Where registers allow (one piece a thread, not kGeneral) the next row's pieces are under way
+// while a row is worked on, whose two sums each wait for the whole workgroup: 16384 rows of
+// 4096 in bf16 take 165 us, without 181 to 195 (805 MB: 4.9 TB/s).
+template <class TY, class TR, int NT, int V, bool kGeneral>
+__global__ __launch_bounds__(NT, V == 1 && !kGeneral ? 4 : 1) void norms_backward_kernel(Args a, BackwardPlan plan,
+                                                                           float *part,
+                                                                           double *part_scale) {
     using RawY = typename TY::Raw;
     using RawR = typename TR::Raw;
-    __shared__ float red[2][NT / 64 * 3];
-    BlockSum<NT / 64, 3> block(red);
+    __shared__ float red[2][NT / 64];
+    BlockSum<NT / 64, 1> block(red);
     const int tid = threadIdx.x;
     const float inv_d = 1.0f / float(a.d);
     const float number = a.scale_kind == MUON_TRAIN_SCALE_SCALAR ? a.scale[0] : float(a.scale_value);
     const bool seq_gate = a.gate_kind == MUON_TRAIN_GATE_SEQUENCE;
+    const bool token_gate = a.gate_kind == MUON_TRAIN_GATE_TOKEN;
+    const bool full_gate = kGeneral && a.gate_kind == MUON_TRAIN_GATE_FULL;
+    const bool vector_scale = kGeneral && a.scale_kind == MUON_TRAIN_SCALE_VECTOR;
     // Of one channel, dn − n·mean(dn·n) = dn·(1 − n²) = dn·eps·ρ² is all cancellation in
     // fp32: it is formed as that product.
     const bool single = a.d == 1;
@@ -156,107 +175,117 @@ __global__ __launch_bounds__(NT) void norms_backward_kernel(Args a, BackwardPlan
     }
 
     int col[V], valid[V];
-    float w1[V][8], w2[V][8], gate[V][8], sc[V][8];
-    float sum_post[V][8], sum_pre[V][8], sum_scale[V][8], scale_total = 0.0f;
+    float w1[V][8], w2[V][8], sum_post[V][8], sum_pre[V][8];
+    float sum_scale[kGeneral ? V : 1][8];
+    double scale_total = 0.0;  // a scalar scale's gradient: one sum over all elements, which cancel
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         col[v] = (v * NT + tid) * 8;
         valid[v] = clamp8(a.d - col[v]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            w1[v][i] = w2[v][i] = gate[v][i] = 1.0f;
-            sc[v][i] = number;
-            sum_post[v][i] = sum_pre[v][i] = sum_scale[v][i] = 0.0f;
+            w1[v][i] = w2[v][i] = 1.0f;
+            sum_post[v][i] = sum_pre[v][i] = 0.0f;
+            if (kGeneral) sum_scale[v][i] = 0.0f;
         }
         if (a.post_weight) load8_any(a.post_weight, col[v], valid[v], a.weight_dtype, w1[v]);
         if (a.pre_weight) load8_any(a.pre_weight, col[v], valid[v], a.weight_dtype, w2[v]);
-        if (a.scale_kind == MUON_TRAIN_SCALE_VECTOR)
-            load8_any(a.scale, col[v], valid[v], MUON_TRAIN_F32, sc[v]);
-        if (a.gate_kind == MUON_TRAIN_GATE_CHANNEL || seq_gate)
-            load8_any(a.gate, sequence * a.d + col[v], valid[v], a.gate_dtype, gate[v]);
+        if (a.gate_kind == MUON_TRAIN_GATE_CHANNEL || seq_gate) {
+            float g[8];
+            load8_any(a.gate, sequence * a.d + col[v], valid[v], a.gate_dtype, g);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w1[v][i] *= g[i];
+        }
     }
-    for (int64_t row = first; row < end; row += step) {
-        Piece<TY> py[V], ph[V];
-        Piece<TR> pr[V], pt[V];
-        const float rho1 = a.stats[2 * row], rho2 = a.stats[2 * row + 1];
+    const bool has_dh = a.d_normed && a.pre_norm, has_dt = a.d_residual_out != nullptr;
+    struct Row {
+        Piece<TY> y[V], h[V];
+        Piece<TR> r[V], t[V];
+        float rho1, rho2, gate;
+    };
+    auto fetch = [&](int64_t row, Row &x) {
+        x.rho1 = a.stats[2 * row];
+        x.rho2 = a.stats[2 * row + 1];
+        x.gate = token_gate ? load_any(a.gate, row, a.gate_dtype) : 1.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            py[v].load(static_cast<const RawY *>(a.y) + row * a.ld_y + col[v], valid[v]);
-            pr[v].load(static_cast<const RawR *>(a.residual) + row * a.ld_residual + col[v], valid[v]);
-            if (a.d_normed && a.pre_norm)
-                ph[v].load(static_cast<const RawY *>(a.d_normed) + row * a.d + col[v], valid[v]);
-            else
-                ph[v].zero();
-            if (a.d_residual_out)
-                pt[v].load(static_cast<const RawR *>(a.d_residual_out) + row * a.d + col[v], valid[v]);
-            else
-                pt[v].zero();
+            x.y[v].load(static_cast<const RawY *>(a.y) + row * a.ld_y + col[v], valid[v]);
+            x.r[v].load(static_cast<const RawR *>(a.residual) + row * a.ld_residual + col[v], valid[v]);
+            if (has_dh) x.h[v].load(static_cast<const RawY *>(a.d_normed) + row * a.d + col[v], valid[v]);
+            else x.h[v].zero();
+            if (has_dt) x.t[v].load(static_cast<const RawR *>(a.d_residual_out) + row * a.d + col[v], valid[v]);
+            else x.t[v].zero();
         }
-        float token = 1.0f;
-        if (a.gate_kind == MUON_TRAIN_GATE_TOKEN) {
-            token = load_any(a.gate, row, a.gate_dtype);
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) gate[v][i] = token;
-        } else if (a.gate_kind == MUON_TRAIN_GATE_FULL) {
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-                load8_any(a.gate, row * a.d + col[v], valid[v], a.gate_dtype, gate[v]);
-        }
-        float n[V][8], m[V][8], dm[V][8];
+    };
+    constexpr bool kAhead = V == 1 && !kGeneral;
+    Row next;
+    if (kAhead && first < end) fetch(first, next);
+    for (int64_t row = first; row < end; row += step) {
+        if (!kAhead) fetch(row, next);
+        const Row x = next;
+        if (kAhead && row + step < end) fetch(row + step, next);
+        const float rho1 = x.rho1, rho2 = x.rho2;
+        float n[V][8], m[V][8], dm[V][8], gate[kGeneral ? V : 1][8], sc[kGeneral ? V : 1][8];
         float dot = 0.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float r[8], dh[8];
-            py[v].get(n[v]);
-            pr[v].get(r);
-            ph[v].get(dh);
+            x.y[v].get(n[v]);
+            x.r[v].get(r);
+            x.h[v].get(dh);
+            if constexpr (kGeneral) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) gate[v][i] = 1.0f, sc[v][i] = number;
+                if (full_gate) load8_any(a.gate, row * a.d + col[v], valid[v], a.gate_dtype, gate[v]);
+                if (vector_scale) load8_any(a.scale, col[v], valid[v], MUON_TRAIN_F32, sc[v]);
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 n[v][i] *= rho1;
-                m[v][i] = fmaf(sc[v][i], r[i], gate[v][i] * (n[v][i] * w1[v][i])) * rho2;
+                float u = x.gate * (n[v][i] * w1[v][i]);
+                if constexpr (kGeneral) u *= gate[v][i];
+                m[v][i] = fmaf(kGeneral ? sc[v][i] : number, r[i], u) * rho2;
                 dm[v][i] = dh[i] * w2[v][i];
                 dot = fmaf(dm[v][i], m[v][i], dot);
                 sum_pre[v][i] = fmaf(dh[i], m[v][i], sum_pre[v][i]);
             }
         }
         const float mean2 = a.pre_norm && !single ? block.sum(dot) * inv_d : 0.0f;
-        const float f2 = single ? rho2 * eps * rho2 * rho2 : rho2;
-        float s[2] = {0.0f, 0.0f};
-        float total_scale = 0.0f;
+        const float f2 = !a.pre_norm ? 0.0f : single ? rho2 * eps * rho2 * rho2 : rho2;
+        float row_dot = 0.0f, row_scale = 0.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float r[8], dt[8], out[8], dgate[8];
-            pr[v].get(r);
-            pt[v].get(dt);
+            x.r[v].get(r);
+            x.t[v].get(dt);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float d_total =
-                    a.pre_norm ? fmaf(f2, dm[v][i] - m[v][i] * mean2, dt[i]) : dt[i];
-                out[i] = sc[v][i] * d_total;
-                total_scale = fmaf(d_total, r[i], total_scale);
-                sum_scale[v][i] = fmaf(d_total, r[i], sum_scale[v][i]);
+                const float d_total = fmaf(f2, dm[v][i] - m[v][i] * mean2, dt[i]);
+                out[i] = (kGeneral ? sc[v][i] : number) * d_total;
+                row_scale = fmaf(d_total, r[i], row_scale);
                 const float with_n = d_total * n[v][i];
-                dgate[i] = with_n * w1[v][i];
-                s[1] += dgate[i];
-                const bool shared = a.gate_kind <= MUON_TRAIN_GATE_SEQUENCE;
-                sum_post[v][i] += shared ? with_n : with_n * gate[v][i];
-                dm[v][i] = d_total * gate[v][i] * w1[v][i];  // dn from here on
-                s[0] = fmaf(dm[v][i], n[v][i], s[0]);
+                dm[v][i] = d_total * w1[v][i];  // dn from here on, but for the token's gate
+                float weighed = with_n * x.gate;
+                if constexpr (kGeneral) {
+                    sum_scale[v][i] = fmaf(d_total, r[i], sum_scale[v][i]);
+                    dgate[i] = with_n * w1[v][i];
+                    weighed *= gate[v][i];
+                    dm[v][i] *= gate[v][i];
+                }
+                sum_post[v][i] += weighed;
+                row_dot = fmaf(dm[v][i], n[v][i], row_dot);
             }
             Piece<TR> o;
             o.set(out);
             o.store(static_cast<RawR *>(a.d_residual) + row * a.d + col[v], valid[v]);
-            if (a.gate_kind == MUON_TRAIN_GATE_FULL && a.d_gate)
+            if (full_gate && a.d_gate)
                 store8_any(a.d_gate, row * a.d + col[v], valid[v], a.gate_dtype, dgate);
         }
-        scale_total += total_scale;
-        block.sum(s);
-        if (a.gate_kind == MUON_TRAIN_GATE_TOKEN && a.d_gate && tid == 0)
-            store_any(a.d_gate, row, a.gate_dtype, s[1]);
-        const float mean1 = a.post_norm && !single ? s[0] * inv_d : 0.0f;
-        const float f1 = a.post_norm && single ? rho1 * eps * rho1 * rho1 : rho1;
+        scale_total += row_scale;
+        row_dot = block.sum(row_dot);
+        if (token_gate && a.d_gate && tid == 0) store_any(a.d_gate, row, a.gate_dtype, row_dot);
+        const float mean1 = a.post_norm && !single ? row_dot * inv_d : 0.0f;
+        const float f1 = x.gate * (a.post_norm && single ? rho1 * eps * rho1 * rho1 : rho1);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float out[8];
@@ -272,11 +301,20 @@ __global__ __launch_bounds__(NT) void norms_backward_kernel(Args a, BackwardPlan
     for (int v = 0; v < V; ++v) {
         store8_any(mine, kSumPost * a.d + col[v], valid[v], MUON_TRAIN_F32, sum_post[v]);
         store8_any(mine, kSumPre * a.d + col[v], valid[v], MUON_TRAIN_F32, sum_pre[v]);
-        if (plan.sums > kSumScale)
-            store8_any(mine, kSumScale * a.d + col[v], valid[v], MUON_TRAIN_F32, sum_scale[v]);
+        if constexpr (kGeneral)
+            if (plan.sums > kSumScale)
+                store8_any(mine, kSumScale * a.d + col[v], valid[v], MUON_TRAIN_F32, sum_scale[v]);
     }
-    const float t = block.sum(scale_total);
-    if (tid == 0) part_scale[blockIdx.x] = t;
+    if (a.scale_kind != MUON_TRAIN_SCALE_SCALAR) return;
+    __shared__ double totals[NT / 64];
+    scale_total = wave_total(scale_total);
+    if ((tid & 63) == 0) totals[tid >> 6] = scale_total;
+    __syncthreads();
+    if (tid == 0) {
+        double t = totals[0];
+        for (int w = 1; w < NT / 64; ++w) t += totals[w];
+        part_scale[blockIdx.x] = t;
+    }
 }
 
 // Adds the workgroups' column sums, in index order within each of 16 runs and then run by
@@ -284,16 +322,16 @@ __global__ __launch_bounds__(NT) void norms_backward_kernel(Args a, BackwardPlan
 constexpr int kFinishRuns = 16;
 __global__ __launch_bounds__(64 * kFinishRuns) void norms_finish_kernel(Args a, BackwardPlan plan,
                                                                         const float *part,
-                                                                        const float *part_scale) {
+                                                                        const double *part_scale) {
     __shared__ float red[kFinishRuns][64];
     const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
     const int64_t d = a.d, stride = plan.sums * d;
     if (int(blockIdx.y) == plan.sums) {  // a scalar scale's gradient
         if (blockIdx.x != 0 || run != 0) return;
-        float t = 0.0f;
+        double t = 0.0;
         for (int64_t g = lane; g < plan.groups; g += 64) t += part_scale[g];
         t = wave_total(t);
-        if (lane == 0) a.d_scale[0] = t;
+        if (lane == 0) a.d_scale[0] = static_cast<float>(t);
         return;
     }
     const int which = blockIdx.y;
@@ -314,7 +352,7 @@ __global__ __launch_bounds__(64 * kFinishRuns) void norms_finish_kernel(Args a, 
         const int64_t lo = g0 + run * share, hi = lo + share < g1 ? lo + share : g1;
         float t = 0.0f;
         if (in) {
-#pragma unroll 4
+#pragma unroll 8
             for (int64_t g = lo; g < hi; ++g) t += p[g * stride];
         }
         return over_runs(t);
@@ -336,31 +374,40 @@ __global__ __launch_bounds__(64 * kFinishRuns) void norms_finish_kernel(Args a, 
         }
         return;
     }
-    // a gate for each sequence: each run takes whole sequences
+    // a gate for each sequence: with 16 sequences or more each run takes whole ones, with
+    // fewer all runs share each
     const int64_t sequences = plan.groups / plan.groups_per_sequence;
     const float w = in && a.post_weight ? load_any(a.post_weight, c, a.weight_dtype) : 1.0f;
     float total = 0.0f;
-    if (in) {
-        for (int64_t b = run; b < sequences; b += kFinishRuns) {
+    auto finish_sequence = [&](int64_t b, float t) {
+        if (a.d_gate) store_any(a.d_gate, b * d + c, a.gate_dtype, t * w);
+        total = fmaf(t, load_any(a.gate, b * d + c, a.gate_dtype), total);
+    };
+    if (sequences >= kFinishRuns) {
+        for (int64_t b = run; in && b < sequences; b += kFinishRuns) {
             float t = 0.0f;
             const float *q = p + b * plan.groups_per_sequence * stride;
 #pragma unroll 4
             for (int64_t g = 0; g < plan.groups_per_sequence; ++g) t += q[g * stride];
-            if (a.d_gate) store_any(a.d_gate, b * d + c, a.gate_dtype, t * w);
-            total = fmaf(t, load_any(a.gate, b * d + c, a.gate_dtype), total);
+            finish_sequence(b, t);
+        }
+        total = over_runs(total);
+    } else {
+        for (int64_t b = 0; b < sequences; ++b) {
+            const float t = sum(b * plan.groups_per_sequence, (b + 1) * plan.groups_per_sequence);
+            if (in && run == 0) finish_sequence(b, t);
         }
     }
-    total = over_runs(total);
     if (in && run == 0 && a.d_post_weight) store_any(a.d_post_weight, c, a.weight_dtype, total);
 }
 
-// Threads and pieces of a row: one piece a thread up to 512 columns in one wave, two up to
-// 1024; then as many waves as two pieces a thread fill, so that weights and sums stay in
-// registers.
+// Threads and pieces of a row.  Forward: two pieces a thread from 512 columns on, up to 107
+// registers, 20 waves a compute unit.  Backward, which holds more: one piece as far as 1024
+// threads go.
 struct Shape {
     int nt, v;
 };
-Shape row_shape(int64_t d) {
+Shape forward_shape(int64_t d) {
     if (d <= 512) return {64, 1};
     if (d <= 1024) return {64, 2};
     if (d <= 2048) return {256, 1};
@@ -368,15 +415,33 @@ Shape row_shape(int64_t d) {
     if (d <= 8192) return {512, 2};
     return {1024, 2};
 }
+Shape backward_shape(int64_t d) {
+    if (d <= 512) return {64, 1};
+    if (d <= 1024) return {128, 1};
+    if (d <= 2048) return {256, 1};
+    if (d <= 4096) return {512, 1};
+    if (d <= 8192) return {1024, 1};
+    return {1024, 2};
+}
 
 template <class F>
-void with_shape(Shape s, F &&f) {
+void with_forward_shape(Shape s, F &&f) {
     using std::integral_constant;
     if (s.nt == 64 && s.v == 1) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
     else if (s.nt == 64) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
     else if (s.nt == 256 && s.v == 1) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
     else if (s.nt == 256) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
     else if (s.nt == 512) f(integral_constant<int, 512>{}, integral_constant<int, 2>{});
+    else f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+}
+template <class F>
+void with_backward_shape(Shape s, F &&f) {
+    using std::integral_constant;
+    if (s.nt == 64) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    else if (s.nt == 128) f(integral_constant<int, 128>{}, integral_constant<int, 1>{});
+    else if (s.nt == 256) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+    else if (s.nt == 512) f(integral_constant<int, 512>{}, integral_constant<int, 1>{});
+    else if (s.v == 1) f(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
     else f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
 }
 template <class F>
@@ -388,12 +453,12 @@ void with_types(const Args &a, F &&f) {
 }
 
 BackwardPlan backward_plan(const Args &a, int cus) {
-    const Shape s = row_shape(a.d);
+    const Shape s = backward_shape(a.d);
     BackwardPlan p{};
     p.nt = s.nt;
     p.v = s.v;
-    // workgroups that the card holds at once (about eight waves a compute unit)
-    const int64_t resident = int64_t(cus) * (512 / s.nt > 1 ? 512 / s.nt : 1);
+    // workgroups that the card holds at once, 16 waves a compute unit
+    const int64_t resident = int64_t(cus) * (1024 / s.nt);
     p.groups_per_sequence = 1;
     if (a.gate_kind == MUON_TRAIN_GATE_SEQUENCE && a.rows > 0) {
         const int64_t sequences = a.rows / a.rows_per_sequence;
@@ -404,7 +469,7 @@ BackwardPlan backward_plan(const Args &a, int cus) {
         p.groups = a.rows < resident ? a.rows : resident;
     }
     p.sums = a.scale_kind == MUON_TRAIN_SCALE_VECTOR ? 3 : 2;
-    p.bytes = sizeof(float) * size_t(p.groups) * (size_t(p.sums) * size_t(a.d) + 1);
+    p.bytes = size_t(p.groups) * (sizeof(double) + sizeof(float) * size_t(p.sums) * size_t(a.d));
     return p;
 }
 
@@ -460,12 +525,12 @@ extern "C" int muon_train_norms_forward(const muon_train_norms_args *args, hipSt
     if (!a.residual_out || (a.pre_norm && !a.normed)) return invalid("norms: null output");
     const int cus = compute_units();
     if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "norms: no device");
-    const Shape s = row_shape(a.d);
+    const Shape s = forward_shape(a.d);
     // as many workgroups as stay resident: each keeps its weights over its rows
     const int64_t resident = int64_t(cus) * (2048 / s.nt);
     const dim3 grid(static_cast<uint32_t>(a.rows < resident ? a.rows : resident));
     with_types(a, [&](auto ty, auto tr) {
-        with_shape(s, [&](auto nt, auto v) {
+        with_forward_shape(s, [&](auto nt, auto v) {
             norms_forward_kernel<decltype(ty), decltype(tr), decltype(nt)::value, decltype(v)::value>
                 <<<grid, s.nt, 0, stream>>>(a);
         });
@@ -494,16 +559,21 @@ extern "C" int muon_train_norms_backward(const muon_train_norms_args *args, void
     const BackwardPlan p = backward_plan(a, cus);
     if (workspace_bytes < p.bytes || (p.bytes > 0 && !workspace))
         return muon_polar::report(MUON_POLAR_ERR_WORKSPACE, "norms: workspace missing or too small");
-    if (reinterpret_cast<uintptr_t>(workspace) % 4 != 0)
-        return invalid("norms: workspace must be 4-byte aligned");
-    float *part = static_cast<float *>(workspace);
-    float *part_scale = part + p.groups * p.sums * a.d;
+    if (reinterpret_cast<uintptr_t>(workspace) % 8 != 0)
+        return invalid("norms: workspace must be 8-byte aligned");
+    double *part_scale = static_cast<double *>(workspace);
+    float *part = reinterpret_cast<float *>(part_scale + p.groups);
     if (a.rows > 0) {
         with_types(a, [&](auto ty, auto tr) {
-            with_shape({p.nt, p.v}, [&](auto nt, auto v) {
-                norms_backward_kernel<decltype(ty), decltype(tr), decltype(nt)::value,
-                                      decltype(v)::value>
-                    <<<dim3(static_cast<uint32_t>(p.groups)), p.nt, 0, stream>>>(a, p, part, part_scale);
+            with_backward_shape({p.nt, p.v}, [&](auto nt, auto v) {
+                const dim3 grid(static_cast<uint32_t>(p.groups));
+                constexpr int kNt = decltype(nt)::value, kV = decltype(v)::value;
+                if (a.gate_kind == MUON_TRAIN_GATE_FULL || a.scale_kind == MUON_TRAIN_SCALE_VECTOR)
+                    norms_backward_kernel<decltype(ty), decltype(tr), kNt, kV, true>
+                        <<<grid, p.nt, 0, stream>>>(a, p, part, part_scale);
+                else
+                    norms_backward_kernel<decltype(ty), decltype(tr), kNt, kV, false>
+                        <<<grid, p.nt, 0, stream>>>(a, p, part, part_scale);
             });
         });
         st = launched("norms_backward");
