@@ -156,6 +156,20 @@ typedef struct muon_train_fp8_matmul_args {
 } muon_train_fp8_matmul_args;
 int muon_train_fp8_matmul(const muon_train_fp8_matmul_args *args, hipStream_t stream);
 
+/* c = held(x) · wᵀ for up to 16 rows of x [m, cols], quantised in blocks of 1 x 128 in the
+ * same kernel: the bits of muon_train_fp8_quantize and muon_train_fp8_matmul.  w: rows of
+ * roundup(cols, 128) values, block_rows 128. */
+typedef struct muon_train_fp8_decode_args {
+    int64_t m, n, cols, ld_x; /* m: 0 to 16 */
+    const void *x;
+    int x_dtype;
+    muon_train_fp8_operand w;
+    void *c; /* [m, n] */
+    int64_t ldc;
+    int c_dtype;
+} muon_train_fp8_decode_args;
+int muon_train_fp8_decode(const muon_train_fp8_decode_args *args, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

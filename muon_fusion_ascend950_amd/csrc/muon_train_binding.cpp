@@ -429,9 +429,29 @@ at::Tensor result_like(const at::Tensor &x, int64_t n) {
 // y = x · wᵀ on a held weight.
 at::Tensor Fp8Linear(const at::Tensor &x, const at::Tensor &values, const at::Tensor &scales) {
     const c10::OptionalDeviceGuard device_guard(x.device());
+    at::Tensor y = result_like(x, values.size(0));
+    const int64_t rows = x.size(-1) > 0 ? x.numel() / x.size(-1) : 0;
+    if (rows <= 16) {  // quantised in the product's own kernel
+        Held w{values, scales};
+        muon_train_fp8_decode_args a{};
+        a.w = operand(w, x);
+        if (a.w.block_rows == kBlock) {
+            TORCH_CHECK(blocks(x.size(-1)) * kBlock == values.size(1), "fp8: operands of different width");
+            const Rows r = as_rows(x);
+            a.m = rows;
+            a.n = a.ldc = values.size(0);
+            a.cols = x.size(-1);
+            a.ld_x = r.ld;
+            a.x = r.t.data_ptr();
+            a.x_dtype = a.c_dtype = dtype_of(x, "fp8: a matrix to quantise");
+            a.c = y.data_ptr();
+            const int st = muon_train_fp8_decode(&a, stream_of(x));
+            TORCH_CHECK(st == MUON_POLAR_OK, "fp8: ", muon_polar_last_error());
+            return y;
+        }
+    }
     Held h;
     quantize(as_matrix(x), 1, &h, nullptr);
-    at::Tensor y = result_like(x, values.size(0));
     at::Tensor y2 = y.view({h.values.size(0), values.size(0)});
     matmul(h, {values, scales}, y2);
     return y;

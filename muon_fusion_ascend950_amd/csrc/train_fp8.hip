@@ -2,6 +2,8 @@
 // held so (include/muon_train.h; the formulas are there).
 #include "train_common.hpp"
 
+#include <type_traits>
+
 namespace muon_train {
 
 namespace {
@@ -405,6 +407,192 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
     }
 }
 
+// ------------------------------------------------------------------ few rows (decoding)
+// Up to 16 rows of a: the weight's bytes bound the product, and each crosses once.  A
+// workgroup of eight waves takes 16·NT output columns; the waves split K, so that one launch
+// has all of a 14336 x 4096 weight's loads under way at once, and their sums meet in LDS in
+// wave order.  A lane supplies row l % 16 of each operand, bytes 16·p .. + 15 and 64 + 16·p
+// .. + 15 of each block (p = l / 16): an instruction reads 64 bytes of a row in a line.
+//
+// X: the rows of a as they come (bf16 or fp32), or already held.  A wave quantises its own
+// part of K: a lane takes eight elements, 16 lanes a block, and the values pass through a
+// corner of LDS of the wave's own into the MFMA's order.  Loads return in order, so x is
+// asked for before the weight: quantising then runs beside the weight's loads.  (With each
+// lane quantising the 32 values that it feeds to the MFMA, behind the weight's loads: one
+// token through 14336 x 4096 took 17.3 us.)
+constexpr int kFewRows = 16;
+constexpr int kFewWaves = 8;
+
+struct Held {};
+struct DecodeArgs {
+    int64_t n, ld_x;
+    int m, cols, blocks;
+    const void *x;
+    const float *x_scales;  // held: element (row, block) at row + block·x_scale_col
+    int64_t x_scale_col;
+    muon_train_fp8_operand w;
+    void *c;
+    int64_t ldc;
+    int c_dtype;
+};
+
+constexpr int kFewBlocks = 4;                               // blocks of K a wave takes at a time
+constexpr int kFewPitch = kFewBlocks * kBlock + 16;         // bytes from row to row of held x in LDS
+constexpr int kFewCorner = kFewRows * (kFewPitch + 4 * kFewBlocks);  // of a wave
+
+// Quantises rows [t0, t0 + T) of x in the wave's blocks from kb on.
+template <class X, int T>
+struct FewRowsInput {
+    Piece<X> p[T];
+    __device__ __forceinline__ void load(const DecodeArgs &a, int t0, int kb, int end) {
+        const int lane = threadIdx.x & 63;
+        const int k = kb * kBlock + 8 * lane;
+        const int valid = k < end * kBlock ? a.cols - k : 0;
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            p[t].zero();
+            if (t0 + t < a.m)
+                p[t].load(static_cast<const typename X::Raw *>(a.x) + (t0 + t) * a.ld_x + k, valid);
+        }
+    }
+    __device__ __forceinline__ void store(const DecodeArgs &a, int t0, uint8_t *values, float *scales) const {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            if (t0 + t >= a.m) break;
+            float f[8], inv[8];
+            p[t].get(f);
+            uint32_t m = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = umax(m, magnitude(f[e]));
+            const float s = scale_of(row_umax(m)), r = 1.0f / s;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) inv[e] = r;
+            *reinterpret_cast<u32x2 *>(values + (t0 + t) * kFewPitch + 8 * lane) = to_fp8(f, inv);
+            if ((lane & 15) == 0) scales[(t0 + t) * kFewBlocks + (lane >> 4)] = s;
+        }
+    }
+};
+
+template <class X, bool kExact, int NT>
+__global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(DecodeArgs a) {
+    constexpr int U = kFewBlocks, kFirst = 4;  // rows of x whose loads go ahead of the weight's
+    constexpr bool kHeld = std::is_same_v<X, Held>;
+    constexpr int kSums = kFewWaves * NT * 64 * 16;
+    constexpr int kLds = kHeld || kFewWaves * kFewCorner < kSums ? kSums : kFewWaves * kFewCorner;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+    const int r = lane & 15, part = lane >> 4;
+    const int token = r < a.m ? r : a.m - 1;  // columns past the rows of x are dropped
+    const int64_t n0 = int64_t(blockIdx.x) * (16 * NT);
+    const int each = (a.blocks + kFewWaves - 1) / kFewWaves;
+    const int first = wave * each, end = first + each < a.blocks ? first + each : a.blocks;
+    const uint8_t *pw[NT];
+    const float *sw[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {  // rows past the end read the last one and are dropped
+        const int64_t n = n0 + 16 * t + r < a.n ? n0 + 16 * t + r : a.n - 1;
+        const int64_t block = (n0 + 16 * t < a.n ? n0 + 16 * t : a.n - 1) / kBlock;
+        pw[t] = static_cast<const uint8_t *>(a.w.values) + n * a.w.ld + 16 * part;
+        sw[t] = a.w.scales + block * a.w.scale_row;
+    }
+    uint8_t *const values = lds + wave * kFewCorner;
+    float *const scales = reinterpret_cast<float *>(values + kFewRows * kFewPitch);
+    f32x4 acc[NT] = {};
+    for (int kb = first; kb < end; kb += U) {
+        i32x4 xlo[U], xhi[U], lo[U][NT], hi[U][NT];
+        float sx[U];
+        auto weight = [&] {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (kb + u < end) {
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        lo[u][t] = *reinterpret_cast<const i32x4 *>(pw[t] + (kb + u) * kBlock);
+                        hi[u][t] = *reinterpret_cast<const i32x4 *>(pw[t] + (kb + u) * kBlock + 64);
+                    }
+                }
+        };
+        if constexpr (kHeld) {
+            const uint8_t *p = static_cast<const uint8_t *>(a.x) + token * a.ld_x + 16 * part;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (kb + u < end) {
+                    xlo[u] = *reinterpret_cast<const i32x4 *>(p + (kb + u) * kBlock);
+                    xhi[u] = *reinterpret_cast<const i32x4 *>(p + (kb + u) * kBlock + 64);
+                    sx[u] = a.x_scales[token + (kb + u) * a.x_scale_col];
+                }
+            weight();
+        } else {
+            for (int t0 = kFirst; t0 < a.m; t0 += kFirst) {
+                FewRowsInput<X, kFirst> x;
+                x.load(a, t0, kb, end);
+                x.store(a, t0, values, scales);
+            }
+            FewRowsInput<X, kFirst> x;
+            x.load(a, 0, kb, end);
+            __builtin_amdgcn_sched_barrier(0);
+            weight();
+            __builtin_amdgcn_sched_barrier(0);
+            x.store(a, 0, values, scales);
+            const uint8_t *p = values + token * kFewPitch + 16 * part;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                xlo[u] = *reinterpret_cast<const i32x4 *>(p + u * kBlock);
+                xhi[u] = *reinterpret_cast<const i32x4 *>(p + u * kBlock + 64);
+                sx[u] = scales[token * kFewBlocks + u];
+            }
+        }
+        auto whole = [](i32x4 l, i32x4 h) {
+            return i32x8{l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3]};
+        };
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (kb + u < end) {
+                Frag<kExact> fx;
+                fx.set(whole(xlo[u], xhi[u]));
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    Frag<kExact> fw;
+                    fw.set(whole(lo[u][t], hi[u][t]));
+                    const f32x4 p = multiply(fw, fx);
+                    const float s = sx[u] * sw[t][(kb + u) * a.w.scale_col];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(p[e], s, acc[t][e]);
+                }
+            }
+    }
+    f32x4 *const sums = reinterpret_cast<f32x4 *>(lds);
+    __syncthreads();  // every wave is done with its corner
+#pragma unroll
+    for (int t = 0; t < NT; ++t) sums[(wave * NT + t) * 64 + lane] = acc[t];
+    __syncthreads();
+    if (wave >= NT) return;
+    f32x4 total = sums[wave * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < kFewWaves; ++w) total += sums[(w * NT + wave) * 64 + lane];
+    const int64_t n = n0 + 16 * wave + 4 * part;
+    if (r < a.m && n < a.n) store4(a.c, r * a.ldc + n, a.n - n < 4 ? int(a.n - n) : 4, a.c_dtype, total);
+}
+
+// 32 columns a workgroup where that still fills the card (a lane's work on x then serves
+// twice the weight), else 16.
+template <class X>
+void launch_few_rows(const DecodeArgs &a, int cus, hipStream_t stream) {
+    const bool exact = a.c_dtype == MUON_TRAIN_F32;
+    const int threads = 64 * kFewWaves;
+    if (a.n >= 32 * int64_t(cus)) {
+        const dim3 grid(static_cast<uint32_t>((a.n + 31) / 32));
+        if (exact) few_rows_kernel<X, true, 2><<<grid, threads, 0, stream>>>(a);
+        else few_rows_kernel<X, false, 2><<<grid, threads, 0, stream>>>(a);
+    } else {
+        const dim3 grid(static_cast<uint32_t>((a.n + 15) / 16));
+        if (exact) few_rows_kernel<X, true, 1><<<grid, threads, 0, stream>>>(a);
+        else few_rows_kernel<X, false, 1><<<grid, threads, 0, stream>>>(a);
+    }
+}
+
 // Tiles by how many of them there are: 256 x 256 where they occupy most compute units,
 // 128 x 128 where those do, else 64 x 64.
 template <int BM, int BN, int WM, int WN, int D>
@@ -492,10 +680,40 @@ extern "C" int muon_train_fp8_matmul(const muon_train_fp8_matmul_args *args, hip
     }
     const int cus = compute_units();
     if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "fp8: no device");
+    if (g.k > 0 && g.m <= kFewRows && g.a.block_rows == 1 && g.b.block_rows == kBlock) {
+        const DecodeArgs d{g.n, g.a.ld, int(g.m), int(g.k), int(g.k / kBlock), g.a.values, g.a.scales,
+                           g.a.scale_col, g.b, g.c, g.ldc, g.c_dtype};
+        launch_few_rows<Held>(d, cus, stream);
+        return launched("fp8_matmul");
+    }
     auto tiles = [&](int64_t t) { return ((g.m + t - 1) / t) * ((g.n + t - 1) / t); };
     if (tiles(64) > INT32_MAX) return invalid("fp8: matrix too large");
     if (2 * tiles(256) >= cus) launch_tiles<256, 256, 128, 64, 2>(g, stream);
     else if (2 * tiles(128) >= cus) launch_tiles<128, 128, 64, 64, 2>(g, stream);
     else launch_tiles<64, 64, 32, 32, 4>(g, stream);
     return launched("fp8_matmul");
+}
+
+extern "C" int muon_train_fp8_decode(const muon_train_fp8_decode_args *args, hipStream_t stream) {
+    if (!args) return invalid("fp8: args is null");
+    const muon_train_fp8_decode_args &g = *args;
+    if (g.m < 0 || g.m > kFewRows) return invalid("fp8: m must be 0 to 16");
+    if (g.n < 0 || g.n > kMaxExtent || g.cols < 1 || g.cols > kMaxExtent)
+        return invalid("fp8: n must be 0 to 2^30 and cols 1 to 2^30");
+    if (!dtype_ok(g.x_dtype) || !dtype_ok(g.c_dtype)) return invalid("fp8: dtype must be float32 or bfloat16");
+    if (g.m == 0 || g.n == 0) return MUON_POLAR_OK;
+    if (!g.x || !g.c) return invalid("fp8: null pointer");
+    if (g.ld_x < g.cols) return invalid("fp8: rows of x must not overlap");
+    if (g.ldc < g.n) return invalid("fp8: rows of c must not overlap");
+    const int64_t blocks = (g.cols + kBlock - 1) / kBlock;
+    const int st = check(g.w, blocks * kBlock);
+    if (st != MUON_POLAR_OK) return st;
+    if (g.w.block_rows != kBlock) return invalid("fp8: block_rows of w must be 128");
+    const int cus = compute_units();
+    if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "fp8: no device");
+    const DecodeArgs d{g.n, g.ld_x, int(g.m), int(g.cols), int(blocks), g.x, nullptr, 0,
+                       g.w, g.c, g.ldc, g.c_dtype};
+    if (g.x_dtype == MUON_TRAIN_BF16) launch_few_rows<Bf16>(d, cus, stream);
+    else launch_few_rows<F32>(d, cus, stream);
+    return launched("fp8_decode");
 }

@@ -333,3 +333,29 @@ def test_matmul_entry_checks_before_any_launch(change, operand, message):
     for empty in ("m", "n"):
         args = MatmulArgs(**{**base, empty: 0}, a=Operand(**good), b=Operand(**good))
         assert lib.muon_train_fp8_matmul(ctypes.byref(args), None) == capi.OK
+
+
+class DecodeArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("m", "n", "cols", "ld_x")] + [
+        ("x", ctypes.c_void_p), ("x_dtype", ctypes.c_int), ("w", Operand), ("c", ctypes.c_void_p),
+        ("ldc", ctypes.c_int64), ("c_dtype", ctypes.c_int)]
+
+
+@pytest.mark.parametrize("change,operand,message", [
+    (dict(m=17), {}, "m must"), (dict(m=-1), {}, "m must"), (dict(cols=0), {}, "cols"),
+    (dict(x_dtype=2), {}, "dtype"), (dict(x=None), {}, "null"), (dict(c=None), {}, "null"),
+    (dict(ld_x=199), {}, "overlap"), (dict(ldc=7), {}, "overlap"),
+    ({}, dict(ld=128), "overlap"), ({}, dict(values=4104), "aligned"),
+    ({}, dict(block_rows=1), "block_rows"),
+])
+def test_decode_entry_checks_before_any_launch(change, operand, message):
+    lib = capi.load()
+    good = dict(values=4096, scales=4096, ld=256, scale_row=1, scale_col=4, block_rows=128)
+    base = dict(m=4, n=8, cols=200, ld_x=200, x=4096, c=4096, ldc=8)
+    args = DecodeArgs(**{**base, **change}, w=Operand(**{**good, **operand}))
+    assert lib.muon_train_fp8_decode(ctypes.byref(args), None) == capi.ERR_INVALID_ARGUMENT
+    assert message in capi.last_error()
+    assert lib.muon_train_fp8_decode(None, None) == capi.ERR_INVALID_ARGUMENT
+    for empty in ("m", "n"):
+        args = DecodeArgs(**{**base, empty: 0}, w=Operand(**good))
+        assert lib.muon_train_fp8_decode(ctypes.byref(args), None) == capi.OK

@@ -265,3 +265,24 @@ def test_another_stream_and_a_graph():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, mf.train.fp8_linear(held_x, w))
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 15, 16, 17])
+@pytest.mark.parametrize("n,k", [(1, 1), (5, 100), (16, 128), (100, 1024), (129, 1100), (8210, 700),
+                                 (300, 14336)])
+@pytest.mark.parametrize("dtype", [F32, B16], ids=str)
+def test_few_tokens(m, n, k, dtype):
+    """Up to 16 tokens are quantised in the product's own kernel: the bits of the two calls,
+    and each token's result is its own whatever the others are."""
+    gen = torch.Generator().manual_seed(m + n + k)
+    x, w = spread(gen, m, k, dtype), randn(gen, n, k)
+    q = mf.train.quantize_fp8(w.cuda(), 128)
+    got = mf.train.fp8_linear(x.cuda(), q)
+    check(got, value(x, 1) @ value(w, 128).t(), F32_SUM)
+    two = mf.train.fp8_matmul(mf.train.quantize_fp8(x.cuda()), q, dtype)
+    assert torch.equal(got, two)
+    x[1:] *= math.inf
+    assert torch.equal(mf.train.fp8_linear(x.cuda(), q)[0], got[0])
+    wide = torch.full((m, k + 3), 7.0, dtype=dtype, device="cuda")
+    wide[:, 3:] = x.cuda()
+    assert torch.equal(mf.train.fp8_linear(wide[:, 3:], q)[0], got[0])
