@@ -3,6 +3,7 @@
 #include "train_common.hpp"
 
 #include <type_traits>
+#include <utility>
 
 namespace muon_train {
 
@@ -14,6 +15,16 @@ using i32x8 = int32_t __attribute__((ext_vector_type(8)));
 using muon_polar::i32x4;
 
 constexpr int kBlock = 128;
+
+// f(0), f(1), ..., f(N - 1) with the index a compile-time constant.
+template <class F, int... I>
+__device__ __forceinline__ void static_for_seq(F &&f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void static_for(F &&f) {
+    static_for_seq(f, std::make_integer_sequence<int, N>{});
+}
 
 // ------------------------------------------------------------------------- quantising
 // One workgroup takes a tile of 128 x 128 elements: thread t the rows 8·(t / 16) .. + 7 and
@@ -288,6 +299,7 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
     MatmulArgs g, int tiles_m, int tiles_n) {
     using Geo = Geometry<BM, BN, WM, WN, D>;
     constexpr int SM = WM / 16, SN = WN / 16, kLoads = Geo::kLoads;
+    constexpr bool kPipelined = D == 2 && !kExact;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[D * Geo::kSlot];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -356,42 +368,138 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
     };
 
     f32x4 acc[SM][SN] = {};
-    if (steps > 0) {
-        for (int s = 0; s < D - 1; ++s)
-#pragma unroll
-            for (int d = 0; d <= kLoads; ++d) issue(d, s, s);
-    }
-    int slot = 0;
-    for (int k = 0; k < steps; ++k) {
-        muon_polar::wait_vm_barrier<(D - 2) * (kLoads + 1)>();
-        const int next = slot == 0 ? D - 1 : slot - 1;  // the slot that step k - 1 left
-        const uint8_t *base = smem + slot * Geo::kSlot;
-        const float *scale_m = reinterpret_cast<const float *>(base + Geo::kPanels) + wm + r;
-        const float *scale_n = reinterpret_cast<const float *>(base + Geo::kPanels) + BM + wn;
-        Frag<kExact> fb[SN];
-        f32x4 sn[SN];
-#pragma unroll
-        for (int j = 0; j < SN; ++j) {
+    if constexpr (kPipelined) {
+        // Software pipeline over the step's MFMAs q = 0 .. SM·SN - 1 (block i = q / SN of a's
+        // rows, j = q % SN of b's): each is followed by the multiply-adds of the one kLag
+        // before it, and the fragments of a's block i + 2 are read while block i is
+        // multiplied.  The barrier of the next step comes before the last block, when this
+        // wave has all of the step's fragments in registers: the next step's first fragments
+        // are read, and the slot refilled, beside that block's MFMAs.  (MFMA, wait,
+        // multiply-add in turn, the two waves of a SIMD covering for each other: 530 us at
+        // 8192 x 14336 x 4096.)
+        constexpr int kQ = SM * SN, kLag = 2, kLast = (SM - 1) * SN;
+        static_assert(D == 2 && !kExact && SM % 4 == 0 && kQ % 4 == 0, "schedule");
+        constexpr int kGap = SM >= 8 ? 2 : 1;  // MFMAs from one DMA instruction to the next
+        // DMA instructions issued in the last block, behind the barrier
+        constexpr int kEarly = (SN + kGap - 1) / kGap < kLoads + 1 ? (SN + kGap - 1) / kGap : kLoads + 1;
+        static_assert((kLoads + 1 - kEarly) * kGap <= kLast, "a step's DMA is issued before its barrier");
+        Frag<false> fa[4], fb[SN];
+        f32x4 t[4], sn[kRowB ? SN : 1], sn_last[kRowB ? SN : 1];
+        float f[SM], f_last = 0.0f;
+        static_for<4>([&](auto c) { t[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; });
+        if constexpr (kRowB) static_for<SN>([&](auto c) { sn_last[c] = t[0]; });
+        auto base_of = [&](int s) { return smem + s * Geo::kSlot; };
+        auto read_a = [&](const uint8_t *base, auto ic) {
+            constexpr int i = decltype(ic)::value;
+            fa[i % 4] = fragment(base + (wm + 16 * i) * kBlock);
+        };
+        auto read_b = [&](const uint8_t *base, auto jc) {
+            constexpr int j = decltype(jc)::value;
             fb[j] = fragment(base + (BM + wn + 16 * j) * kBlock);
-            if constexpr (kRowB) sn[j] = *reinterpret_cast<const f32x4 *>(scale_n + 16 * j + 4 * part);
-        }
-        const float sb = kRowB ? 1.0f : scale_n[0];
+        };
+        auto read_scales = [&](const uint8_t *base) {
+            const float *scale_m = reinterpret_cast<const float *>(base + Geo::kPanels) + wm + r;
+            const float *scale_n = reinterpret_cast<const float *>(base + Geo::kPanels) + BM + wn;
+            const float sb = kRowB ? 1.0f : scale_n[0];
+            static_for<SM>([&](auto ic) { f[ic] = scale_m[16 * ic] * sb; });
+            if constexpr (kRowB)
+                static_for<SN>([&](auto jc) {
+                    sn[jc] = *reinterpret_cast<const f32x4 *>(scale_n + 16 * jc + 4 * part);
+                });
+        };
+        auto add = [&](auto qc, float factor, const f32x4 &factor_n) {
+            constexpr int q = decltype(qc)::value, i = q / SN, j = q % SN;
 #pragma unroll
-        for (int i = 0; i < SM; ++i) {
-            const Frag<kExact> fa = fragment(base + (wm + 16 * i) * kBlock);
-            const float sm = scale_m[16 * i] * sb;
+            for (int e = 0; e < 4; ++e)
+                acc[i][j][e] = fmaf(t[q % 4][e], kRowB ? factor * factor_n[e] : factor, acc[i][j][e]);
+        };
+        if (steps > 0) {
+            static_for<kLoads + 1>([&](auto d) { issue(d, 0, 0); });
+            static_for<kEarly>([&](auto d) { issue(d, 1, 1); });
+            muon_polar::wait_vm_barrier<kEarly>();
+            const uint8_t *base = base_of(0);
+            read_scales(base);
+            read_a(base, std::integral_constant<int, 0>{});
+            read_a(base, std::integral_constant<int, 1>{});
+            static_for<SN>([&](auto jc) { read_b(base, jc); });
+        }
+        for (int k = 0; k < steps; ++k) {
+            const int slot = k & 1;
+            const uint8_t *base = base_of(slot), *after = base_of(slot ^ 1);
+            static_for<kQ>([&](auto qc) {
+                constexpr int q = decltype(qc)::value, i = q / SN, j = q % SN;
+                if constexpr (q == kLast) {
+                    f_last = f[SM - 1];
+                    if constexpr (kRowB) static_for<SN>([&](auto c) { sn_last[c] = sn[c]; });
+                    muon_polar::wait_vm_barrier<0>();
+                }
+                t[q % 4] = multiply(fb[j], fa[i % 4]);
+                __builtin_amdgcn_sched_barrier(0);
+                constexpr int p = (q + kQ - kLag) % kQ;  // the MFMA kLag before, maybe last step's
+                constexpr bool old = q < kLag;
+                if constexpr (old || q - kLag >= kLast)
+                    add(std::integral_constant<int, p>{}, f_last, sn_last[kRowB ? p % SN : 0]);
+                else
+                    add(std::integral_constant<int, p>{}, f[p / SN], sn[kRowB ? p % SN : 0]);
+                if constexpr (j == 0 && i + 2 < SM) read_a(base, std::integral_constant<int, i + 2>{});
+                if constexpr (q < kLast) {
+                    constexpr int d = kEarly + q / kGap;
+                    if constexpr (q % kGap == 0 && d <= kLoads) issue(d, k + 1, slot ^ 1);
+                } else {
+                    // the multiply-adds of the blocks before the last are done with f by now
+                    if constexpr (q == kLast) read_a(after, std::integral_constant<int, 0>{});
+                    if constexpr (q == kLast + 1) read_a(after, std::integral_constant<int, 1>{});
+                    read_b(after, std::integral_constant<int, j>{});
+                    if constexpr (q == kLast + kLag) read_scales(after);
+                    constexpr int d = (q - kLast) / kGap;
+                    if constexpr ((q - kLast) % kGap == 0 && d < kEarly) issue(d, k + 2, slot);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        }
+        if (steps > 0)
+            static_for<kLag>([&](auto c) {
+                add(std::integral_constant<int, kQ - kLag + decltype(c)::value>{}, f_last,
+                    sn_last[kRowB ? SN - kLag + decltype(c)::value : 0]);
+            });
+    } else {
+        if (steps > 0) {
+            for (int s = 0; s < D - 1; ++s)
+#pragma unroll
+                for (int d = 0; d <= kLoads; ++d) issue(d, s, s);
+        }
+        int slot = 0;
+        for (int k = 0; k < steps; ++k) {
+            muon_polar::wait_vm_barrier<(D - 2) * (kLoads + 1)>();
+            const int next = slot == 0 ? D - 1 : slot - 1;  // the slot that step k - 1 left
+            const uint8_t *base = smem + slot * Geo::kSlot;
+            const float *scale_m = reinterpret_cast<const float *>(base + Geo::kPanels) + wm + r;
+            const float *scale_n = reinterpret_cast<const float *>(base + Geo::kPanels) + BM + wn;
+            Frag<kExact> fb[SN];
+            f32x4 sn[SN];
 #pragma unroll
             for (int j = 0; j < SN; ++j) {
-                const f32x4 t = multiply(fb[j], fa);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    acc[i][j][e] = fmaf(t[e], kRowB ? sm * sn[j][e] : sm, acc[i][j][e]);
+                fb[j] = fragment(base + (BM + wn + 16 * j) * kBlock);
+                if constexpr (kRowB) sn[j] = *reinterpret_cast<const f32x4 *>(scale_n + 16 * j + 4 * part);
             }
+            const float sb = kRowB ? 1.0f : scale_n[0];
 #pragma unroll
-            for (int d = i * (kLoads + 1) / SM; d < (i + 1) * (kLoads + 1) / SM; ++d)
-                issue(d, k + D - 1, next);
+            for (int i = 0; i < SM; ++i) {
+                const Frag<kExact> fa = fragment(base + (wm + 16 * i) * kBlock);
+                const float sm = scale_m[16 * i] * sb;
+#pragma unroll
+                for (int j = 0; j < SN; ++j) {
+                    const f32x4 t = multiply(fb[j], fa);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        acc[i][j][e] = fmaf(t[e], kRowB ? sm * sn[j][e] : sm, acc[i][j][e]);
+                }
+#pragma unroll
+                for (int d = i * (kLoads + 1) / SM; d < (i + 1) * (kLoads + 1) / SM; ++d)
+                    issue(d, k + D - 1, next);
+            }
+            slot = slot + 1 == D ? 0 : slot + 1;
         }
-        slot = slot + 1 == D ? 0 : slot + 1;
     }
     muon_polar::wait_vm<0>();  // no DMA into LDS outlives the workgroup
 
