@@ -274,8 +274,10 @@ __device__ __forceinline__ void tile_of(int w, int tiles_m, int tiles_n, int &tm
 // A tile of BM x BN outputs, waves of WM x WN.  K runs in steps of one block of 128: the
 // step's panels (rows of 128 bytes) and scales come to LDS by DMA, D steps in a ring, so
 // that step k + D - 1 streams in while step k is multiplied.  A row's 16-byte chunk c lies
-// at place c ^ ((row >> 1) & 7): the 16 rows of a fragment read meet 16 different places of
-// the 256-byte bank window.
+// at place c ^ ((row >> 1) & 7), and a lane of k-part p reads chunks p and p + 4 (both
+// operands in the same order, which is all that the MFMA asks for): the 16 lanes that LDS
+// serves at once then meet 16 different places of the 256-byte bank window.  (Chunks 2p and
+// 2p + 1 met half as many.)
 //
 // The operand b, whose rows are output columns, is the MFMA's A side: a lane then holds
 // four consecutive columns of one output row, and a's scale is one number a lane.  Each
@@ -358,10 +360,10 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
 
     const int wm = (wave % (BM / WM)) * WM, wn = (wave / (BM / WM)) * WN;
     const int r = lane & 15, part = lane >> 4;
-    const int lane_at = r * kBlock + (((2 * part) ^ ((r >> 1) & 7)) << 4);
+    const int lane_at = r * kBlock + ((part ^ ((r >> 1) & 7)) << 4);
     auto fragment = [&](const uint8_t *panel) {
         const i32x4 lo = *reinterpret_cast<const i32x4 *>(panel + lane_at);
-        const i32x4 hi = *reinterpret_cast<const i32x4 *>(panel + (lane_at ^ 16));
+        const i32x4 hi = *reinterpret_cast<const i32x4 *>(panel + (lane_at ^ 64));
         Frag<kExact> f;
         f.set(i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
         return f;
