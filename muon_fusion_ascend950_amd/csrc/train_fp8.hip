@@ -380,14 +380,14 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
         // multiply-add in turn, the two waves of a SIMD covering for each other: 530 us at
         // 8192 x 14336 x 4096.)
         constexpr int kQ = SM * SN, kLag = 2, kLast = (SM - 1) * SN;
-        static_assert(D == 2 && !kExact && SM % 4 == 0 && kQ % 4 == 0, "schedule");
-        constexpr int kGap = SM >= 8 ? 2 : 1;  // MFMAs from one DMA instruction to the next
+        static_assert(D == 2 && !kExact && SM % 4 == 0 && kQ % 4 == 0 && kLag < SN, "schedule");
+        constexpr int kGap = 1;  // MFMAs from one DMA instruction to the next
         // DMA instructions issued in the last block, behind the barrier
         constexpr int kEarly = (SN + kGap - 1) / kGap < kLoads + 1 ? (SN + kGap - 1) / kGap : kLoads + 1;
         static_assert((kLoads + 1 - kEarly) * kGap <= kLast, "a step's DMA is issued before its barrier");
         Frag<false> fa[4], fb[SN];
         f32x4 t[4], sn[kRowB ? SN : 1], sn_last[kRowB ? SN : 1];
-        float f[SM], f_last = 0.0f;
+        float f[SM], sb = 0.0f, factor = 0.0f;  // a's scales, b's, their product for the block at hand
         static_for<4>([&](auto c) { t[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; });
         if constexpr (kRowB) static_for<SN>([&](auto c) { sn_last[c] = t[0]; });
         auto base_of = [&](int s) { return smem + s * Geo::kSlot; };
@@ -402,15 +402,16 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
         auto read_scales = [&](const uint8_t *base) {
             const float *scale_m = reinterpret_cast<const float *>(base + Geo::kPanels) + wm + r;
             const float *scale_n = reinterpret_cast<const float *>(base + Geo::kPanels) + BM + wn;
-            const float sb = kRowB ? 1.0f : scale_n[0];
-            static_for<SM>([&](auto ic) { f[ic] = scale_m[16 * ic] * sb; });
+            static_for<SM>([&](auto ic) { f[ic] = scale_m[16 * ic]; });
+            if constexpr (!kRowB) sb = scale_n[0];
             if constexpr (kRowB)
                 static_for<SN>([&](auto jc) {
                     sn[jc] = *reinterpret_cast<const f32x4 *>(scale_n + 16 * jc + 4 * part);
                 });
         };
-        auto add = [&](auto qc, float factor, const f32x4 &factor_n) {
+        auto add = [&](auto qc, const f32x4 &factor_n) {
             constexpr int q = decltype(qc)::value, i = q / SN, j = q % SN;
+            if constexpr (j == 0) factor = kRowB ? f[i] : f[i] * sb;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 acc[i][j][e] = fmaf(t[q % 4][e], kRowB ? factor * factor_n[e] : factor, acc[i][j][e]);
@@ -431,7 +432,6 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
             static_for<kQ>([&](auto qc) {
                 constexpr int q = decltype(qc)::value, i = q / SN, j = q % SN;
                 if constexpr (q == kLast) {
-                    f_last = f[SM - 1];
                     if constexpr (kRowB) static_for<SN>([&](auto c) { sn_last[c] = sn[c]; });
                     muon_polar::wait_vm_barrier<0>();
                 }
@@ -440,18 +440,18 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
                 constexpr int p = (q + kQ - kLag) % kQ;  // the MFMA kLag before, maybe last step's
                 constexpr bool old = q < kLag;
                 if constexpr (old || q - kLag >= kLast)
-                    add(std::integral_constant<int, p>{}, f_last, sn_last[kRowB ? p % SN : 0]);
+                    add(std::integral_constant<int, p>{}, sn_last[kRowB ? p % SN : 0]);
                 else
-                    add(std::integral_constant<int, p>{}, f[p / SN], sn[kRowB ? p % SN : 0]);
+                    add(std::integral_constant<int, p>{}, sn[kRowB ? p % SN : 0]);
                 if constexpr (j == 0 && i + 2 < SM) read_a(base, std::integral_constant<int, i + 2>{});
                 if constexpr (q < kLast) {
                     constexpr int d = kEarly + q / kGap;
                     if constexpr (q % kGap == 0 && d <= kLoads) issue(d, k + 1, slot ^ 1);
                 } else {
-                    // the multiply-adds of the blocks before the last are done with f by now
                     if constexpr (q == kLast) read_a(after, std::integral_constant<int, 0>{});
                     if constexpr (q == kLast + 1) read_a(after, std::integral_constant<int, 1>{});
                     read_b(after, std::integral_constant<int, j>{});
+                    // the last block's factor is formed: the scales give way to the next step's
                     if constexpr (q == kLast + kLag) read_scales(after);
                     constexpr int d = (q - kLast) / kGap;
                     if constexpr ((q - kLast) % kGap == 0 && d < kEarly) issue(d, k + 2, slot);
@@ -461,7 +461,7 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
         }
         if (steps > 0)
             static_for<kLag>([&](auto c) {
-                add(std::integral_constant<int, kQ - kLag + decltype(c)::value>{}, f_last,
+                add(std::integral_constant<int, kQ - kLag + decltype(c)::value>{},
                     sn_last[kRowB ? SN - kLag + decltype(c)::value : 0]);
             });
     } else {
