@@ -223,8 +223,18 @@ __device__ __forceinline__ f32x4 multiply(const Frag<true> &a, const Frag<true> 
     return t;
 }
 
-// 4 B per lane from rsrc + voffset into LDS at lds_base (wave-uniform) + 4·lane (see
-// dma_16B for the wait state).
+// 16 B per lane from rsrc + voffset + soffset into LDS at lds_base (wave-uniform) + 16·lane
+// (see dma_16B for the wait state).  The step goes into soffset, a scalar: added to the
+// lanes' offsets it took two vector instructions a DMA instruction from the multiply-adds.
+__device__ __forceinline__ void dma_16B_step(muon_polar::i32x4 rsrc, uint32_t lds_base,
+                                             uint32_t voffset, uint32_t soffset) {
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+                 :
+                 : "v"(voffset), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(soffset)),
+                   "{m0}"(__builtin_amdgcn_readfirstlane(lds_base))
+                 : "memory");
+}
+// 4 B per lane from rsrc + voffset into LDS at lds_base (wave-uniform) + 4·lane.
 __device__ __forceinline__ void dma_4B(muon_polar::i32x4 rsrc, uint32_t lds_base, uint32_t voffset) {
     asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
                  :
@@ -346,13 +356,11 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
     const uint32_t lds0 = muon_polar::lds_addr(smem);
     auto issue = [&](int d, int step, int slot) {
         const uint32_t base = lds0 + slot * Geo::kSlot;
+        const int s = step < steps ? step : steps - 1;  // past the end: the last step once more
         if (d < kLoads) {
             const int row0 = 8 * (wave * kLoads + d);
-            const uint32_t at = step < steps ? off[d] + step * kBlock : muon_polar::kOob;
-            // a row outside the matrix stays outside: kOob + k is past every buffer
-            muon_polar::dma_16B(row0 < BM ? rs_a : rs_b, base + row0 * kBlock, at);
+            dma_16B_step(row0 < BM ? rs_a : rs_b, base + row0 * kBlock, off[d], s * kBlock);
         } else {
-            const int s = step < steps ? step : steps - 1;
             const auto rs = muon_polar::make_buffer_rsrc(sbase + s * sstep, 0x7ffffffcu);
             dma_4B(rs, base + Geo::kPanels + sblock * 256, soff);
         }
