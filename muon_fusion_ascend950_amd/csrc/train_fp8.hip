@@ -15,6 +15,7 @@ using i32x8 = int32_t __attribute__((ext_vector_type(8)));
 using muon_polar::i32x4;
 
 constexpr int kBlock = 128;
+using u32x4_any = uint32_t __attribute__((ext_vector_type(4), aligned(2)));  // at any element's address
 
 // f(0), f(1), ..., f(N - 1) with the index a compile-time constant.
 template <class F, int... I>
@@ -234,11 +235,13 @@ __device__ __forceinline__ void dma_16B_step(muon_polar::i32x4 rsrc, uint32_t ld
                    "{m0}"(__builtin_amdgcn_readfirstlane(lds_base))
                  : "memory");
 }
-// 4 B per lane from rsrc + voffset into LDS at lds_base (wave-uniform) + 4·lane.
-__device__ __forceinline__ void dma_4B(muon_polar::i32x4 rsrc, uint32_t lds_base, uint32_t voffset) {
-    asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
+// The same with 4 B per lane.
+__device__ __forceinline__ void dma_4B_step(muon_polar::i32x4 rsrc, uint32_t lds_base,
+                                            uint32_t voffset, uint32_t soffset) {
+    asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, %2 offen lds"
                  :
-                 : "v"(voffset), "s"(rsrc), "{m0}"(__builtin_amdgcn_readfirstlane(lds_base))
+                 : "v"(voffset), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(soffset)),
+                   "{m0}"(__builtin_amdgcn_readfirstlane(lds_base))
                  : "memory");
 }
 
@@ -264,6 +267,34 @@ __device__ __forceinline__ void store4(void *c, int64_t at, int count, int dtype
             for (int e = 0; e < 3; ++e)
                 if (e < count) p[e] = v[e];
         }
+    }
+}
+
+// Exchanges that turn a wave's results into whole lines of 128 bytes.  A lane (r, p) = (l %
+// 16, l / 16) holds four columns 16·j + 4·p of row r for each j.  Stored as they are, a line
+// is written in four instructions of 32 bytes each, and the stores of 256 tiles that end
+// together took 12 us (33.5 MB; whole lines fill memory at 6.9 TB/s).
+//
+// (a, b) <- parts (a0 b0 a2 b2, a1 b1 a3 b3) of (a0 a1 b0 b1, a2 a3 b2 b3) of (a, b): from
+// columns 16·j and 16·(j + 1) to the low and high four of the eight columns 8·p.
+__device__ __forceinline__ void turn_parts(uint32_t &a, uint32_t &b) {
+    const auto x = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    const auto y = __builtin_amdgcn_permlane16_swap(x[0], x[1], false, false);
+    a = y[0];
+    b = y[1];
+}
+// Rows r and r ^ 8 swap pieces: a lane's pieces a and b, 64 bytes apart in its row, become
+// pieces of rows r % 8 and 8 + r % 8, piece p + 4·(r / 8) of their line.
+__device__ __forceinline__ void turn_rows(u32x4 &a, u32x4 &b, int r) {
+    constexpr int kRowRotate8 = 0x128;
+    const bool high = r >= 8;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t give = high ? a[e] : b[e];
+        const uint32_t got = __builtin_amdgcn_update_dpp(give, give, kRowRotate8, 0xf, 0xf, false);
+        const uint32_t mine = high ? b[e] : a[e];
+        a[e] = high ? got : mine;
+        b[e] = high ? mine : got;
     }
 }
 
@@ -304,6 +335,7 @@ struct Geometry {
     static_assert(kScaleLoads <= kWaves, "one scale load a wave");
     static_assert((D - 1) * (kLoads + 1) <= 63, "vmcnt range");
     static_assert(D * kSlot <= 160 * 1024, "LDS");
+    static constexpr bool kTwoSlots = D == 2;
 };
 
 template <int BM, int BN, int WM, int WN, int D, bool kExact, bool kRowB>
@@ -311,48 +343,49 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
     MatmulArgs g, int tiles_m, int tiles_n) {
     using Geo = Geometry<BM, BN, WM, WN, D>;
     constexpr int SM = WM / 16, SN = WN / 16, kLoads = Geo::kLoads;
-    constexpr bool kPipelined = D == 2 && !kExact;
+    constexpr bool kPipelined = Geo::kTwoSlots && !kExact && !kRowB;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[D * Geo::kSlot];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-    int tm, tn;
-    tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
-    const int64_t m0 = int64_t(tm) * BM, n0 = int64_t(tn) * BN;
-    const int rows_m = g.m - m0 < BM ? int(g.m - m0) : BM;
-    const int rows_n = g.n - n0 < BN ? int(g.n - n0) : BN;
     const int steps = static_cast<int>(g.k / kBlock);
 
-    // DMA: instruction d of this wave moves rows 8·(wave·kLoads + d) .. + 7 of the step's
-    // BM + BN panel rows; rows outside the matrices read as zeros.
-    const auto rs_a = muon_polar::make_buffer_rsrc(static_cast<const uint8_t *>(g.a.values) + m0 * g.a.ld,
-                                                   static_cast<uint32_t>(rows_m * g.a.ld));
-    const auto rs_b = muon_polar::make_buffer_rsrc(static_cast<const uint8_t *>(g.b.values) + n0 * g.b.ld,
-                                                   static_cast<uint32_t>(rows_n * g.b.ld));
-    uint32_t off[kLoads];
-#pragma unroll
-    for (int d = 0; d < kLoads; ++d) {
-        const int row = 8 * (wave * kLoads + d) + (lane >> 3);
-        const int chunk = (lane & 7) ^ ((row >> 1) & 7);
-        const bool is_a = row < BM;
-        const int at = is_a ? row : row - BM;
-        off[d] = at < (is_a ? rows_m : rows_n)
-                     ? static_cast<uint32_t>(at * (is_a ? g.a.ld : g.b.ld) + 16 * chunk)
-                     : muon_polar::kOob;
-    }
-    // scales: 64 rows' worth of the step's BM + BN, one each (rows past the end: the last's)
+    // DMA: instruction d of this wave moves rows 8·(wave·kLoads + d) .. + 7 of a step's
+    // BM + BN panel rows; rows outside the matrices read as zeros.  Behind them the scales:
+    // 64 rows' worth a wave, one each (rows past the end: the last's).
     const int sblock = wave % Geo::kScaleLoads;
     const bool scale_a = sblock * 64 < BM;
     const muon_train_fp8_operand &so = scale_a ? g.a : g.b;
-    const int srow = (scale_a ? sblock * 64 : sblock * 64 - BM) + lane;
-    const int64_t sfirst = scale_a ? m0 : n0;
-    const int slast = (scale_a ? rows_m : rows_n) - 1;
-    const int64_t sat = sfirst + (srow < slast ? srow : slast);
-    const uint32_t soff = static_cast<uint32_t>(
-        4 * ((so.block_rows == 1 ? sat : sat / kBlock) - (so.block_rows == 1 ? sfirst : sfirst / kBlock)) *
-        so.scale_row);
-    const float *sbase = so.scales + (so.block_rows == 1 ? sfirst : sfirst / kBlock) * so.scale_row;
-    const int64_t sstep = so.scale_col;
-
+    i32x4 rs_a, rs_b, rs_scale;
+    uint32_t off[kLoads], soff;
+    const uint32_t sstep = static_cast<uint32_t>(4 * so.scale_col);
+    auto aim = [&](int tile) {  // at a tile's first step
+        int tm, tn;
+        tile_of(tile, tiles_m, tiles_n, tm, tn);
+        const int64_t m0 = int64_t(tm) * BM, n0 = int64_t(tn) * BN;
+        const int rows_m = g.m - m0 < BM ? int(g.m - m0) : BM;
+        const int rows_n = g.n - n0 < BN ? int(g.n - n0) : BN;
+        rs_a = muon_polar::make_buffer_rsrc(static_cast<const uint8_t *>(g.a.values) + m0 * g.a.ld,
+                                            static_cast<uint32_t>(rows_m * g.a.ld));
+        rs_b = muon_polar::make_buffer_rsrc(static_cast<const uint8_t *>(g.b.values) + n0 * g.b.ld,
+                                            static_cast<uint32_t>(rows_n * g.b.ld));
+#pragma unroll
+        for (int d = 0; d < kLoads; ++d) {
+            const int row = 8 * (wave * kLoads + d) + (lane >> 3);
+            const int chunk = (lane & 7) ^ ((row >> 1) & 7);
+            const bool is_a = row < BM;
+            const int at = is_a ? row : row - BM;
+            off[d] = at < (is_a ? rows_m : rows_n)
+                         ? static_cast<uint32_t>(at * (is_a ? g.a.ld : g.b.ld) + 16 * chunk)
+                         : muon_polar::kOob;
+        }
+        const int srow = (scale_a ? sblock * 64 : sblock * 64 - BM) + lane;
+        const int64_t sfirst = scale_a ? m0 : n0;
+        const int slast = (scale_a ? rows_m : rows_n) - 1;
+        const int64_t sat = sfirst + (srow < slast ? srow : slast);
+        const int64_t from = so.block_rows == 1 ? sfirst : sfirst / kBlock;
+        soff = static_cast<uint32_t>(4 * ((so.block_rows == 1 ? sat : sat / kBlock) - from) * so.scale_row);
+        rs_scale = muon_polar::make_buffer_rsrc(so.scales + from * so.scale_row, 0x7ffffffcu);
+    };
     const uint32_t lds0 = muon_polar::lds_addr(smem);
     auto issue = [&](int d, int step, int slot) {
         const uint32_t base = lds0 + slot * Geo::kSlot;
@@ -361,8 +394,7 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
             const int row0 = 8 * (wave * kLoads + d);
             dma_16B_step(row0 < BM ? rs_a : rs_b, base + row0 * kBlock, off[d], s * kBlock);
         } else {
-            const auto rs = muon_polar::make_buffer_rsrc(sbase + s * sstep, 0x7ffffffcu);
-            dma_4B(rs, base + Geo::kPanels + sblock * 256, soff);
+            dma_4B_step(rs_scale, base + Geo::kPanels + sblock * 256, soff, s * sstep);
         }
     };
 
@@ -378,26 +410,83 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
     };
 
     f32x4 acc[SM][SN] = {};
+    auto store = [&](int tile) {
+        int tm, tn;
+        tile_of(tile, tiles_m, tiles_n, tm, tn);
+        const int64_t m0 = int64_t(tm) * BM + wm, n0 = int64_t(tn) * BN + wn;
+        if (SN == 4 && n0 + WN <= g.n) {  // lines of 128 bytes: 64 columns of bf16, 32 of fp32
+            auto put = [&](int i, u32x4 v, int half, int64_t bytes) {
+                const int64_t m = m0 + 16 * i + 8 * half + (r & 7);
+                if (m >= g.m) return;
+                uint8_t *row = static_cast<uint8_t *>(g.c) + (m * g.ldc + n0) * (kExact ? 4 : 2);
+                __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any *>(row + bytes + 16 * part + 64 * (r >> 3)));
+            };
+#pragma unroll
+            for (int i = 0; i < SM; ++i) {
+                if constexpr (kExact) {
+#pragma unroll
+                    for (int j = 0; j < SN; j += 2) {
+                        u32x4 a = __builtin_bit_cast(u32x4, acc[i][j]);
+                        u32x4 b = __builtin_bit_cast(u32x4, acc[i][j + 1]);
+                        turn_rows(a, b, r);
+                        put(i, a, 0, 64 * j);
+                        put(i, b, 1, 64 * j);
+                    }
+                } else {
+                    uint32_t w[4][2];  // bf16 pairs of the four j
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            w[j][h] = f32_to_bf16_bits(acc[i][j % SN][2 * h]) |
+                                      uint32_t(f32_to_bf16_bits(acc[i][j % SN][2 * h + 1])) << 16;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        turn_parts(w[0][h], w[1][h]);
+                        turn_parts(w[2][h], w[3][h]);
+                    }
+                    u32x4 a{w[0][0], w[0][1], w[1][0], w[1][1]}, b{w[2][0], w[2][1], w[3][0], w[3][1]};
+                    turn_rows(a, b, r);
+                    put(i, a, 0, 0);
+                    put(i, b, 1, 0);
+                }
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < SM; ++i) {
+            const int64_t m = m0 + 16 * i + r;
+            if (m >= g.m) continue;
+#pragma unroll
+            for (int j = 0; j < SN; ++j) {
+                const int64_t n = n0 + 16 * j + 4 * part;
+                if (n < g.n) store4(g.c, m * g.ldc + n, g.n - n < 4 ? int(g.n - n) : 4, g.c_dtype, acc[i][j]);
+            }
+        }
+    };
+    if (steps == 0) {
+        for (int tile = blockIdx.x; tile < tiles_m * tiles_n; tile += gridDim.x) store(tile);
+        return;
+    }
     if constexpr (kPipelined) {
         // Software pipeline over the step's MFMAs q = 0 .. SM·SN - 1 (block i = q / SN of a's
         // rows, j = q % SN of b's): each is followed by the multiply-adds of the one kLag
-        // before it, and the fragments of a's block i + 2 are read while block i is
-        // multiplied.  The barrier of the next step comes before the last block, when this
-        // wave has all of the step's fragments in registers: the next step's first fragments
-        // are read, and the slot refilled, beside that block's MFMAs.  (MFMA, wait,
+        // before it, and the fragments of a's block i + 3 are read while block i is
+        // multiplied.  The barrier of the next step comes before the last two blocks, when
+        // this wave has all of the step's fragments in registers: the next step's first
+        // fragments are read, and the slot refilled, beside those blocks' MFMAs.  (MFMA, wait,
         // multiply-add in turn, the two waves of a SIMD covering for each other: 530 us at
         // 8192 x 14336 x 4096.)
-        constexpr int kQ = SM * SN, kLag = 2, kLast = (SM - 1) * SN;
+        //
+        // The workgroup's tiles are one stream of steps: in the last two of a tile the DMA
+        // fetches the first two of the next, and a tile's results are stored beside the next
+        // one's first loads.  (A workgroup a tile: 12 us between one tile's last step and the
+        // next one's first, 84 of 439 us there.)
+        constexpr int kQ = SM * SN, kLag = 2, kBar = (SM - 2) * SN, kLast = (SM - 1) * SN;
         static_assert(D == 2 && !kExact && SM % 4 == 0 && kQ % 4 == 0 && kLag < SN, "schedule");
-        constexpr int kGap = 1;  // MFMAs from one DMA instruction to the next
-        // DMA instructions issued in the last block, behind the barrier
-        constexpr int kEarly = (SN + kGap - 1) / kGap < kLoads + 1 ? (SN + kGap - 1) / kGap : kLoads + 1;
-        static_assert((kLoads + 1 - kEarly) * kGap <= kLast, "a step's DMA is issued before its barrier");
         Frag<false> fa[4], fb[SN];
         f32x4 t[4], sn[kRowB ? SN : 1], sn_last[kRowB ? SN : 1];
         float f[SM], sb = 0.0f, factor = 0.0f;  // a's scales, b's, their product for the block at hand
-        static_for<4>([&](auto c) { t[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; });
-        if constexpr (kRowB) static_for<SN>([&](auto c) { sn_last[c] = t[0]; });
         auto base_of = [&](int s) { return smem + s * Geo::kSlot; };
         auto read_a = [&](const uint8_t *base, auto ic) {
             constexpr int i = decltype(ic)::value;
@@ -424,60 +513,75 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
             for (int e = 0; e < 4; ++e)
                 acc[i][j][e] = fmaf(t[q % 4][e], kRowB ? factor * factor_n[e] : factor, acc[i][j][e]);
         };
-        if (steps > 0) {
-            static_for<kLoads + 1>([&](auto d) { issue(d, 0, 0); });
-            static_for<kEarly>([&](auto d) { issue(d, 1, 1); });
-            muon_polar::wait_vm_barrier<kEarly>();
-            const uint8_t *base = base_of(0);
-            read_scales(base);
-            read_a(base, std::integral_constant<int, 0>{});
-            read_a(base, std::integral_constant<int, 1>{});
-            static_for<SN>([&](auto jc) { read_b(base, jc); });
-        }
-        for (int k = 0; k < steps; ++k) {
-            const int slot = k & 1;
-            const uint8_t *base = base_of(slot), *after = base_of(slot ^ 1);
-            static_for<kQ>([&](auto qc) {
-                constexpr int q = decltype(qc)::value, i = q / SN, j = q % SN;
-                if constexpr (q == kLast) {
-                    if constexpr (kRowB) static_for<SN>([&](auto c) { sn_last[c] = sn[c]; });
-                    muon_polar::wait_vm_barrier<0>();
+        auto clear = [&] {  // nothing summed, nothing left to add
+            factor = 0.0f;
+            static_for<4>([&](auto c) { t[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; });
+            if constexpr (kRowB) static_for<SN>([&](auto c) { sn_last[c] = t[0]; });
+#pragma unroll
+            for (int i = 0; i < SM; ++i)
+#pragma unroll
+                for (int j = 0; j < SN; ++j) acc[i][j] = t[0];
+        };
+        const int total = tiles_m * tiles_n;
+        aim(blockIdx.x);
+        static_for<kLoads + 1>([&](auto d) { issue(d, 0, 0); });
+        static_for<kLoads + 1>([&](auto d) { issue(d, 1, 1); });
+        muon_polar::wait_vm_barrier<kLoads + 1>();
+        read_scales(base_of(0));
+        static_for<3>([&](auto ic) { read_a(base_of(0), ic); });
+        static_for<SN>([&](auto jc) { read_b(base_of(0), jc); });
+        clear();
+        int slot = 0;
+        for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
+            // the steps whose slots take the tile's own steps, then those whose slots take the
+            // next tile's (with none left, this one's once more)
+            for (int phase = 0; phase < 2; ++phase) {
+                if (phase == 1 && tile + static_cast<int>(gridDim.x) < total) aim(tile + gridDim.x);
+                const int from = phase == 0 ? 2 : 0, to = phase == 0 ? steps : 2;
+                for (int ahead = from; ahead < to; ++ahead, slot ^= 1) {
+                    const uint8_t *base = base_of(slot), *after = base_of(slot ^ 1);
+                    static_for<kQ>([&](auto qc) {
+                        constexpr int q = decltype(qc)::value, i = q / SN, j = q % SN;
+                        if constexpr (q == kBar) muon_polar::wait_vm_barrier<0>();
+                        if constexpr (q == kLast && kRowB) static_for<SN>([&](auto c) { sn_last[c] = sn[c]; });
+                        t[q % 4] = multiply(fb[j], fa[i % 4]);
+                        __builtin_amdgcn_sched_barrier(0);
+                        constexpr int p = (q + kQ - kLag) % kQ;  // kLag before, maybe last step's
+                        if constexpr (q < kLag || q - kLag >= kLast)
+                            add(std::integral_constant<int, p>{}, sn_last[kRowB ? p % SN : 0]);
+                        else
+                            add(std::integral_constant<int, p>{}, sn[kRowB ? p % SN : 0]);
+                        if constexpr (j == 0 && i + 3 < SM)
+                            read_a(base, std::integral_constant<int, i + 3>{});
+                        if constexpr (q >= kBar) {
+                            constexpr int n = q - kBar;
+                            if constexpr (n < 2) read_a(after, std::integral_constant<int, n>{});
+                            if constexpr (q == kLast) read_a(after, std::integral_constant<int, 2>{});
+                            if constexpr (q >= kLast) read_b(after, std::integral_constant<int, j>{});
+                            // the last block's factor is formed: the scales give way
+                            if constexpr (q == kLast + kLag) read_scales(after);
+                            // kLoads + 1 DMA instructions over the 2·SN MFMAs
+                            static_for<kLoads + 1>([&](auto dc) {
+                                constexpr int d = decltype(dc)::value;
+                                if constexpr (d * 2 * SN / (kLoads + 1) == n) issue(d, ahead, slot);
+                            });
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    });
                 }
-                t[q % 4] = multiply(fb[j], fa[i % 4]);
-                __builtin_amdgcn_sched_barrier(0);
-                constexpr int p = (q + kQ - kLag) % kQ;  // the MFMA kLag before, maybe last step's
-                constexpr bool old = q < kLag;
-                if constexpr (old || q - kLag >= kLast)
-                    add(std::integral_constant<int, p>{}, sn_last[kRowB ? p % SN : 0]);
-                else
-                    add(std::integral_constant<int, p>{}, sn[kRowB ? p % SN : 0]);
-                if constexpr (j == 0 && i + 2 < SM) read_a(base, std::integral_constant<int, i + 2>{});
-                if constexpr (q < kLast) {
-                    constexpr int d = kEarly + q / kGap;
-                    if constexpr (q % kGap == 0 && d <= kLoads) issue(d, k + 1, slot ^ 1);
-                } else {
-                    if constexpr (q == kLast) read_a(after, std::integral_constant<int, 0>{});
-                    if constexpr (q == kLast + 1) read_a(after, std::integral_constant<int, 1>{});
-                    read_b(after, std::integral_constant<int, j>{});
-                    // the last block's factor is formed: the scales give way to the next step's
-                    if constexpr (q == kLast + kLag) read_scales(after);
-                    constexpr int d = (q - kLast) / kGap;
-                    if constexpr ((q - kLast) % kGap == 0 && d < kEarly) issue(d, k + 2, slot);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            });
-        }
-        if (steps > 0)
+            }
             static_for<kLag>([&](auto c) {
                 add(std::integral_constant<int, kQ - kLag + decltype(c)::value>{},
                     sn_last[kRowB ? SN - kLag + decltype(c)::value : 0]);
             });
-    } else {
-        if (steps > 0) {
-            for (int s = 0; s < D - 1; ++s)
-#pragma unroll
-                for (int d = 0; d <= kLoads; ++d) issue(d, s, s);
+            store(tile);
+            clear();
         }
+    } else {
+        aim(blockIdx.x);
+        for (int s = 0; s < D - 1; ++s)
+#pragma unroll
+            for (int d = 0; d <= kLoads; ++d) issue(d, s, s);
         int slot = 0;
         for (int k = 0; k < steps; ++k) {
             muon_polar::wait_vm_barrier<(D - 2) * (kLoads + 1)>();
@@ -510,19 +614,9 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
             }
             slot = slot + 1 == D ? 0 : slot + 1;
         }
+        store(blockIdx.x);
     }
     muon_polar::wait_vm<0>();  // no DMA into LDS outlives the workgroup
-
-#pragma unroll
-    for (int i = 0; i < SM; ++i) {
-        const int64_t m = m0 + wm + 16 * i + r;
-        if (m >= g.m) continue;
-#pragma unroll
-        for (int j = 0; j < SN; ++j) {
-            const int64_t n = n0 + wn + 16 * j + 4 * part;
-            if (n < g.n) store4(g.c, m * g.ldc + n, g.n - n < 4 ? int(g.n - n) : 4, g.c_dtype, acc[i][j]);
-        }
-    }
 }
 
 // ------------------------------------------------------------------ few rows (decoding)
@@ -714,11 +808,14 @@ void launch_few_rows(const DecodeArgs &a, int cus, hipStream_t stream) {
 // Tiles by how many of them there are: 256 x 256 where they occupy most compute units,
 // 128 x 128 where those do, else 64 x 64.
 template <int BM, int BN, int WM, int WN, int D>
-void launch_tiles(const MatmulArgs &g, hipStream_t stream) {
+void launch_tiles(const MatmulArgs &g, int cus, hipStream_t stream) {
     using Geo = Geometry<BM, BN, WM, WN, D>;
     const int tm = static_cast<int>((g.m + BM - 1) / BM), tn = static_cast<int>((g.n + BN - 1) / BN);
-    const dim3 grid(static_cast<uint32_t>(tm) * static_cast<uint32_t>(tn));
     const bool exact = g.c_dtype == MUON_TRAIN_F32, row_b = g.b.block_rows == 1;
+    // pipelined kernels walk their tiles: as many workgroups as stay resident
+    const int64_t tiles = int64_t(tm) * tn;
+    const int64_t resident = int64_t(cus) * (160 * 1024 / (D * Geo::kSlot));
+    const dim3 grid(static_cast<uint32_t>(Geo::kTwoSlots && !exact && !row_b && tiles > resident ? resident : tiles));
     auto go = [&](auto e, auto r) {
         matmul_kernel<BM, BN, WM, WN, D, decltype(e)::value, decltype(r)::value>
             <<<grid, Geo::kThreads, 0, stream>>>(g, tm, tn);
@@ -742,6 +839,10 @@ int check(const muon_train_fp8_operand &o, int64_t k) {
     // the rows of a tile are reached by 31-bit offsets
     if (o.ld > (1 << 22)) return invalid("fp8: rows of values lie too far apart");
     if (o.block_rows != 1 && o.block_rows != kBlock) return invalid("fp8: block_rows must be 1 or 128");
+    // so are the scales of a tile
+    if (o.scale_row < 0 || o.scale_row > (1 << 26) || o.scale_col < 0 ||
+        o.scale_col > (int64_t(1) << 28) / (k / kBlock + 1))
+        return invalid("fp8: scales lie too far apart");
     if (o.block_rows == 1 && o.scale_row != 1)
         return invalid("fp8: scales of single rows must lie next to each other");
     return MUON_POLAR_OK;
@@ -806,9 +907,10 @@ extern "C" int muon_train_fp8_matmul(const muon_train_fp8_matmul_args *args, hip
     }
     auto tiles = [&](int64_t t) { return ((g.m + t - 1) / t) * ((g.n + t - 1) / t); };
     if (tiles(64) > INT32_MAX) return invalid("fp8: matrix too large");
-    if (2 * tiles(256) >= cus) launch_tiles<256, 256, 128, 64, 2>(g, stream);
-    else if (2 * tiles(128) >= cus) launch_tiles<128, 128, 64, 64, 2>(g, stream);
-    else launch_tiles<64, 64, 32, 32, 4>(g, stream);
+    // (a single block of K leaves nothing to pipeline)
+    if (g.k == kBlock || 2 * tiles(128) < cus) launch_tiles<64, 64, 32, 32, 4>(g, cus, stream);
+    else if (2 * tiles(256) >= cus) launch_tiles<256, 256, 128, 64, 2>(g, cus, stream);
+    else launch_tiles<128, 128, 64, 64, 2>(g, cus, stream);
     return launched("fp8_matmul");
 }
 
