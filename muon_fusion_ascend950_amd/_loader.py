@@ -112,19 +112,20 @@ def load_library() -> None:
     def fake_fp8_linear(x, values, scales):
         return x.new_empty((*x.shape[:-1], values.shape[0]))
 
+    def held_bytes(like, rows, cols, block_rows):
+        width = -(-cols // 128) * 128
+        scales = width // 128 * (rows if block_rows == 1 else -(-rows // 128))
+        return like.new_empty((-(-rows * width // 256) * 256 + 4 * scales,), dtype=torch.uint8)
+
     def fake_fp8_linear_forward(x, weight, save):
         n, k = weight.shape
-        none = x.new_empty((0,)), x.new_empty((0,))
-        xt = held(x, k, x.numel() // k, 1) if save & 1 else none
-        wt = held(x, k, n, 128) if save & 2 else none
-        if save & 2:  # a view of the weight's own scales
-            wt = wt[0], wt[1].new_empty(wt[1].shape[::-1]).t()
-        return (x.new_empty((*x.shape[:-1], n)), *xt, *wt)
+        xt = held_bytes(x, k, x.numel() // k, 1) if save & 1 else x.new_empty((0,))
+        wt = held_bytes(x, k, n, 128) if save & 2 else x.new_empty((0,))
+        return x.new_empty((*x.shape[:-1], n)), xt, wt
 
-    def fake_fp8_linear_backward(dy, xt_values, xt_scales, wt_values, wt_scales, weight_dtype,
-                                 wanted):
-        dx = dy.new_empty((*dy.shape[:-1], wt_values.shape[0]) if wanted & 1 else (0,))
-        dw = dy.new_empty((dy.shape[-1], xt_values.shape[0]) if wanted & 2 else (0,),
+    def fake_fp8_linear_backward(dy, saved_x, saved_w, k, weight_dtype, wanted):
+        dx = dy.new_empty((*dy.shape[:-1], k) if wanted & 1 else (0,))
+        dw = dy.new_empty((dy.shape[-1], k) if wanted & 2 else (0,),
                           dtype=weight_dtype if wanted & 2 else dy.dtype)
         return dx, dw
 

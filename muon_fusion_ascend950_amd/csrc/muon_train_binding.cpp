@@ -324,38 +324,22 @@ Held empty_held(const at::Tensor &like, int64_t rows, int64_t cols, int64_t bloc
     return h;
 }
 
-// x as held values, and the transposed x, as wanted.
-void quantize(const at::Tensor &x, int64_t block_rows, Held *plain, Held *turned) {
+Held quantize(const at::Tensor &x, int64_t block_rows) {
     TORCH_CHECK(x.device().is_cuda() && x.dim() == 2, "fp8: a matrix on a ROCm (HIP) device is needed");
     const Rows r = as_rows(x);
-    const int64_t rows = x.size(0), cols = x.size(1);
     muon_train_fp8_quantize_args a{};
-    a.rows = rows;
-    a.cols = cols;
+    a.rows = x.size(0);
+    a.cols = x.size(1);
     a.ld_x = r.ld;
     a.x = r.t.data_ptr();
     a.x_dtype = dtype_of(x, "fp8: a matrix to quantise");
     a.block_rows = static_cast<int>(block_rows);
-    if (plain || (block_rows != 1 && turned)) {
-        Held h = empty_held(x, plain ? rows : 0, cols, block_rows);
-        if (!plain) h.scales = at::empty({blocks(rows), blocks(cols)}, h.scales.options());
-        if (plain) a.values = h.values.data_ptr();
-        a.scales = h.scales.data_ptr<float>();
-        if (plain) *plain = h;
-        if (turned && block_rows != 1) turned->scales = h.scales.t();
-    }
-    if (turned) {
-        if (block_rows == 1) {
-            *turned = empty_held(x, cols, rows, 1);
-            a.scales_t = turned->scales.data_ptr<float>();
-        } else {
-            turned->values = at::empty({cols, blocks(rows) * kBlock},
-                                       x.options().dtype(at::kFloat8_e4m3fn));
-        }
-        a.values_t = turned->values.data_ptr();
-    }
+    Held h = empty_held(x, a.rows, a.cols, block_rows);
+    a.values = h.values.data_ptr();
+    a.scales = h.scales.data_ptr<float>();
     const int st = muon_train_fp8_quantize(&a, stream_of(x));
     TORCH_CHECK(st == MUON_POLAR_OK, "fp8: ", muon_polar_last_error());
+    return h;
 }
 
 muon_train_fp8_operand operand(Held &h, const at::Tensor &like) {
@@ -404,8 +388,7 @@ void matmul(Held a, Held b, at::Tensor &c) {
 
 std::tuple<at::Tensor, at::Tensor> QuantizeFp8(const at::Tensor &x, int64_t block_rows) {
     const c10::OptionalDeviceGuard device_guard(x.device());
-    Held h;
-    quantize(x, block_rows, &h, nullptr);
+    Held h = quantize(x, block_rows);
     return {h.values, h.scales};
 }
 
@@ -417,9 +400,69 @@ at::Tensor Fp8Matmul(const at::Tensor &a, const at::Tensor &a_scales, const at::
     return c;
 }
 
-at::Tensor as_matrix(const at::Tensor &x) {
-    return x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+// What a linear layer holds for itself, values and scales in one buffer: x (or a gradient)
+// in rows, or the weight in 128 x 128 blocks, as they are or transposed.
+struct Layout {
+    int64_t rows, cols; // of the held matrix
+    int64_t block_rows;
+    bool turned; // a transposed weight: its scales lie in the weight's own order
+    int64_t width() const { return blocks(cols) * kBlock; }
+    int64_t scales_at() const { return (rows * width() + 255) / 256 * 256; }
+    int64_t bytes() const {
+        return scales_at() + 4 * blocks(cols) * (block_rows == 1 ? rows : blocks(rows));
+    }
+    at::Tensor empty(const at::Tensor &like) const {
+        return at::empty({bytes()}, like.options().dtype(at::kByte));
+    }
+    uint8_t *values(const at::Tensor &t) const { return t.data_ptr<uint8_t>(); }
+    float *scales(const at::Tensor &t) const {
+        return reinterpret_cast<float *>(t.data_ptr<uint8_t>() + scales_at());
+    }
+    muon_train_fp8_operand operand(const at::Tensor &t) const {
+        muon_train_fp8_operand o{};
+        o.values = values(t);
+        o.scales = scales(t);
+        o.ld = width();
+        o.block_rows = static_cast<int>(block_rows);
+        o.scale_row = block_rows == 1 || turned ? 1 : blocks(cols);
+        o.scale_col = block_rows == 1 ? rows : turned ? blocks(rows) : 1;
+        return o;
+    }
+};
+
+// x [.., cols] as rows, held and / or transposed and held (buffers may be undefined).
+void hold_rows(const at::Tensor &x, const at::Tensor &plain, const at::Tensor &turned) {
+    const Rows r = as_rows(x);
+    const int64_t cols = x.size(-1);
+    const Layout p{r.rows, cols, 1, false}, t{cols, r.rows, 1, false};
+    muon_train_fp8_quantize_args a{};
+    a.rows = r.rows;
+    a.cols = cols;
+    a.ld_x = r.ld;
+    a.x = r.t.data_ptr();
+    a.x_dtype = dtype_of(x, "fp8: a matrix to quantise");
+    a.block_rows = 1;
+    if (plain.defined()) a.values = p.values(plain), a.scales = p.scales(plain);
+    if (turned.defined()) a.values_t = t.values(turned), a.scales_t = t.scales(turned);
+    const int st = muon_train_fp8_quantize(&a, stream_of(x));
+    TORCH_CHECK(st == MUON_POLAR_OK, "fp8: ", muon_polar_last_error());
 }
+
+void multiply(const muon_train_fp8_operand &a, int64_t m, const muon_train_fp8_operand &b, int64_t n,
+              int64_t k, const at::Tensor &c) {
+    muon_train_fp8_matmul_args g{};
+    g.a = a;
+    g.b = b;
+    g.m = m;
+    g.n = g.ldc = n;
+    g.k = k;
+    g.c = c.data_ptr();
+    g.c_dtype = dtype_of(c, "fp8: the result");
+    const int st = muon_train_fp8_matmul(&g, stream_of(c));
+    TORCH_CHECK(st == MUON_POLAR_OK, "fp8: ", muon_polar_last_error());
+}
+
+int64_t rows_of(const at::Tensor &x) { return x.size(-1) > 0 ? x.numel() / x.size(-1) : 0; }
 at::Tensor result_like(const at::Tensor &x, int64_t n) {
     auto sizes = x.sizes().vec();
     sizes.back() = n;
@@ -429,70 +472,96 @@ at::Tensor result_like(const at::Tensor &x, int64_t n) {
 // y = x · wᵀ on a held weight.
 at::Tensor Fp8Linear(const at::Tensor &x, const at::Tensor &values, const at::Tensor &scales) {
     const c10::OptionalDeviceGuard device_guard(x.device());
+    const int64_t rows = rows_of(x), cols = x.size(-1);
     at::Tensor y = result_like(x, values.size(0));
-    const int64_t rows = x.size(-1) > 0 ? x.numel() / x.size(-1) : 0;
-    if (rows <= 16) {  // quantised in the product's own kernel
-        Held w{values, scales};
+    Held held{values, scales};
+    const muon_train_fp8_operand w = operand(held, x);
+    TORCH_CHECK(blocks(cols) * kBlock == values.size(1), "fp8: operands of different width");
+    if (rows <= 16 && w.block_rows == kBlock) {  // quantised in the product's own kernel
         muon_train_fp8_decode_args a{};
-        a.w = operand(w, x);
-        if (a.w.block_rows == kBlock) {
-            TORCH_CHECK(blocks(x.size(-1)) * kBlock == values.size(1), "fp8: operands of different width");
-            const Rows r = as_rows(x);
-            a.m = rows;
-            a.n = a.ldc = values.size(0);
-            a.cols = x.size(-1);
-            a.ld_x = r.ld;
-            a.x = r.t.data_ptr();
-            a.x_dtype = a.c_dtype = dtype_of(x, "fp8: a matrix to quantise");
-            a.c = y.data_ptr();
-            const int st = muon_train_fp8_decode(&a, stream_of(x));
-            TORCH_CHECK(st == MUON_POLAR_OK, "fp8: ", muon_polar_last_error());
-            return y;
-        }
+        const Rows r = as_rows(x);
+        a.w = w;
+        a.m = rows;
+        a.n = a.ldc = values.size(0);
+        a.cols = cols;
+        a.ld_x = r.ld;
+        a.x = r.t.data_ptr();
+        a.x_dtype = a.c_dtype = dtype_of(x, "fp8: a matrix to quantise");
+        a.c = y.data_ptr();
+        const int st = muon_train_fp8_decode(&a, stream_of(x));
+        TORCH_CHECK(st == MUON_POLAR_OK, "fp8: ", muon_polar_last_error());
+        return y;
     }
-    Held h;
-    quantize(as_matrix(x), 1, &h, nullptr);
-    at::Tensor y2 = y.view({h.values.size(0), values.size(0)});
-    matmul(h, {values, scales}, y2);
+    const Layout q{rows, cols, 1, false};
+    const at::Tensor xq = q.empty(x);
+    hold_rows(x, xq, {});
+    multiply(q.operand(xq), rows, w, values.size(0), q.width(), y);
     return y;
 }
 
 // y = x · weightᵀ, and what the backward pass needs: the transposed x along the tokens
 // (save & 1, for the weight's gradient) and the transposed weight (save & 2, for x's).
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> Fp8LinearForward(
-    const at::Tensor &x, const at::Tensor &weight, int64_t save) {
+std::tuple<at::Tensor, at::Tensor, at::Tensor> Fp8LinearForward(const at::Tensor &x,
+                                                                const at::Tensor &weight,
+                                                                int64_t save) {
     const c10::OptionalDeviceGuard device_guard(x.device());
-    Held xq, xt, wq, wt;
-    quantize(as_matrix(x), 1, &xq, (save & 1) ? &xt : nullptr);
-    quantize(weight, kBlock, &wq, (save & 2) ? &wt : nullptr);
-    at::Tensor y = result_like(x, weight.size(0));
-    at::Tensor y2 = y.view({xq.values.size(0), weight.size(0)});
-    matmul(xq, wq, y2);
-    for (Held *h : {&xt, &wt})
-        if (!h->values.defined()) h->values = h->scales = none(x);
-    return {y, xt.values, xt.scales, wt.values, wt.scales};
+    TORCH_CHECK(x.device().is_cuda() && weight.device() == x.device() && weight.dim() == 2 &&
+                    x.dim() >= 1 && weight.size(1) == x.size(-1) && weight.numel() > 0,
+                "fp8: x [.., K] and weight [N, K] on one ROCm (HIP) device");
+    const int64_t rows = rows_of(x), k = weight.size(1), n = weight.size(0);
+    const Layout q{rows, k, 1, false}, xt{k, rows, 1, false}, w{n, k, kBlock, false},
+        wt{k, n, kBlock, true};
+    at::Tensor y = result_like(x, n), xq = q.empty(x), wq = w.empty(x);
+    at::Tensor saved_x = (save & 1) ? xt.empty(x) : at::Tensor();
+    at::Tensor saved_w = (save & 2) ? wt.empty(x) : at::Tensor();
+    hold_rows(x, xq, saved_x);
+    const Rows r = as_rows(weight);
+    muon_train_fp8_quantize_args a{};
+    a.rows = n;
+    a.cols = k;
+    a.ld_x = r.ld;
+    a.x = r.t.data_ptr();
+    a.x_dtype = dtype_of(weight, "fp8: the weight");
+    a.block_rows = static_cast<int>(kBlock);
+    a.values = w.values(wq);
+    muon_train_fp8_operand held = w.operand(wq);
+    if (saved_w.defined()) {  // one set of scales serves both
+        a.values_t = wt.values(saved_w);
+        held.scales = wt.scales(saved_w);
+    }
+    a.scales = const_cast<float *>(held.scales);
+    const int st = muon_train_fp8_quantize(&a, stream_of(x));
+    TORCH_CHECK(st == MUON_POLAR_OK, "fp8: ", muon_polar_last_error());
+    multiply(q.operand(xq), rows, held, n, q.width(), y);
+    for (at::Tensor *t : {&saved_x, &saved_w})
+        if (!t->defined()) *t = none(x);
+    return {y, saved_x, saved_w};
 }
 
 // Gradients of x (with the saved transposed weight) and of the weight (with the saved
-// transposed x), as wanted (1: x, 2: weight).
-std::tuple<at::Tensor, at::Tensor> Fp8LinearBackward(const at::Tensor &dy, const at::Tensor &xt_values,
-                                                     const at::Tensor &xt_scales,
-                                                     const at::Tensor &wt_values,
-                                                     const at::Tensor &wt_scales,
+// transposed x) of k columns, as wanted (1: x, 2: weight).
+std::tuple<at::Tensor, at::Tensor> Fp8LinearBackward(const at::Tensor &dy, const at::Tensor &saved_x,
+                                                     const at::Tensor &saved_w, int64_t k,
                                                      at::ScalarType weight_dtype, int64_t wanted) {
     const c10::OptionalDeviceGuard device_guard(dy.device());
-    Held g, gt;
-    const at::Tensor dy2 = as_matrix(dy);
-    quantize(dy2, 1, (wanted & 1) ? &g : nullptr, (wanted & 2) ? &gt : nullptr);
+    TORCH_CHECK(dy.device().is_cuda() && dy.dim() >= 1 && dy.size(-1) > 0,
+                "fp8: a gradient [.., N] on a ROCm (HIP) device is needed");
+    const int64_t rows = rows_of(dy), n = dy.size(-1);
+    const Layout g{rows, n, 1, false}, gt{n, rows, 1, false}, xt{k, rows, 1, false},
+        wt{k, n, kBlock, true};
+    TORCH_CHECK(!(wanted & 1) || saved_w.numel() == wt.bytes(), "fp8: saved for another gradient");
+    TORCH_CHECK(!(wanted & 2) || saved_x.numel() == xt.bytes(), "fp8: saved for another gradient");
+    const at::Tensor gq = (wanted & 1) ? g.empty(dy) : at::Tensor();
+    const at::Tensor gtq = (wanted & 2) ? gt.empty(dy) : at::Tensor();
+    if (wanted & 3) hold_rows(dy, gq, gtq);
     at::Tensor dx = none(dy), dw = none(dy);
     if (wanted & 1) {
-        dx = result_like(dy, wt_values.size(0));
-        at::Tensor dx2 = dx.view({dy2.size(0), wt_values.size(0)});
-        matmul(g, {wt_values, wt_scales}, dx2);
+        dx = result_like(dy, k);
+        multiply(g.operand(gq), rows, wt.operand(saved_w), k, g.width(), dx);
     }
     if (wanted & 2) {
-        dw = at::empty({dy2.size(1), xt_values.size(0)}, dy.options().dtype(weight_dtype));
-        matmul(gt, {xt_values, xt_scales}, dw);
+        dw = at::empty({n, k}, dy.options().dtype(weight_dtype));
+        multiply(gt.operand(gtq), n, xt.operand(saved_x), k, gt.width(), dw);
     }
     return {dx, dw};
 }
@@ -779,11 +848,10 @@ struct Fp8LinearFunction : torch::autograd::Function<Fp8LinearFunction> {
         const at::AutoDispatchBelowADInplaceOrView below;
         // wanted: 1 x, 2 weight; the weight's gradient needs x saved and the other way round
         const int64_t save = (wanted & 2) >> 1 | (wanted & 1) << 1;
-        auto [y, xt, xts, wt, wts] =
-            MUON_TRAIN_OP("fp8_linear_forward", Fp8LinearForward).call(x, weight, save);
-        ctx->save_for_backward({xt, xts, wt, wts});
-        ctx->saved_data["choices"] =
-            std::vector<int64_t>{wanted, static_cast<int64_t>(weight.scalar_type())};
+        auto [y, xt, wt] = MUON_TRAIN_OP("fp8_linear_forward", Fp8LinearForward).call(x, weight, save);
+        ctx->save_for_backward({xt, wt});
+        ctx->saved_data["choices"] = std::vector<int64_t>{
+            wanted, static_cast<int64_t>(weight.scalar_type()), weight.size(1)};
         return y;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
@@ -791,7 +859,7 @@ struct Fp8LinearFunction : torch::autograd::Function<Fp8LinearFunction> {
         const auto t = ctx->get_saved_variables();
         const auto choices = ctx->saved_data["choices"].toIntVector();
         auto [dx, dw] = MUON_TRAIN_OP("fp8_linear_backward", Fp8LinearBackward)
-                            .call(grads[0], t[0], t[1], t[2], t[3],
+                            .call(grads[0], t[0], t[1], choices[2],
                                   static_cast<at::ScalarType>(choices[1]), choices[0]);
         variable_list result(3);
         if (choices[0] & 1) result[0] = dx;
@@ -849,10 +917,9 @@ TORCH_LIBRARY_FRAGMENT(muon_ascend950, m) {
     m.def("fp8_matmul(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales, ScalarType dtype) -> "
           "Tensor");
     m.def("fp8_linear(Tensor x, Tensor values, Tensor scales) -> Tensor");
-    m.def("fp8_linear_forward(Tensor x, Tensor weight, int save) -> "
-          "(Tensor, Tensor, Tensor, Tensor, Tensor)");
-    m.def("fp8_linear_backward(Tensor dy, Tensor xt_values, Tensor xt_scales, Tensor wt_values, "
-          "Tensor wt_scales, ScalarType weight_dtype, int wanted) -> (Tensor, Tensor)");
+    m.def("fp8_linear_forward(Tensor x, Tensor weight, int save) -> (Tensor, Tensor, Tensor)");
+    m.def("fp8_linear_backward(Tensor dy, Tensor saved_x, Tensor saved_w, int k, "
+          "ScalarType weight_dtype, int wanted) -> (Tensor, Tensor)");
 
     m.def("block_norms(Tensor y, Tensor residual, Tensor? post_weight, Tensor? gate, "
           "Tensor? scale, float scale_value, Tensor? pre_weight, bool post_norm, bool pre_norm, "

@@ -176,6 +176,29 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_kernel(QuantArgs a, in
     asm volatile("s_nop 1");
 }
 
+// Rows alone, for matrices of too few tiles to fill the card: a workgroup takes 16 rows of a
+// block column, a thread eight elements, so that a small call waits for one load.
+template <class T>
+__global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(QuantArgs a, int col_tiles) {
+    const int64_t row = int64_t(blockIdx.x / col_tiles) * 16 + (threadIdx.x >> 4);
+    const int64_t tile_c = blockIdx.x % col_tiles, col0 = tile_c * kBlock + 8 * (threadIdx.x & 15);
+    if (row >= a.rows) return;  // whole rows of 16 lanes
+    const int64_t left = a.cols - col0;
+    Piece<T> p;
+    p.load(static_cast<const typename T::Raw *>(a.x) + row * a.ld_x + col0, left < 0 ? 0 : left > 8 ? 8 : int(left));
+    float x[8], inv[8];
+    p.get(x);
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = umax(m, magnitude(x[e]));
+    const float s = scale_of(row_umax(m)), r = 1.0f / s;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) inv[e] = r;
+    const u32x2 q = to_fp8(x, inv);
+    __builtin_memcpy(static_cast<uint8_t *>(a.values) + row * (int64_t(col_tiles) * kBlock) + col0, &q, 8);
+    if ((threadIdx.x & 15) == 0) a.scales[tile_c * a.rows + row] = s;
+}
+
 // -------------------------------------------------------------------------- products
 // v_mfma_f32_16x16x128_f8f6f4 on e4m3 values: lane l supplies 32 consecutive values (k-part
 // l / 16 of the 128) of row l % 16 of A and of column l % 16 of B, and receives
@@ -870,8 +893,14 @@ extern "C" int muon_train_fp8_quantize(const muon_train_fp8_quantize_args *args,
         return invalid("fp8: values must be 16-byte aligned");
     const int64_t tr = (a.rows + kBlock - 1) / kBlock, tc = (a.cols + kBlock - 1) / kBlock;
     if (tr * tc > INT32_MAX) return invalid("fp8: matrix too large");
-    const dim3 grid(static_cast<uint32_t>(tr * tc));
     const int t = static_cast<int>(tc);
+    if (a.block_rows == 1 && !a.values_t && tr * tc < 512) {
+        const dim3 few(static_cast<uint32_t>((a.rows + 15) / 16 * tc));
+        if (a.x_dtype == MUON_TRAIN_BF16) quantize_rows_kernel<Bf16><<<few, kQuantThreads, 0, stream>>>(a, t);
+        else quantize_rows_kernel<F32><<<few, kQuantThreads, 0, stream>>>(a, t);
+        return launched("fp8_quantize");
+    }
+    const dim3 grid(static_cast<uint32_t>(tr * tc));
     if (a.x_dtype == MUON_TRAIN_BF16) {
         if (a.block_rows == 1) quantize_kernel<Bf16, 1><<<grid, kQuantThreads, 0, stream>>>(a, t);
         else quantize_kernel<Bf16, kBlock><<<grid, kQuantThreads, 0, stream>>>(a, t);

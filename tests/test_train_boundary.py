@@ -273,8 +273,9 @@ def test_fp8_calls_refuse_and_fake():
         assert y.shape == (2, 3, 130) and y.requires_grad
         ops = torch.ops.muon_ascend950
         _, *saved = ops.fp8_linear_forward(x, w, 3)
-        assert saved[0].shape == (300, 128) and saved[2].shape == (300, 256)
-        dx, dw = ops.fp8_linear_backward(y, *saved, F32, 3)
+        # x along 6 tokens, the weight along 130 rows: values, then scales
+        assert saved[0].shape == (300 * 128 + 4 * 300,) and saved[1].shape == (300 * 256 + 4 * 2 * 3,)
+        dx, dw = ops.fp8_linear_backward(y, *saved, 300, F32, 3)
         assert dx.shape == x.shape and dx.dtype == B16 and dw.shape == w.shape and dw.dtype == F32
 
 
