@@ -33,12 +33,12 @@ _fp8_linear_serve = _ops.fp8_linear_serve.default
 _DTYPES = (torch.float32, torch.bfloat16)
 
 
-def _tensors(**named) -> None:
-    """Every argument is a tensor (None: one that may be left out); the operators check the
-    rest."""
-    for name, t in named.items():
-        if t is not None and not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
+def _blame(required, optional) -> None:
+    """After an operator refused its arguments: the one that is no tensor, if any (the
+    operators check the rest; looking first would cost every call a microsecond)."""
+    for name, t in {**required, **optional}.items():
+        if not isinstance(t, torch.Tensor) and (t is not None or name in required):
+            raise TypeError(f"{name} must be a torch.Tensor") from None
 
 
 def block_norms(y: torch.Tensor, residual: torch.Tensor, *, post_weight=None, gate=None,
@@ -58,14 +58,18 @@ def block_norms(y: torch.Tensor, residual: torch.Tensor, *, post_weight=None, ga
     ``[B, ..., D]``) or y's shape.  residual_scale: a number, or a float32 tensor of one
     or D elements.  Gradients of all tensors, those of broadcast ones summed.
     """
-    _tensors(y=y, residual=residual, post_weight=post_weight, gate=gate, pre_weight=pre_weight)
     scale, value = None, 1.0
     if isinstance(residual_scale, torch.Tensor):
         scale = residual_scale
     else:
         value = float(residual_scale)
-    out, normed = _block_norms(y, residual, post_weight, gate, scale, value, pre_weight, post_norm,
-                               pre_norm, eps)
+    try:
+        out, normed = _block_norms(y, residual, post_weight, gate, scale, value, pre_weight,
+                                   post_norm, pre_norm, eps)
+    except Exception:
+        _blame(dict(y=y, residual=residual),
+               dict(post_weight=post_weight, gate=gate, pre_weight=pre_weight))
+        raise
     return out, (normed if pre_norm else None)
 
 
@@ -89,10 +93,13 @@ def distill_topk(logits: torch.Tensor, teacher_logits: torch.Tensor,
     or whose entries are all -inf, has no first term and no gradient from it; a label
     outside ``[0, V)`` (such as -100) leaves its row without the second.
     """
-    _tensors(logits=logits, teacher_logits=teacher_logits, teacher_indices=teacher_indices,
-             labels=labels)
-    return _distill_topk(logits, teacher_logits, teacher_indices, labels, float(temperature),
-                         float(label_weight))
+    try:
+        return _distill_topk(logits, teacher_logits, teacher_indices, labels, temperature,
+                             label_weight)
+    except Exception:
+        _blame(dict(logits=logits, teacher_logits=teacher_logits, teacher_indices=teacher_indices),
+               dict(labels=labels))
+        raise
 
 
 def distill_topk_with_grad(logits: torch.Tensor, teacher_logits: torch.Tensor,
@@ -106,16 +113,18 @@ def distill_topk_with_grad(logits: torch.Tensor, teacher_logits: torch.Tensor,
     grad_loss: a number or float32 ``[...]`` (0 for tokens that do not count).  ``out``
     receives the gradient; it may be ``logits`` itself, which is then overwritten.
     """
-    _tensors(logits=logits, teacher_logits=teacher_logits, teacher_indices=teacher_indices,
-             labels=labels, out=out)
     weight, value = None, 1.0
     if isinstance(grad_loss, torch.Tensor):
         weight = grad_loss
     else:
         value = float(grad_loss)
-    loss, grad = _distill_topk_with_grad(logits, teacher_logits, teacher_indices, labels,
-                                         float(temperature), float(label_weight), weight, value,
-                                         out)
+    try:
+        loss, grad = _distill_topk_with_grad(logits, teacher_logits, teacher_indices, labels,
+                                             temperature, label_weight, weight, value, out)
+    except Exception:
+        _blame(dict(logits=logits, teacher_logits=teacher_logits, teacher_indices=teacher_indices),
+               dict(labels=labels, out=out))
+        raise
     return loss, (grad if out is None else out)
 
 
@@ -229,9 +238,12 @@ def fp8_linear(x: torch.Tensor, weight) -> torch.Tensor:
     and x quantised in blocks of 128 along the axis that each product sums over), or
     ``Fp8Blocks`` (serving: no gradient).
     """
-    _tensors(x=x)
-    if isinstance(weight, Fp8Blocks):
-        return _fp8_linear_serve(x, weight.values, weight.scales, weight.shape[1])
-    if not isinstance(weight, torch.Tensor):
-        raise TypeError("weight must be a torch.Tensor or Fp8Blocks")
-    return _fp8_linear_train(x, weight)
+    try:
+        if isinstance(weight, Fp8Blocks):
+            return _fp8_linear_serve(x, weight.values, weight.scales, weight.shape[1])
+        return _fp8_linear_train(x, weight)
+    except Exception:
+        _blame(dict(x=x), {})
+        if not isinstance(weight, (torch.Tensor, Fp8Blocks)):
+            raise TypeError("weight must be a torch.Tensor or Fp8Blocks") from None
+        raise

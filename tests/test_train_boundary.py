@@ -360,3 +360,14 @@ def test_decode_entry_checks_before_any_launch(change, operand, message):
     for empty in ("m", "n"):
         args = DecodeArgs(**{**base, empty: 0}, w=Operand(**good))
         assert lib.muon_train_fp8_decode(ctypes.byref(args), None) == capi.OK
+
+
+def test_missing_tensors_are_named():
+    with FakeTensorMode():
+        for call, name in ((lambda: train.block_norms(None, _cuda(2, 8)), "y"),
+                           (lambda: train.distill_topk(_cuda(2, 8), None, _cuda(2, 1, dtype=torch.int64)),
+                            "teacher_logits"),
+                           (lambda: train.fp8_linear(None, _cuda(2, 8)), "x"),
+                           (lambda: train.fp8_linear(_cuda(2, 8), 3.0), "weight")):
+            with pytest.raises(TypeError, match=name):
+                call()
