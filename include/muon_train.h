@@ -9,8 +9,9 @@
  * All functions are asynchronous on the given HIP stream.  Pointers are device pointers
  * unless said otherwise; structs are read during the call only.  No function allocates
  * device memory or synchronises.  Return value: MUON_POLAR_OK (0) or a negative
- * muon_polar_status; muon_polar_last_error() gives the detail.  Results are the same
- * bits on every run: no sum depends on the order in which workgroups arrive.
+ * muon_polar_status; muon_polar_last_error() gives the detail.  Outputs must not overlap
+ * inputs or each other but where that is said; the large ones are checked.  Results are the
+ * same bits on every run: no sum depends on the order in which workgroups arrive.
  * No reference counterpart: the reference orthogonalises one matrix and leaves the
  * training step to its caller (README.md:130).
  */

@@ -14,6 +14,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include "muon_train.h"
@@ -130,7 +131,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> NormsForward(
             rows_per_sequence, post_norm, pre_norm, eps);
     at::Tensor out = at::empty(y.sizes(), residual.options());
     at::Tensor normed = pre_norm ? at::empty(y.sizes(), y.options()) : none(y);
-    at::Tensor stats = at::empty({save ? n.a.rows : 0, 2}, y.options().dtype(at::kFloat));
+    at::Tensor stats;
+    if (save) stats = at::empty({n.a.rows, 2}, y.options().dtype(at::kFloat));
     n.a.residual_out = out.data_ptr();
     if (pre_norm) n.a.normed = normed.data_ptr();
     if (save) n.a.stats = stats.data_ptr<float>();
@@ -256,7 +258,8 @@ std::tuple<at::Tensor, at::Tensor> DistillForward(const at::Tensor &logits,
     const c10::OptionalDeviceGuard device_guard(logits.device());
     Distill d(logits, teacher_logits, teacher_indices, labels, temperature, label_weight);
     at::Tensor loss = d.per_row(logits);
-    at::Tensor stats = at::empty({save ? d.a.rows : 0, 4}, loss.options());
+    at::Tensor stats;
+    if (save) stats = at::empty({d.a.rows, 4}, loss.options());
     d.a.loss = loss.data_ptr<float>();
     if (save) d.a.stats = stats.data_ptr<float>();
     const int st = muon_train_distill_forward(&d.a, stream_of(logits));
@@ -611,8 +614,19 @@ constexpr at::ScalarType kFp8[] = {at::kFloat8_e4m3fn};
 bool wants_grad(const at::Tensor &t) { return t.requires_grad(); }
 bool wants_grad(const OptTensor &t) { return given(t) && t->requires_grad(); }
 OptTensor maybe(const at::Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
-void no_second_gradient(const char *what) {
-    TORCH_CHECK(!at::GradMode::is_enabled(), what, ": its gradient has no gradient of its own");
+// Gradients that have none of their own: in a pass that keeps its graph, asking them for one
+// is an error.
+variable_list only_once(variable_list grads, const char *what) {
+    if (!at::GradMode::is_enabled()) return grads;
+    for (at::Tensor &g : grads) {
+        if (!g.defined()) continue;
+        g = g.detach();
+        g.set_requires_grad(true);
+    }
+    const auto error = std::make_shared<torch::autograd::DelayedError>(
+        std::string(what) + ": its gradient has no gradient of its own",
+        static_cast<int64_t>(grads.size()));
+    return (*error)(std::move(grads));
 }
 
 // ---------------------------------------------------------------------------- norms
@@ -660,7 +674,6 @@ struct BlockNormsFunction : torch::autograd::Function<BlockNormsFunction> {
         return {out, normed};
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        no_second_gradient("block_norms");
         variable_list result(13);
         const bool pre_norm = ctx->saved_data["choices"].toIntVector()[3];
         if (!grads[0].defined() && !(grads[1].defined() && pre_norm)) return result;
@@ -668,6 +681,7 @@ struct BlockNormsFunction : torch::autograd::Function<BlockNormsFunction> {
         const auto numbers = ctx->saved_data["numbers"].toDoubleVector();
         const auto choices = ctx->saved_data["choices"].toIntVector();
         const int64_t wanted = choices[4];
+        const at::AutoDispatchBelowADInplaceOrView below;
         auto [dy, dr, d_post, d_gate, d_scale, d_pre] =
             MUON_TRAIN_OP("norms_backward", NormsBackward)
                 .call(t[0], t[1], maybe(t[2]), maybe(t[3]), maybe(t[4]), numbers[0], maybe(t[5]),
@@ -679,7 +693,7 @@ struct BlockNormsFunction : torch::autograd::Function<BlockNormsFunction> {
         if (wanted & 2) result[3] = d_gate;
         if (wanted & 4) result[4] = d_scale;
         if (wanted & 8) result[5] = d_pre;
-        return result;
+        return only_once(std::move(result), "block_norms");
     }
 };
 
@@ -785,13 +799,13 @@ struct DistillFunction : torch::autograd::Function<DistillFunction> {
         return loss;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        no_second_gradient("distill_topk");
+        const at::AutoDispatchBelowADInplaceOrView below;
         const auto t = ctx->get_saved_variables();
         const auto numbers = ctx->saved_data["numbers"].toDoubleVector();
         variable_list result(6);
         result[0] = MUON_TRAIN_OP("distill_backward", DistillBackward)
                         .call(t[0], t[1], t[2], maybe(t[3]), numbers[0], numbers[1], t[4], grads[0]);
-        return result;
+        return only_once(std::move(result), "distill_topk");
     }
 };
 
@@ -855,7 +869,7 @@ struct Fp8LinearFunction : torch::autograd::Function<Fp8LinearFunction> {
         return y;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        no_second_gradient("fp8_linear");
+        const at::AutoDispatchBelowADInplaceOrView below;
         const auto t = ctx->get_saved_variables();
         const auto choices = ctx->saved_data["choices"].toIntVector();
         auto [dx, dw] = MUON_TRAIN_OP("fp8_linear_backward", Fp8LinearBackward)
@@ -864,7 +878,7 @@ struct Fp8LinearFunction : torch::autograd::Function<Fp8LinearFunction> {
         variable_list result(3);
         if (choices[0] & 1) result[0] = dx;
         if (choices[0] & 2) result[1] = dw;
-        return result;
+        return only_once(std::move(result), "fp8_linear");
     }
 };
 

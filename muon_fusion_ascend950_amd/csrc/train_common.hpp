@@ -29,6 +29,12 @@ inline int launched(const char *what) {
     return muon_polar::report(MUON_POLAR_ERR_HIP, msg);
 }
 
+// Whether two buffers meet (a null one meets none).
+inline bool meet(const void *a, int64_t a_bytes, const void *b, int64_t b_bytes) {
+    const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && x < y + static_cast<uintptr_t>(b_bytes) && y < x + static_cast<uintptr_t>(a_bytes);
+}
+
 // Compute units of the current device (asked once per device), or 0 with an error.
 int compute_units() noexcept;
 

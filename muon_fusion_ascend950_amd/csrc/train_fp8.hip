@@ -893,6 +893,11 @@ extern "C" int muon_train_fp8_quantize(const muon_train_fp8_quantize_args *args,
         return invalid("fp8: values must be 16-byte aligned");
     const int64_t tr = (a.rows + kBlock - 1) / kBlock, tc = (a.cols + kBlock - 1) / kBlock;
     if (tr * tc > INT32_MAX) return invalid("fp8: matrix too large");
+    const int64_t x_bytes = ((a.rows - 1) * a.ld_x + a.cols) * (a.x_dtype == MUON_TRAIN_BF16 ? 2 : 4);
+    const int64_t v_bytes = a.rows * tc * kBlock, t_bytes = a.cols * tr * kBlock;
+    if (meet(a.x, x_bytes, a.values, v_bytes) || meet(a.x, x_bytes, a.values_t, t_bytes) ||
+        meet(a.values, v_bytes, a.values_t, t_bytes))
+        return invalid("fp8: x and values must not overlap");
     const int t = static_cast<int>(tc);
     if (a.block_rows == 1 && !a.values_t && tr * tc < 512) {
         const dim3 few(static_cast<uint32_t>((a.rows + 15) / 16 * tc));
@@ -926,6 +931,10 @@ extern "C" int muon_train_fp8_matmul(const muon_train_fp8_matmul_args *args, hip
         if (st == MUON_POLAR_OK) st = check(g.b, g.k);
         if (st != MUON_POLAR_OK) return st;
     }
+    const int64_t c_bytes = ((g.m - 1) * g.ldc + g.n) * (g.c_dtype == MUON_TRAIN_BF16 ? 2 : 4);
+    if (g.k > 0 && (meet(g.c, c_bytes, g.a.values, (g.m - 1) * g.a.ld + g.k) ||
+                    meet(g.c, c_bytes, g.b.values, (g.n - 1) * g.b.ld + g.k)))
+        return invalid("fp8: c must not overlap its operands");
     const int cus = compute_units();
     if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "fp8: no device");
     if (g.k > 0 && g.m <= kFewRows && g.a.block_rows == 1 && g.b.block_rows == kBlock) {
@@ -958,6 +967,11 @@ extern "C" int muon_train_fp8_decode(const muon_train_fp8_decode_args *args, hip
     const int st = check(g.w, blocks * kBlock);
     if (st != MUON_POLAR_OK) return st;
     if (g.w.block_rows != kBlock) return invalid("fp8: block_rows of w must be 128");
+    const int64_t c_bytes = ((g.m - 1) * g.ldc + g.n) * (g.c_dtype == MUON_TRAIN_BF16 ? 2 : 4);
+    const int64_t x_bytes = ((g.m - 1) * g.ld_x + g.cols) * (g.x_dtype == MUON_TRAIN_BF16 ? 2 : 4);
+    if (meet(g.c, c_bytes, g.x, x_bytes) ||
+        meet(g.c, c_bytes, g.w.values, (g.n - 1) * g.w.ld + blocks * kBlock))
+        return invalid("fp8: c must not overlap its operands");
     const int cus = compute_units();
     if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "fp8: no device");
     const DecodeArgs d{g.n, g.ld_x, int(g.m), int(g.cols), int(blocks), g.x, nullptr, 0,

@@ -19,6 +19,7 @@
 #include "train_common.hpp"
 
 #include <mutex>
+#include <utility>
 
 namespace muon_train {
 
@@ -497,6 +498,21 @@ int check(const Args *a) {
     return MUON_POLAR_OK;
 }
 
+// Whether an output [rows, d] meets one of the inputs that a pass reads, or another output.
+bool outputs_meet(const Args &a, const void *r_out, const void *y_out, const void *r_in,
+                  const void *y_in) {
+    const int64_t sy = a.y_dtype == MUON_TRAIN_BF16 ? 2 : 4, sr = a.residual_dtype == MUON_TRAIN_BF16 ? 2 : 4;
+    const int64_t whole_y = a.rows * a.d * sy, whole_r = a.rows * a.d * sr;
+    const int64_t span_y = ((a.rows - 1) * a.ld_y + a.d) * sy;
+    const int64_t span_r = ((a.rows - 1) * a.ld_residual + a.d) * sr;
+    bool bad = meet(r_out, whole_r, y_out, whole_y);
+    const std::pair<const void *, int64_t> outs[] = {{r_out, whole_r}, {y_out, whole_y}};
+    for (const auto &[out, bytes] : outs)
+        bad = bad || meet(out, bytes, a.y, span_y) || meet(out, bytes, a.residual, span_r) ||
+              meet(out, bytes, r_in, whole_r) || meet(out, bytes, y_in, whole_y);
+    return bad;
+}
+
 }  // namespace
 
 int compute_units() noexcept {
@@ -523,6 +539,8 @@ extern "C" int muon_train_norms_forward(const muon_train_norms_args *args, hipSt
     if (st != MUON_POLAR_OK || args->rows == 0) return st;
     const Args a = *args;
     if (!a.residual_out || (a.pre_norm && !a.normed)) return invalid("norms: null output");
+    if (outputs_meet(a, a.residual_out, a.pre_norm ? a.normed : nullptr, nullptr, nullptr))
+        return invalid("norms: outputs must not overlap inputs or each other");
     const int cus = compute_units();
     if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "norms: no device");
     const Shape s = forward_shape(a.d);
@@ -556,6 +574,8 @@ extern "C" int muon_train_norms_backward(const muon_train_norms_args *args, void
     const int cus = compute_units();
     if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "norms: no device");
     if (a.rows > 0 && (!a.stats || !a.d_y || !a.d_residual)) return invalid("norms: null output");
+    if (a.rows > 0 && outputs_meet(a, a.d_residual, a.d_y, a.d_residual_out, a.d_normed))
+        return invalid("norms: outputs must not overlap inputs or each other");
     const BackwardPlan p = backward_plan(a, cus);
     if (workspace_bytes < p.bytes || (p.bytes > 0 && !workspace))
         return muon_polar::report(MUON_POLAR_ERR_WORKSPACE, "norms: workspace missing or too small");

@@ -115,12 +115,13 @@ class NormsArgs(ctypes.Structure):
     (dict(gate_kind=2, rows_per_sequence=3, gate=4096), "rows_per_sequence"),
     (dict(gate_kind=1), "null"), (dict(scale_kind=1), "null"), (dict(y=None), "null"),
     (dict(ld_y=7), "overlap"), (dict(residual_out=None), "null output"),
-    (dict(normed=None), "null output"),
+    (dict(normed=None), "null output"), (dict(normed=(1 << 20) + 124), "overlap"),
+    (dict(residual_out=(1 << 21) - 124), "overlap"), (dict(normed=(1 << 22) + 64), "overlap"),
 ])
 def test_norms_entry_checks_before_any_launch(change, message):
     lib = capi.load()
-    base = dict(rows=4, d=8, rows_per_sequence=4, ld_y=8, ld_residual=8, y=4096, residual=4096,
-                eps=1e-6, pre_norm=1, residual_out=4096, normed=4096)
+    base = dict(rows=4, d=8, rows_per_sequence=4, ld_y=8, ld_residual=8, y=1 << 20, residual=1 << 21,
+                eps=1e-6, pre_norm=1, residual_out=1 << 22, normed=1 << 23)
     args = NormsArgs(**{**base, **change})
     assert lib.muon_train_norms_forward(ctypes.byref(args), None) == capi.ERR_INVALID_ARGUMENT
     assert message in capi.last_error()
@@ -299,11 +300,11 @@ class MatmulArgs(ctypes.Structure):
     (dict(rows=-1), "rows"), (dict(cols=1 << 31), "cols"), (dict(x_dtype=3), "dtype"),
     (dict(block_rows=64), "block_rows"), (dict(x=None), "null"), (dict(values=None), "null"),
     (dict(scales=None), "null"), (dict(values_t=4096), "null"), (dict(ld_x=9), "overlap"),
-    (dict(values=4100), "aligned"), (dict(rows=1 << 30, cols=1 << 30, ld_x=1 << 30), "too large"),
+    (dict(values=4100), "aligned"), (dict(x=(1 << 21) + 16), "overlap"), (dict(rows=1 << 30, cols=1 << 30, ld_x=1 << 30), "too large"),
 ])
 def test_quantize_entry_checks_before_any_launch(change, message):
     lib = capi.load()
-    base = dict(rows=4, cols=10, ld_x=10, x=4096, block_rows=1, values=4096, scales=4096)
+    base = dict(rows=4, cols=10, ld_x=10, x=1 << 20, block_rows=1, values=1 << 21, scales=1 << 22)
     args = QuantizeArgs(**{**base, **change})
     assert lib.muon_train_fp8_quantize(ctypes.byref(args), None) == capi.ERR_INVALID_ARGUMENT
     assert message in capi.last_error()
@@ -319,12 +320,14 @@ def test_quantize_entry_checks_before_any_launch(change, message):
     ({}, dict(scales=None), "null"), ({}, dict(values=4104), "aligned"), ({}, dict(ld=264), "aligned"),
     ({}, dict(ld=128), "overlap"), ({}, dict(ld=1 << 23), "far apart"),
     ({}, dict(block_rows=2), "block_rows"), ({}, dict(scale_row=2), "next to each other"),
+    ({}, dict(scale_row=1 << 27), "far apart"), ({}, dict(scale_col=1 << 28), "far apart"),
+    (dict(c=(1 << 20) + 128), {}, "overlap"),
     (dict(m=1 << 30, n=1 << 30, ldc=1 << 30), {}, None),
 ])
 def test_matmul_entry_checks_before_any_launch(change, operand, message):
     lib = capi.load()
-    good = dict(values=4096, scales=4096, ld=256, scale_row=1, scale_col=4, block_rows=1)
-    base = dict(m=4, n=8, k=256, c=4096, ldc=8)
+    good = dict(values=1 << 20, scales=1 << 22, ld=256, scale_row=1, scale_col=4, block_rows=1)
+    base = dict(m=4, n=8, k=256, c=1 << 24, ldc=8)
     args = MatmulArgs(**{**base, **change}, a=Operand(**{**good, **operand}), b=Operand(**good))
     status = lib.muon_train_fp8_matmul(ctypes.byref(args), None)
     if message is None:  # too large, or no device to say for
@@ -347,12 +350,13 @@ class DecodeArgs(ctypes.Structure):
     (dict(x_dtype=2), {}, "dtype"), (dict(x=None), {}, "null"), (dict(c=None), {}, "null"),
     (dict(ld_x=199), {}, "overlap"), (dict(ldc=7), {}, "overlap"),
     ({}, dict(ld=128), "overlap"), ({}, dict(values=4104), "aligned"),
-    ({}, dict(block_rows=1), "block_rows"),
+    ({}, dict(block_rows=1), "block_rows"), (dict(c=(1 << 23) - 4), {}, "overlap"),
+    (dict(x=(1 << 24) + 4), {}, "overlap"),
 ])
 def test_decode_entry_checks_before_any_launch(change, operand, message):
     lib = capi.load()
-    good = dict(values=4096, scales=4096, ld=256, scale_row=1, scale_col=4, block_rows=128)
-    base = dict(m=4, n=8, cols=200, ld_x=200, x=4096, c=4096, ldc=8)
+    good = dict(values=1 << 20, scales=1 << 22, ld=256, scale_row=1, scale_col=4, block_rows=128)
+    base = dict(m=4, n=8, cols=200, ld_x=200, x=1 << 23, c=1 << 24, ldc=8)
     args = DecodeArgs(**{**base, **change}, w=Operand(**{**good, **operand}))
     assert lib.muon_train_fp8_decode(ctypes.byref(args), None) == capi.ERR_INVALID_ARGUMENT
     assert message in capi.last_error()

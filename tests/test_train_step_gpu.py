@@ -51,3 +51,19 @@ def test_traced_step_equals_eager():
     got = run(torch.compile(step, backend="aot_eager", fullgraph=True))
     # the sums around the operators are torch's and may be fused differently: none is here
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_gradients_have_none_of_their_own():
+    """A pass that keeps its graph gives the same gradients; differentiating them is refused."""
+    gen = torch.Generator().manual_seed(1)
+    x = torch.randn(20, 160, generator=gen).cuda().requires_grad_(True)
+    w = torch.randn(130, 160, generator=gen).cuda().requires_grad_(True)
+    teacher = torch.randn(20, 3, generator=gen).cuda()
+    index = torch.randint(0, 130, (20, 3), generator=gen).cuda()
+    for out in (train.block_norms(x, x, gate=w[0])[1].sum(), train.fp8_linear(x, w).sum(),
+                train.distill_topk(x, teacher, index).sum()):
+        (plain,) = torch.autograd.grad(out, x, retain_graph=True)
+        (kept,) = torch.autograd.grad(out, x, create_graph=True)
+        assert torch.equal(plain, kept)
+        with pytest.raises(RuntimeError, match="no gradient of its own"):
+            kept.sum().backward()
