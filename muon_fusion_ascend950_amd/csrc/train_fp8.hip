@@ -366,6 +366,8 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
     MatmulArgs g, int tiles_m, int tiles_n) {
     using Geo = Geometry<BM, BN, WM, WN, D>;
     constexpr int SM = WM / 16, SN = WN / 16, kLoads = Geo::kLoads;
+    // The pipeline's registers leave no room for bf16 fragments (kExact) or a scale for each
+    // column (kRowB: 60 spilled, 8192 x 14336 x 8192 in 1275 us against 1004 without).
     constexpr bool kPipelined = Geo::kTwoSlots && !kExact && !kRowB;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[D * Geo::kSlot];
     const int lane = threadIdx.x & 63;
@@ -506,9 +508,9 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
         // one's first loads.  (A workgroup a tile: 12 us between one tile's last step and the
         // next one's first, 84 of 439 us there.)
         constexpr int kQ = SM * SN, kLag = 2, kBar = (SM - 2) * SN, kLast = (SM - 1) * SN;
-        static_assert(D == 2 && !kExact && SM % 4 == 0 && kQ % 4 == 0 && kLag < SN, "schedule");
+        static_assert(D == 2 && SM % 4 == 0 && kQ % 4 == 0 && kLag < SN, "schedule");
         Frag<false> fa[4], fb[SN];
-        f32x4 t[4], sn[kRowB ? SN : 1], sn_last[kRowB ? SN : 1];
+        f32x4 t[4];
         float f[SM], sb = 0.0f, factor = 0.0f;  // a's scales, b's, their product for the block at hand
         auto base_of = [&](int s) { return smem + s * Geo::kSlot; };
         auto read_a = [&](const uint8_t *base, auto ic) {
@@ -521,25 +523,18 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
         };
         auto read_scales = [&](const uint8_t *base) {
             const float *scale_m = reinterpret_cast<const float *>(base + Geo::kPanels) + wm + r;
-            const float *scale_n = reinterpret_cast<const float *>(base + Geo::kPanels) + BM + wn;
             static_for<SM>([&](auto ic) { f[ic] = scale_m[16 * ic]; });
-            if constexpr (!kRowB) sb = scale_n[0];
-            if constexpr (kRowB)
-                static_for<SN>([&](auto jc) {
-                    sn[jc] = *reinterpret_cast<const f32x4 *>(scale_n + 16 * jc + 4 * part);
-                });
+            sb = *(reinterpret_cast<const float *>(base + Geo::kPanels) + BM + wn);
         };
-        auto add = [&](auto qc, const f32x4 &factor_n) {
+        auto add = [&](auto qc) {
             constexpr int q = decltype(qc)::value, i = q / SN, j = q % SN;
-            if constexpr (j == 0) factor = kRowB ? f[i] : f[i] * sb;
+            if constexpr (j == 0) factor = f[i] * sb;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                acc[i][j][e] = fmaf(t[q % 4][e], kRowB ? factor * factor_n[e] : factor, acc[i][j][e]);
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(t[q % 4][e], factor, acc[i][j][e]);
         };
         auto clear = [&] {  // nothing summed, nothing left to add
             factor = 0.0f;
             static_for<4>([&](auto c) { t[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; });
-            if constexpr (kRowB) static_for<SN>([&](auto c) { sn_last[c] = t[0]; });
 #pragma unroll
             for (int i = 0; i < SM; ++i)
 #pragma unroll
@@ -566,14 +561,10 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
                     static_for<kQ>([&](auto qc) {
                         constexpr int q = decltype(qc)::value, i = q / SN, j = q % SN;
                         if constexpr (q == kBar) muon_polar::wait_vm_barrier<0>();
-                        if constexpr (q == kLast && kRowB) static_for<SN>([&](auto c) { sn_last[c] = sn[c]; });
                         t[q % 4] = multiply(fb[j], fa[i % 4]);
                         __builtin_amdgcn_sched_barrier(0);
-                        constexpr int p = (q + kQ - kLag) % kQ;  // kLag before, maybe last step's
-                        if constexpr (q < kLag || q - kLag >= kLast)
-                            add(std::integral_constant<int, p>{}, sn_last[kRowB ? p % SN : 0]);
-                        else
-                            add(std::integral_constant<int, p>{}, sn[kRowB ? p % SN : 0]);
+                        // that of kLag before, at first the last step's
+                        add(std::integral_constant<int, (q + kQ - kLag) % kQ>{});
                         if constexpr (j == 0 && i + 3 < SM)
                             read_a(base, std::integral_constant<int, i + 3>{});
                         if constexpr (q >= kBar) {
@@ -594,8 +585,7 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
                 }
             }
             static_for<kLag>([&](auto c) {
-                add(std::integral_constant<int, kQ - kLag + decltype(c)::value>{},
-                    sn_last[kRowB ? SN - kLag + decltype(c)::value : 0]);
+                add(std::integral_constant<int, kQ - kLag + decltype(c)::value>{});
             });
             store(tile);
             clear();
@@ -828,8 +818,6 @@ void launch_few_rows(const DecodeArgs &a, int cus, hipStream_t stream) {
     }
 }
 
-// Tiles by how many of them there are: 256 x 256 where they occupy most compute units,
-// 128 x 128 where those do, else 64 x 64.
 template <int BM, int BN, int WM, int WN, int D>
 void launch_tiles(const MatmulArgs &g, int cus, hipStream_t stream) {
     using Geo = Geometry<BM, BN, WM, WN, D>;
@@ -945,10 +933,22 @@ extern "C" int muon_train_fp8_matmul(const muon_train_fp8_matmul_args *args, hip
     }
     auto tiles = [&](int64_t t) { return ((g.m + t - 1) / t) * ((g.n + t - 1) / t); };
     if (tiles(64) > INT32_MAX) return invalid("fp8: matrix too large");
+    // A tile takes a compute unit's share of the tiles in turn: the tile whose turns, at the
+    // time of one of its own size, end first.  Times as shares of a 256 x 256 tile's, measured
+    // at K = 4096 (us a turn): 128 x 128 19.5 of 55, in fp32 32 of 110; 64 x 64 7.7 and 13.3.
+    // On both sides of the borders: 1024 x 2048 in 64s 17.3 us, in 128s 27.3; 1024 x 4096
+    // 31.3 and 28.1; 2048 x 4096 in 128s 40.0, in 256s 51.6; 3000 x 4096 59.1 and 53.6 (fp32
+    // 100 and 111); 4096 x 6144 112 and 105 (fp32 192 and 215).
+    const bool exact = g.c_dtype == MUON_TRAIN_F32;
+    auto cost = [&](int64_t t, int share) { return (tiles(t) + cus - 1) / cus * share; };
+    const int64_t cost64 = cost(64, exact ? 12 : 14), cost128 = cost(128, exact ? 29 : 35);
     // (a single block of K leaves nothing to pipeline)
-    if (g.k == kBlock || 2 * tiles(128) < cus) launch_tiles<64, 64, 32, 32, 4>(g, cus, stream);
-    else if (2 * tiles(256) >= cus) launch_tiles<256, 256, 128, 64, 2>(g, cus, stream);
-    else launch_tiles<128, 128, 64, 64, 2>(g, cus, stream);
+    if (g.k <= kBlock || (cost64 <= cost128 && cost64 <= cost(256, 100)))
+        launch_tiles<64, 64, 32, 32, 4>(g, cus, stream);
+    else if (cost128 <= cost(256, 100))
+        launch_tiles<128, 128, 64, 64, 2>(g, cus, stream);
+    else
+        launch_tiles<256, 256, 128, 64, 2>(g, cus, stream);
     return launched("fp8_matmul");
 }
 
