@@ -171,7 +171,7 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_kernel(QuantArgs a, in
                                        tile_r * kBlock + b) =
                 *reinterpret_cast<const u32x4 *>(turned + c * kTilePitch + b);
     }
-    // The check of store-data hazards reads the code in address order, past the program's
+    // tests/isa_hazards.py reads the code in address order, past the program's
     // end: two wait states keep it from pairing the last store with the block laid out there.
     asm volatile("s_nop 1");
 }
