@@ -268,6 +268,24 @@ __device__ __forceinline__ void dma_4B_step(muon_polar::i32x4 rsrc, uint32_t lds
                  : "memory");
 }
 
+// Waits for the oldest of this wave's memory instructions, the kLate behind them left under
+// way if `behind` says that there are so many, and meets the workgroup's other waves.  (Branching
+// inside one statement: a branch of the program's own splits the schedule around it, and the
+// registers spill, 5.6 times the time.)
+template <int kLate>
+__device__ __forceinline__ void wait_dma_barrier(int behind) {
+    static_assert(kLate <= 63, "vmcnt range");
+    asm volatile("s_cmp_lg_u32 %0, 0\n\t"
+                 "s_cbranch_scc1 .Ldma%=\n\t"
+                 "s_waitcnt vmcnt(0)\n"
+                 ".Ldma%=:\n\t"
+                 "s_waitcnt vmcnt(%1) lgkmcnt(0)\n\t"
+                 "s_barrier"
+                 :
+                 : "s"(behind), "n"(kLate)
+                 : "memory", "scc");
+}
+
 // Four consecutive results of a row, the first `count` of them inside the matrix.
 __device__ __forceinline__ void store4(void *c, int64_t at, int count, int dtype, f32x4 v) {
     if (dtype == MUON_TRAIN_BF16) {
@@ -356,6 +374,7 @@ struct Geometry {
     static constexpr int kScaleLoads = (BM + BN) / 64;      // 256 B ones of the workgroup
     static_assert(kPanels % (1024 * kWaves) == 0 && BM % 64 == 0 && BN % 64 == 0, "whole DMA blocks");
     static_assert(kScaleLoads <= kWaves, "one scale load a wave");
+    static_assert(BM % (8 * kLoads) == 0, "a wave loads from one panel");
     static_assert((D - 1) * (kLoads + 1) <= 63, "vmcnt range");
     static_assert(D * kSlot <= 160 * 1024, "LDS");
     static constexpr bool kTwoSlots = D == 2;
@@ -380,7 +399,9 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
     const int sblock = wave % Geo::kScaleLoads;
     const bool scale_a = sblock * 64 < BM;
     const muon_train_fp8_operand &so = scale_a ? g.a : g.b;
-    i32x4 rs_a, rs_b, rs_scale;
+    const bool load_a = 8 * wave * kLoads < BM;  // a wave's rows are all a's or all b's
+    const muon_train_fp8_operand &lo = load_a ? g.a : g.b;
+    i32x4 rs, rs_scale;
     uint32_t off[kLoads], soff;
     const uint32_t sstep = static_cast<uint32_t>(4 * so.scale_col);
     auto aim = [&](int tile) {  // at a tile's first step
@@ -389,19 +410,15 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
         const int64_t m0 = int64_t(tm) * BM, n0 = int64_t(tn) * BN;
         const int rows_m = g.m - m0 < BM ? int(g.m - m0) : BM;
         const int rows_n = g.n - n0 < BN ? int(g.n - n0) : BN;
-        rs_a = muon_polar::make_buffer_rsrc(static_cast<const uint8_t *>(g.a.values) + m0 * g.a.ld,
-                                            static_cast<uint32_t>(rows_m * g.a.ld));
-        rs_b = muon_polar::make_buffer_rsrc(static_cast<const uint8_t *>(g.b.values) + n0 * g.b.ld,
-                                            static_cast<uint32_t>(rows_n * g.b.ld));
+        const int rows = load_a ? rows_m : rows_n;
+        rs = muon_polar::make_buffer_rsrc(static_cast<const uint8_t *>(lo.values) + (load_a ? m0 : n0) * lo.ld,
+                                          static_cast<uint32_t>(rows * lo.ld));
 #pragma unroll
         for (int d = 0; d < kLoads; ++d) {
             const int row = 8 * (wave * kLoads + d) + (lane >> 3);
             const int chunk = (lane & 7) ^ ((row >> 1) & 7);
-            const bool is_a = row < BM;
-            const int at = is_a ? row : row - BM;
-            off[d] = at < (is_a ? rows_m : rows_n)
-                         ? static_cast<uint32_t>(at * (is_a ? g.a.ld : g.b.ld) + 16 * chunk)
-                         : muon_polar::kOob;
+            const int at = load_a ? row : row - BM;
+            off[d] = at < rows ? static_cast<uint32_t>(at * lo.ld + 16 * chunk) : muon_polar::kOob;
         }
         const int srow = (scale_a ? sblock * 64 : sblock * 64 - BM) + lane;
         const int64_t sfirst = scale_a ? m0 : n0;
@@ -417,7 +434,7 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
         const int s = step < steps ? step : steps - 1;  // past the end: the last step once more
         if (d < kLoads) {
             const int row0 = 8 * (wave * kLoads + d);
-            dma_16B_step(row0 < BM ? rs_a : rs_b, base + row0 * kBlock, off[d], s * kBlock);
+            dma_16B_step(rs, base + row0 * kBlock, off[d], s * kBlock);
         } else {
             dma_4B_step(rs_scale, base + Geo::kPanels + sblock * 256, soff, s * sstep);
         }
@@ -435,14 +452,16 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
     };
 
     f32x4 acc[SM][SN] = {};
+    // True if each lane's results went out in 2·SM·(kExact ? 2 : 1) whole stores.
     auto store = [&](int tile) {
         int tm, tn;
         tile_of(tile, tiles_m, tiles_n, tm, tn);
         const int64_t m0 = int64_t(tm) * BM + wm, n0 = int64_t(tn) * BN + wn;
+        const bool whole = m0 + WM <= g.m;
         if (SN == 4 && n0 + WN <= g.n) {  // lines of 128 bytes: 64 columns of bf16, 32 of fp32
             auto put = [&](int i, u32x4 v, int half, int64_t bytes) {
                 const int64_t m = m0 + 16 * i + 8 * half + (r & 7);
-                if (m >= g.m) return;
+                if (!whole && m >= g.m) return;
                 uint8_t *row = static_cast<uint8_t *>(g.c) + (m * g.ldc + n0) * (kExact ? 4 : 2);
                 __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any *>(row + bytes + 16 * part + 64 * (r >> 3)));
             };
@@ -476,7 +495,7 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
                     put(i, b, 1, 0);
                 }
             }
-            return;
+            return whole;
         }
 #pragma unroll
         for (int i = 0; i < SM; ++i) {
@@ -488,6 +507,7 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
                 if (n < g.n) store4(g.c, m * g.ldc + n, g.n - n < 4 ? int(g.n - n) : 4, g.c_dtype, acc[i][j]);
             }
         }
+        return false;
     };
     if (steps == 0) {
         for (int tile = blockIdx.x; tile < tiles_m * tiles_n; tile += gridDim.x) store(tile);
@@ -506,7 +526,9 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
         // The workgroup's tiles are one stream of steps: in the last two of a tile the DMA
         // fetches the first two of the next, and a tile's results are stored beside the next
         // one's first loads.  (A workgroup a tile: 12 us between one tile's last step and the
-        // next one's first, 84 of 439 us there.)
+        // next one's first, 84 of 439 us there.)  The first barrier then waits for the DMA
+        // before the stores, not for the stores (418 -> 412 us there); the second one, behind
+        // which the DMA was issued, for both.
         constexpr int kQ = SM * SN, kLag = 2, kBar = (SM - 2) * SN, kLast = (SM - 1) * SN;
         static_assert(D == 2 && SM % 4 == 0 && kQ % 4 == 0 && kLag < SN, "schedule");
         Frag<false> fa[4], fb[SN];
@@ -549,7 +571,7 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
         static_for<3>([&](auto ic) { read_a(base_of(0), ic); });
         static_for<SN>([&](auto jc) { read_b(base_of(0), jc); });
         clear();
-        int slot = 0;
+        int slot = 0, stored = 0;
         for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
             // the steps whose slots take the tile's own steps, then those whose slots take the
             // next tile's (with none left, this one's once more)
@@ -560,7 +582,10 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
                     const uint8_t *base = base_of(slot), *after = base_of(slot ^ 1);
                     static_for<kQ>([&](auto qc) {
                         constexpr int q = decltype(qc)::value, i = q / SN, j = q % SN;
-                        if constexpr (q == kBar) muon_polar::wait_vm_barrier<0>();
+                        if constexpr (q == kBar) {
+                            wait_dma_barrier<2 * SM>(stored);
+                            stored = 0;
+                        }
                         t[q % 4] = multiply(fb[j], fa[i % 4]);
                         __builtin_amdgcn_sched_barrier(0);
                         // that of kLag before, at first the last step's
@@ -587,7 +612,7 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
             static_for<kLag>([&](auto c) {
                 add(std::integral_constant<int, kQ - kLag + decltype(c)::value>{});
             });
-            store(tile);
+            stored = __builtin_amdgcn_readfirstlane(store(tile));
             clear();
         }
     } else {
