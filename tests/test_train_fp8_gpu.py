@@ -131,6 +131,22 @@ def test_exact_sums():
         assert torch.equal(mf.train.fp8_matmul(qa, qb, F32).cpu(), a @ b.t())
 
 
+@pytest.mark.parametrize("m,n,k", [(4100, 4610, 256), (4360, 4501, 640), (4608, 4608, 384), (2200, 2300, 200)])
+def test_workgroups_of_several_tiles(m, n, k):
+    """bf16 results of more tiles than compute units.  Ones and zeros of both signs: a block's
+    sums are whole numbers up to 128, far above what the fp8 MFMAs lose, the total is exact in
+    fp32 and rounded once."""
+    gen = torch.Generator().manual_seed(k)
+    a = torch.randint(-1, 2, (m, k), generator=gen).float().cuda()
+    b = torch.randint(-1, 2, (n, k), generator=gen).float().cuda()
+    blocks = -(-k // 128)
+    qa = mf.train.Fp8Blocks(a.to(F8), torch.ones(m, blocks, device="cuda"))
+    qb = mf.train.Fp8Blocks(b.to(F8), torch.ones(-(-n // 128), blocks, device="cuda"))
+    want = (a @ b.t()).to(B16)
+    for _ in range(3):
+        assert torch.equal(mf.train.fp8_matmul(qa, qb, B16), want)
+
+
 def test_each_block_has_its_scale():
     """One element of a in each block of 128, scales that are powers of two of their place:
     the product of one block with ones, exactly."""
