@@ -156,6 +156,12 @@ typedef struct muon_train_fp8_matmul_args {
     int c_dtype;
 } muon_train_fp8_matmul_args;
 int muon_train_fp8_matmul(const muon_train_fp8_matmul_args *args, hipStream_t stream);
+/* The same with a workspace (16-byte aligned): a product of few tiles and a long k is then
+ * split along k over the compute units, its parts added up in order.  Bytes that it takes, 0 if
+ * it is not split (host call; a null workspace: not split). */
+int muon_train_fp8_matmul_workspace(const muon_train_fp8_matmul_args *args, size_t *bytes);
+int muon_train_fp8_matmul_in(const muon_train_fp8_matmul_args *args, void *workspace,
+                             size_t workspace_bytes, hipStream_t stream);
 
 /* c = held(x) · wᵀ for up to 16 rows of x [m, cols], quantised in blocks of 1 x 128 in the
  * same kernel: the bits of muon_train_fp8_quantize and muon_train_fp8_matmul.  w: rows of

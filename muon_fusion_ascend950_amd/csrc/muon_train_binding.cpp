@@ -372,6 +372,18 @@ muon_train_fp8_operand operand(Held &h, const at::Tensor &like) {
     return o;
 }
 
+// With the workspace that the product asks for (few tiles of a long K).
+void multiply(const muon_train_fp8_matmul_args &g, const at::Tensor &c) {
+    size_t bytes = 0;
+    int st = muon_train_fp8_matmul_workspace(&g, &bytes);
+    at::Tensor workspace;
+    if (st == MUON_POLAR_OK && bytes > 0)
+        workspace = at::empty({static_cast<int64_t>(bytes)}, c.options().dtype(at::kByte));
+    if (st == MUON_POLAR_OK)
+        st = muon_train_fp8_matmul_in(&g, workspace.defined() ? workspace.data_ptr() : nullptr, bytes, stream_of(c));
+    TORCH_CHECK(st == MUON_POLAR_OK, "fp8: ", muon_polar_last_error());
+}
+
 // c [m, n] = a · bᵀ
 void matmul(Held a, Held b, at::Tensor &c) {
     muon_train_fp8_matmul_args g{};
@@ -385,8 +397,7 @@ void matmul(Held a, Held b, at::Tensor &c) {
     g.c = c.data_ptr();
     g.ldc = g.n;
     g.c_dtype = dtype_of(c, "fp8: the result");
-    const int st = muon_train_fp8_matmul(&g, stream_of(c));
-    TORCH_CHECK(st == MUON_POLAR_OK, "fp8: ", muon_polar_last_error());
+    multiply(g, c);
 }
 
 std::tuple<at::Tensor, at::Tensor> QuantizeFp8(const at::Tensor &x, int64_t block_rows) {
@@ -461,8 +472,7 @@ void multiply(const muon_train_fp8_operand &a, int64_t m, const muon_train_fp8_o
     g.k = k;
     g.c = c.data_ptr();
     g.c_dtype = dtype_of(c, "fp8: the result");
-    const int st = muon_train_fp8_matmul(&g, stream_of(c));
-    TORCH_CHECK(st == MUON_POLAR_OK, "fp8: ", muon_polar_last_error());
+    multiply(g, c);
 }
 
 int64_t rows_of(const at::Tensor &x) { return x.size(-1) > 0 ? x.numel() / x.size(-1) : 0; }

@@ -382,7 +382,7 @@ struct Geometry {
 
 template <int BM, int BN, int WM, int WN, int D, bool kExact, bool kRowB>
 __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmul_kernel(
-    MatmulArgs g, int tiles_m, int tiles_n) {
+    MatmulArgs g, int tiles_m, int tiles_n, int parts) {
     using Geo = Geometry<BM, BN, WM, WN, D>;
     constexpr int SM = WM / 16, SN = WN / 16, kLoads = Geo::kLoads;
     // The pipeline's registers leave no room for bf16 fragments (kExact) or a scale for each
@@ -391,7 +391,17 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
     __shared__ __attribute__((aligned(1024))) uint8_t smem[D * Geo::kSlot];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-    const int steps = static_cast<int>(g.k / kBlock);
+    // Workgroup blockIdx.x takes part blockIdx.x % parts of K, steps [first, steps), and leaves its
+    // sums in that part's matrix.  (Pipelined kernels take all of K.)
+    int steps = static_cast<int>(g.k / kBlock), first = 0, at_tile = blockIdx.x;
+    if constexpr (!Geo::kTwoSlots)
+        if (parts > 1) {
+            const int part = at_tile % parts, each = (steps + parts - 1) / parts;
+            at_tile /= parts;
+            first = part * each;
+            steps = first + each < steps ? first + each : steps;
+            g.c = static_cast<float *>(g.c) + part * g.m * g.ldc;
+        }
 
     // DMA: instruction d of this wave moves rows 8·(wave·kLoads + d) .. + 7 of a step's
     // BM + BN panel rows; rows outside the matrices read as zeros.  Behind them the scales:
@@ -616,12 +626,12 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
             clear();
         }
     } else {
-        aim(blockIdx.x);
+        aim(at_tile);
         for (int s = 0; s < D - 1; ++s)
 #pragma unroll
-            for (int d = 0; d <= kLoads; ++d) issue(d, s, s);
+            for (int d = 0; d <= kLoads; ++d) issue(d, first + s, s);
         int slot = 0;
-        for (int k = 0; k < steps; ++k) {
+        for (int k = first; k < steps; ++k) {
             muon_polar::wait_vm_barrier<(D - 2) * (kLoads + 1)>();
             const int next = slot == 0 ? D - 1 : slot - 1;  // the slot that step k - 1 left
             const uint8_t *base = smem + slot * Geo::kSlot;
@@ -652,7 +662,7 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
             }
             slot = slot + 1 == D ? 0 : slot + 1;
         }
-        store(blockIdx.x);
+        store(at_tile);
     }
     muon_polar::wait_vm<0>();  // no DMA into LDS outlives the workgroup
 }
@@ -844,17 +854,17 @@ void launch_few_rows(const DecodeArgs &a, int cus, hipStream_t stream) {
 }
 
 template <int BM, int BN, int WM, int WN, int D>
-void launch_tiles(const MatmulArgs &g, int cus, hipStream_t stream) {
+void launch_tiles(const MatmulArgs &g, bool exact, int parts, int cus, hipStream_t stream) {
     using Geo = Geometry<BM, BN, WM, WN, D>;
     const int tm = static_cast<int>((g.m + BM - 1) / BM), tn = static_cast<int>((g.n + BN - 1) / BN);
-    const bool exact = g.c_dtype == MUON_TRAIN_F32, row_b = g.b.block_rows == 1;
+    const bool row_b = g.b.block_rows == 1;
     // pipelined kernels walk their tiles: as many workgroups as stay resident
     const int64_t tiles = int64_t(tm) * tn;
     const int64_t resident = int64_t(cus) * (160 * 1024 / (D * Geo::kSlot));
-    const dim3 grid(static_cast<uint32_t>(Geo::kTwoSlots && !exact && !row_b && tiles > resident ? resident : tiles));
+    const dim3 grid(static_cast<uint32_t>(Geo::kTwoSlots && !exact && !row_b && tiles > resident ? resident : tiles * parts));
     auto go = [&](auto e, auto r) {
         matmul_kernel<BM, BN, WM, WN, D, decltype(e)::value, decltype(r)::value>
-            <<<grid, Geo::kThreads, 0, stream>>>(g, tm, tn);
+            <<<grid, Geo::kThreads, 0, stream>>>(g, tm, tn, parts);
     };
     using std::bool_constant;
     if (exact && row_b) go(bool_constant<true>{}, bool_constant<true>{});
@@ -929,9 +939,10 @@ extern "C" int muon_train_fp8_quantize(const muon_train_fp8_quantize_args *args,
     return launched("fp8_quantize");
 }
 
-extern "C" int muon_train_fp8_matmul(const muon_train_fp8_matmul_args *args, hipStream_t stream) {
-    if (!args) return invalid("fp8: args is null");
-    const MatmulArgs g = *args;
+namespace muon_train {
+namespace {
+
+int check(const MatmulArgs &g) {
     if (g.m < 0 || g.n < 0 || g.k < 0 || g.m > kMaxExtent || g.n > kMaxExtent || g.k > kMaxExtent)
         return invalid("fp8: m, n and k must be 0 to 2^30");
     if (g.k % kBlock != 0) return invalid("fp8: k must be a multiple of 128");
@@ -948,33 +959,119 @@ extern "C" int muon_train_fp8_matmul(const muon_train_fp8_matmul_args *args, hip
     if (g.k > 0 && (meet(g.c, c_bytes, g.a.values, (g.m - 1) * g.a.ld + g.k) ||
                     meet(g.c, c_bytes, g.b.values, (g.n - 1) * g.b.ld + g.k)))
         return invalid("fp8: c must not overlap its operands");
+    return MUON_POLAR_OK;
+}
+
+int64_t tiles(const MatmulArgs &g, int64_t t) { return ((g.m + t - 1) / t) * ((g.n + t - 1) / t); }
+
+bool few_rows(const MatmulArgs &g) {
+    return g.k > 0 && g.m <= kFewRows && g.a.block_rows == 1 && g.b.block_rows == kBlock;
+}
+
+// Side of a product's tiles.  A tile takes a compute unit's share of the tiles in turn: the
+// tile whose turns, at the time of one of its own size, end first.  Times as shares of a 256 x
+// 256 tile's, measured at K = 4096 (us a turn): 128 x 128 19.5 of 55, in fp32 32 of 110; 64 x
+// 64 7.7 and 13.3.  On both sides of the borders: 1024 x 2048 in 64s 17.3 us, in 128s 27.3;
+// 1024 x 4096 31.3 and 28.1; 2048 x 4096 in 128s 40.0, in 256s 51.6; 3000 x 4096 59.1 and 53.6
+// (fp32 100 and 111); 4096 x 6144 112 and 105 (fp32 192 and 215).
+int tile_side(const MatmulArgs &g, int cus) {
+    if (g.k <= kBlock) return 64;  // a single block of K leaves nothing to pipeline
+    const bool exact = g.c_dtype == MUON_TRAIN_F32;
+    auto cost = [&](int64_t t, int share) { return (tiles(g, t) + cus - 1) / cus * share; };
+    const int64_t cost64 = cost(64, exact ? 12 : 14), cost128 = cost(128, exact ? 29 : 35);
+    if (cost64 <= cost128 && cost64 <= cost(256, 100)) return 64;
+    return cost128 <= cost(256, 100) ? 128 : 256;
+}
+
+// Parts of K that 64 x 64 tiles are split into where they leave compute units idle.  A tile's
+// unit takes in no more than 58 GB/s (29 bytes a clock) however many loads are under way: two
+// rings of half the steps each, in one workgroup, took 31.7 us against 33.6 at 32 x 4096 x
+// 14336, the parts on other units 15.7 with their joining (fp32 50 -> 19.6).  One workgroup a
+// unit: two took 17.4.  A part keeps enough steps to fill its ring, and the join costs what
+// some 16 steps do: 128 x 4096 x 4096 saves 16 of 32 steps, 11.1 and 11.4 us (fp32 16.1 and
+// 14.2); 64 x 4096 x 4096 saves 24, 11.0 and 9.9; 512 x 768 x 2048 would save 8, 7.1 and 8.8.
+int split_parts(const MatmulArgs &g, int cus) {
+    constexpr int kSplitSteps = 4, kSplitGain = 16;
+    if (few_rows(g) || tile_side(g, cus) != 64) return 1;
+    const int64_t steps = g.k / kBlock;
+    int64_t parts = cus / tiles(g, 64);
+    if (parts > steps / kSplitSteps) parts = steps / kSplitSteps;
+    if (parts < 2 || steps - steps / parts < kSplitGain) return 1;
+    const int64_t each = (steps + parts - 1) / parts;
+    return static_cast<int>((steps + each - 1) / each);
+}
+
+int64_t split_pitch(const MatmulArgs &g) { return (g.n + 3) / 4 * 4; }
+int64_t split_bytes(const MatmulArgs &g, int parts) { return parts < 2 ? 0 : 4 * parts * g.m * split_pitch(g); }
+
+// c = the parts' sums in the parts' order, four columns a thread.
+__global__ __launch_bounds__(256) void join_kernel(MatmulArgs g, const float *sums, int64_t pitch, int parts) {
+    const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x, quads = pitch / 4;
+    if (at >= g.m * quads) return;
+    const f32x4 *p = reinterpret_cast<const f32x4 *>(sums) + at;
+    f32x4 total = p[0];
+    for (int i = 1; i < parts; ++i) total += p[i * g.m * quads];
+    const int64_t m = at / quads, n = at % quads * 4;
+    store4(g.c, m * g.ldc + n, g.n - n < 4 ? int(g.n - n) : 4, g.c_dtype, total);
+}
+
+int matmul(const MatmulArgs &g, float *workspace, size_t bytes, hipStream_t stream) {
+    const int st = check(g);
+    if (st != MUON_POLAR_OK || g.m == 0 || g.n == 0) return st;
     const int cus = compute_units();
     if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "fp8: no device");
-    if (g.k > 0 && g.m <= kFewRows && g.a.block_rows == 1 && g.b.block_rows == kBlock) {
+    if (few_rows(g)) {
         const DecodeArgs d{g.n, g.a.ld, int(g.m), int(g.k), int(g.k / kBlock), g.a.values, g.a.scales,
                            g.a.scale_col, g.b, g.c, g.ldc, g.c_dtype};
         launch_few_rows<Held>(d, cus, stream);
         return launched("fp8_matmul");
     }
-    auto tiles = [&](int64_t t) { return ((g.m + t - 1) / t) * ((g.n + t - 1) / t); };
-    if (tiles(64) > INT32_MAX) return invalid("fp8: matrix too large");
-    // A tile takes a compute unit's share of the tiles in turn: the tile whose turns, at the
-    // time of one of its own size, end first.  Times as shares of a 256 x 256 tile's, measured
-    // at K = 4096 (us a turn): 128 x 128 19.5 of 55, in fp32 32 of 110; 64 x 64 7.7 and 13.3.
-    // On both sides of the borders: 1024 x 2048 in 64s 17.3 us, in 128s 27.3; 1024 x 4096
-    // 31.3 and 28.1; 2048 x 4096 in 128s 40.0, in 256s 51.6; 3000 x 4096 59.1 and 53.6 (fp32
-    // 100 and 111); 4096 x 6144 112 and 105 (fp32 192 and 215).
+    if (tiles(g, 64) > INT32_MAX) return invalid("fp8: matrix too large");
     const bool exact = g.c_dtype == MUON_TRAIN_F32;
-    auto cost = [&](int64_t t, int share) { return (tiles(t) + cus - 1) / cus * share; };
-    const int64_t cost64 = cost(64, exact ? 12 : 14), cost128 = cost(128, exact ? 29 : 35);
-    // (a single block of K leaves nothing to pipeline)
-    if (g.k <= kBlock || (cost64 <= cost128 && cost64 <= cost(256, 100)))
-        launch_tiles<64, 64, 32, 32, 4>(g, cus, stream);
-    else if (cost128 <= cost(256, 100))
-        launch_tiles<128, 128, 64, 64, 2>(g, cus, stream);
-    else
-        launch_tiles<256, 256, 128, 64, 2>(g, cus, stream);
+    const int side = tile_side(g, cus), parts = workspace ? split_parts(g, cus) : 1;
+    if (parts > 1) {
+        if (bytes < static_cast<size_t>(split_bytes(g, parts))) return invalid("fp8: workspace too small");
+        MatmulArgs part = g;
+        part.c = workspace;
+        part.ldc = split_pitch(g);
+        part.c_dtype = MUON_TRAIN_F32;
+        launch_tiles<64, 64, 32, 32, 4>(part, exact, parts, cus, stream);
+        const int64_t quads = g.m * (split_pitch(g) / 4);
+        join_kernel<<<static_cast<uint32_t>((quads + 255) / 256), 256, 0, stream>>>(g, workspace, split_pitch(g), parts);
+    } else if (side == 64) {
+        launch_tiles<64, 64, 32, 32, 4>(g, exact, 1, cus, stream);
+    } else if (side == 128) {
+        launch_tiles<128, 128, 64, 64, 2>(g, exact, 1, cus, stream);
+    } else {
+        launch_tiles<256, 256, 128, 64, 2>(g, exact, 1, cus, stream);
+    }
     return launched("fp8_matmul");
+}
+
+}  // namespace
+}  // namespace muon_train
+
+extern "C" int muon_train_fp8_matmul(const muon_train_fp8_matmul_args *args, hipStream_t stream) {
+    if (!args) return invalid("fp8: args is null");
+    return matmul(*args, nullptr, 0, stream);
+}
+
+extern "C" int muon_train_fp8_matmul_workspace(const muon_train_fp8_matmul_args *args, size_t *bytes) {
+    if (!args || !bytes) return invalid("fp8: args is null");
+    *bytes = 0;
+    const int st = check(*args);
+    if (st != MUON_POLAR_OK || args->m == 0 || args->n == 0) return st;
+    const int cus = compute_units();
+    if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "fp8: no device");
+    *bytes = static_cast<size_t>(split_bytes(*args, split_parts(*args, cus)));
+    return MUON_POLAR_OK;
+}
+
+extern "C" int muon_train_fp8_matmul_in(const muon_train_fp8_matmul_args *args, void *workspace,
+                                        size_t workspace_bytes, hipStream_t stream) {
+    if (!args) return invalid("fp8: args is null");
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return invalid("fp8: workspace must be 16-byte aligned");
+    return matmul(*args, static_cast<float *>(workspace), workspace_bytes, stream);
 }
 
 extern "C" int muon_train_fp8_decode(const muon_train_fp8_decode_args *args, hipStream_t stream) {

@@ -375,3 +375,22 @@ def test_missing_tensors_are_named():
                            (lambda: train.fp8_linear(_cuda(2, 8), 3.0), "weight")):
             with pytest.raises(TypeError, match=name):
                 call()
+
+
+def test_matmul_workspace_entry():
+    lib = capi.load()
+    good = dict(values=1 << 20, scales=1 << 22, ld=256, scale_row=1, scale_col=4, block_rows=1)
+    args = MatmulArgs(m=4, n=8, k=256, c=1 << 24, ldc=8, a=Operand(**good), b=Operand(**good))
+    size = ctypes.c_size_t(7)
+    assert lib.muon_train_fp8_matmul_workspace(None, ctypes.byref(size)) == capi.ERR_INVALID_ARGUMENT
+    assert lib.muon_train_fp8_matmul_workspace(ctypes.byref(args), None) == capi.ERR_INVALID_ARGUMENT
+    assert lib.muon_train_fp8_matmul_in(None, None, ctypes.c_size_t(0), None) == capi.ERR_INVALID_ARGUMENT
+    odd = ctypes.c_void_p((1 << 26) + 8)
+    assert lib.muon_train_fp8_matmul_in(ctypes.byref(args), odd, ctypes.c_size_t(64), None) == capi.ERR_INVALID_ARGUMENT
+    assert "aligned" in capi.last_error()
+    args.m = -1
+    assert lib.muon_train_fp8_matmul_workspace(ctypes.byref(args), ctypes.byref(size)) == capi.ERR_INVALID_ARGUMENT
+    assert size.value == 0
+    args.m = 0
+    assert lib.muon_train_fp8_matmul_workspace(ctypes.byref(args), ctypes.byref(size)) == capi.OK and size.value == 0
+    assert lib.muon_train_fp8_matmul_in(ctypes.byref(args), None, ctypes.c_size_t(0), None) == capi.OK

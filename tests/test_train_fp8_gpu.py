@@ -147,6 +147,42 @@ def test_workgroups_of_several_tiles(m, n, k):
         assert torch.equal(mf.train.fp8_matmul(qa, qb, B16), want)
 
 
+@pytest.mark.parametrize("m,n,k", [(17, 64, 2700), (32, 1000, 5000), (64, 4096, 4096), (65, 129, 128 * 23),
+                                   (100, 1, 4000), (130, 2050, 2560)])
+@pytest.mark.parametrize("b_rows", [1, 128])
+@pytest.mark.parametrize("dtype", [F32, B16], ids=str)
+def test_split_products(m, n, k, b_rows, dtype):
+    """Few tiles of a long K: the parts of K meet in the parts' order."""
+    gen = torch.Generator().manual_seed(m + n + k)
+    a, b = spread(gen, m, k, F32), randn(gen, n, k)
+    want = value(a, 1).cuda() @ value(b, b_rows).cuda().t()
+    qa, qb = mf.train.quantize_fp8(a.cuda()), mf.train.quantize_fp8(b.cuda(), b_rows)
+    got = mf.train.fp8_matmul(qa, qb, dtype)
+    check(got, want, F32_SUM)
+    assert torch.equal(got, mf.train.fp8_matmul(qa, qb, dtype))
+
+
+def test_split_product_of_a_nan_row_and_in_a_graph():
+    gen = torch.Generator().manual_seed(8)
+    a, b = randn(gen, 40, 5000), randn(gen, 300, 5000)
+    qb = mf.train.quantize_fp8(b.cuda(), 128)
+    clean = mf.train.fp8_matmul(mf.train.quantize_fp8(a.cuda()), qb)
+    a[7, 4990] = math.nan
+    x = a.cuda()
+    qa = mf.train.quantize_fp8(x)
+    got = mf.train.fp8_matmul(qa, qb)
+    rows = [i for i in range(40) if i != 7]
+    assert got[7].isnan().all() and torch.equal(got[rows], clean[rows])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = mf.train.fp8_matmul(mf.train.quantize_fp8(x), qb)
+    for step in range(4):
+        x.copy_(randn(gen, 40, 5000))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, mf.train.fp8_matmul(mf.train.quantize_fp8(x), qb)), step
+
+
 def test_each_block_has_its_scale():
     """One element of a in each block of 128, scales that are powers of two of their place:
     the product of one block with ones, exactly."""
