@@ -490,7 +490,12 @@ at::Tensor Fp8Linear(const at::Tensor &x, const at::Tensor &values, const at::Te
     Held held{values, scales};
     const muon_train_fp8_operand w = operand(held, x);
     TORCH_CHECK(blocks(cols) * kBlock == values.size(1), "fp8: operands of different width");
-    if (rows <= 16 && w.block_rows == kBlock) {  // quantised in the product's own kernel
+    // Up to 16 rows can be quantised in the product's own kernel.  Each workgroup then does that
+    // work, four rows and 4096 columns a pass of some 1 us; a launch of its own takes 3 us.
+    // (12 rows of 4096 columns, three passes: 2.4 us over the product of held rows; 16, four
+    // passes: 3.5; one row of 14336 2.7, five rows 7.6, 16 rows 17.7.)  The bits are the same.
+    const int64_t passes = (rows + 3) / 4 * ((cols + 4095) / 4096);
+    if (rows <= 16 && passes < 4 && w.block_rows == kBlock) {
         muon_train_fp8_decode_args a{};
         const Rows r = as_rows(x);
         a.w = w;

@@ -338,3 +338,15 @@ def test_few_tokens(m, n, k, dtype):
     wide = torch.full((m, k + 3), 7.0, dtype=dtype, device="cuda")
     wide[:, 3:] = x.cuda()
     assert torch.equal(mf.train.fp8_linear(wide[:, 3:], q)[0], got[0])
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 300, 9000), (4, 40, 12288), (12, 8200, 4096), (13, 100, 4000), (5, 70, 4097)])
+@pytest.mark.parametrize("dtype", [F32, B16], ids=str)
+def test_few_tokens_of_long_rows(m, n, k, dtype):
+    """Both sides of the sizes up to which the product's own kernel quantises."""
+    gen = torch.Generator().manual_seed(m + n + k)
+    x, w = spread(gen, m, k, dtype), randn(gen, n, k)
+    q = mf.train.quantize_fp8(w.cuda(), 128)
+    got = mf.train.fp8_linear(x.cuda(), q)
+    check(got, value(x, 1) @ value(w, 128).t(), F32_SUM)
+    assert torch.equal(got, mf.train.fp8_matmul(mf.train.quantize_fp8(x.cuda()), q, dtype))
