@@ -148,6 +148,21 @@ def test_an_index_that_occurs_twice():
     run_all(s, tau=2.0, lam=0.5)
 
 
+@pytest.mark.parametrize("k", [15, 16, 17, 100, 1024])
+def test_indices_that_occur_often(k):
+    """Each of an element's entries counts, wherever they stand among the others."""
+    s = make(5, 3000, k, F32, labels=True, seed=k)
+    gen = torch.Generator().manual_seed(k)
+    s["index"][1:] = torch.randint(0, 6, (4, k), generator=gen).cuda() * 499
+    s["labels"][2] = 499
+    run_all(s, tau=2.0, lam=0.5)
+
+
+@pytest.mark.parametrize("v,dtype", [(98304, F32), (98311, F32), (140000, F32), (131080, B16), (160001, B16)], ids=str)
+def test_rows_in_registers_and_lds(v, dtype):
+    run_all(make(3, v, 40, dtype, labels=True), tau=1.5, lam=0.3)
+
+
 def test_masked_and_extreme_logits():
     s = make(8, 1003, 5, F32)
     s["z"][:, -3:] = -math.inf
