@@ -403,8 +403,14 @@ __global__ __launch_bounds__(64 * kFinishRuns) void norms_finish_kernel(Args a, 
 }
 
 // Threads and pieces of a row.  Forward: two pieces a thread from 512 columns on, up to 107
-// registers, 20 waves a compute unit.  Backward, which holds more: one piece as far as 1024
-// threads go.
+// registers, 20 waves a compute unit.  Backward, which holds more: two pieces and up to 256
+// registers, 8 waves a compute unit; in bf16 with values that rows share one piece, whose 128
+// registers also hold the next row's, 16 waves, as far as 512 threads go.  16384 rows: of 4096
+// in bf16 161 us with one piece, 169 with two; with an fp32 residual 284 with one (some spilled)
+// and 237 with two, all in fp32 365 and 308; of 5120 (1024 threads would spill more, three in
+// eight of them idle) in bf16 254 and 250, fp32 residual 506 and 299, all in fp32 658 and 383.
+// Past 8192 columns two pieces of 1024 threads have 128 registers and spill: 8192 rows of 16384
+// in bf16 809 us, 38 % of the copy rate.
 struct Shape {
     int nt, v;
 };
@@ -416,13 +422,18 @@ Shape forward_shape(int64_t d) {
     if (d <= 8192) return {512, 2};
     return {1024, 2};
 }
-Shape backward_shape(int64_t d) {
-    if (d <= 512) return {64, 1};
-    if (d <= 1024) return {128, 1};
-    if (d <= 2048) return {256, 1};
-    if (d <= 4096) return {512, 1};
-    if (d <= 8192) return {1024, 1};
-    return {1024, 2};
+bool general(const Args &a) {
+    return a.gate_kind == MUON_TRAIN_GATE_FULL || a.scale_kind == MUON_TRAIN_SCALE_VECTOR;
+}
+bool one_piece(const Args &a) {
+    return a.y_dtype == MUON_TRAIN_BF16 && a.residual_dtype == MUON_TRAIN_BF16 && !general(a);
+}
+Shape backward_shape(const Args &a) {
+    if (a.d <= 512) return {64, 1};
+    const bool one = a.d <= 4096 && one_piece(a);
+    for (int nt = 64; nt < 512; nt *= 2)
+        if (a.d <= 16 * nt) return one ? Shape{2 * nt, 1} : Shape{nt, 2};
+    return {a.d <= 8192 ? 512 : 1024, 2};
 }
 
 template <class F>
@@ -435,15 +446,23 @@ void with_forward_shape(Shape s, F &&f) {
     else if (s.nt == 512) f(integral_constant<int, 512>{}, integral_constant<int, 2>{});
     else f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
 }
-template <class F>
+template <bool kOnePiece, class F>
 void with_backward_shape(Shape s, F &&f) {
     using std::integral_constant;
-    if (s.nt == 64) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-    else if (s.nt == 128) f(integral_constant<int, 128>{}, integral_constant<int, 1>{});
-    else if (s.nt == 256) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
-    else if (s.nt == 512) f(integral_constant<int, 512>{}, integral_constant<int, 1>{});
-    else if (s.v == 1) f(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
-    else f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+    constexpr integral_constant<int, 1> one{};
+    constexpr integral_constant<int, 2> two{};
+    if (s.nt == 1024) return f(integral_constant<int, 1024>{}, two);
+    if (s.nt == 512 && s.v == 2) return f(integral_constant<int, 512>{}, two);
+    if (s.nt == 64 && s.v == 1) return f(integral_constant<int, 64>{}, one);
+    if constexpr (kOnePiece) {
+        if (s.nt == 128) f(integral_constant<int, 128>{}, one);
+        else if (s.nt == 256) f(integral_constant<int, 256>{}, one);
+        else f(integral_constant<int, 512>{}, one);
+    } else {
+        if (s.nt == 64) f(integral_constant<int, 64>{}, two);
+        else if (s.nt == 128) f(integral_constant<int, 128>{}, two);
+        else f(integral_constant<int, 256>{}, two);
+    }
 }
 template <class F>
 void with_types(const Args &a, F &&f) {
@@ -454,12 +473,12 @@ void with_types(const Args &a, F &&f) {
 }
 
 BackwardPlan backward_plan(const Args &a, int cus) {
-    const Shape s = backward_shape(a.d);
+    const Shape s = backward_shape(a);
     BackwardPlan p{};
     p.nt = s.nt;
     p.v = s.v;
-    // workgroups that the card holds at once, 16 waves a compute unit
-    const int64_t resident = int64_t(cus) * (1024 / s.nt);
+    // workgroups that the card holds at once: 16 waves a compute unit, 8 of two pieces
+    const int64_t resident = int64_t(cus) * (s.v == 1 || s.nt == 1024 ? 1024 / s.nt : 512 / s.nt);
     p.groups_per_sequence = 1;
     if (a.gate_kind == MUON_TRAIN_GATE_SEQUENCE && a.rows > 0) {
         const int64_t sequences = a.rows / a.rows_per_sequence;
@@ -585,16 +604,16 @@ extern "C" int muon_train_norms_backward(const muon_train_norms_args *args, void
     float *part = reinterpret_cast<float *>(part_scale + p.groups);
     if (a.rows > 0) {
         with_types(a, [&](auto ty, auto tr) {
-            with_backward_shape({p.nt, p.v}, [&](auto nt, auto v) {
-                const dim3 grid(static_cast<uint32_t>(p.groups));
-                constexpr int kNt = decltype(nt)::value, kV = decltype(v)::value;
-                if (a.gate_kind == MUON_TRAIN_GATE_FULL || a.scale_kind == MUON_TRAIN_SCALE_VECTOR)
-                    norms_backward_kernel<decltype(ty), decltype(tr), kNt, kV, true>
-                        <<<grid, p.nt, 0, stream>>>(a, p, part, part_scale);
-                else
-                    norms_backward_kernel<decltype(ty), decltype(tr), kNt, kV, false>
-                        <<<grid, p.nt, 0, stream>>>(a, p, part, part_scale);
-            });
+            auto go = [&](auto is_general) {
+                constexpr bool kGeneral = decltype(is_general)::value;
+                constexpr bool kOnePiece = std::is_same_v<decltype(ty), Bf16> && std::is_same_v<decltype(tr), Bf16> && !kGeneral;
+                with_backward_shape<kOnePiece>({p.nt, p.v}, [&](auto nt, auto v) {
+                    norms_backward_kernel<decltype(ty), decltype(tr), decltype(nt)::value, decltype(v)::value, kGeneral>
+                        <<<static_cast<uint32_t>(p.groups), p.nt, 0, stream>>>(a, p, part, part_scale);
+                });
+            };
+            if (general(a)) go(std::true_type{});
+            else go(std::false_type{});
         });
         st = launched("norms_backward");
         if (st != MUON_POLAR_OK) return st;
