@@ -176,27 +176,65 @@ __global__ __launch_bounds__(NT, V == 1 && !kGeneral ? 4 : 1) void norms_backwar
     }
 
     int col[V], valid[V];
-    float w1[V][8], w2[V][8], sum_post[V][8], sum_pre[V][8];
-    float sum_scale[kGeneral ? V : 1][8];
-    double scale_total = 0.0;  // a scalar scale's gradient: one sum over all elements, which cancel
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         col[v] = (v * NT + tid) * 8;
         valid[v] = clamp8(a.d - col[v]);
+    }
+    constexpr bool kWide = NT == 1024;  // sums in LDS, weights not held
+    float held1[kWide ? 1 : V][8], held2[kWide ? 1 : V][8], held_sum[2][kWide ? 1 : V][8];
+    __shared__ muon_polar::f32x4 lds_sum[kWide ? 4 * V * NT : 1];
+    float sum_scale[kGeneral ? V : 1][8];
+    // w1: post_weight times a gate that rows share; w2: pre_weight.
+    auto read_weights = [&](int v, float (&w1)[8], float (&w2)[8]) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            w1[v][i] = w2[v][i] = 1.0f;
-            sum_post[v][i] = sum_pre[v][i] = 0.0f;
-            if (kGeneral) sum_scale[v][i] = 0.0f;
-        }
-        if (a.post_weight) load8_any(a.post_weight, col[v], valid[v], a.weight_dtype, w1[v]);
-        if (a.pre_weight) load8_any(a.pre_weight, col[v], valid[v], a.weight_dtype, w2[v]);
+        for (int i = 0; i < 8; ++i) w1[i] = w2[i] = 1.0f;
+        if (a.post_weight) load8_any(a.post_weight, col[v], valid[v], a.weight_dtype, w1);
+        if (a.pre_weight) load8_any(a.pre_weight, col[v], valid[v], a.weight_dtype, w2);
         if (a.gate_kind == MUON_TRAIN_GATE_CHANNEL || seq_gate) {
             float g[8];
             load8_any(a.gate, sequence * a.d + col[v], valid[v], a.gate_dtype, g);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w1[v][i] *= g[i];
+            for (int i = 0; i < 8; ++i) w1[i] *= g[i];
         }
+    };
+    auto weights = [&](int v, float (&w1)[8], float (&w2)[8]) {
+        if constexpr (kWide) {
+            read_weights(v, w1, w2);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w1[i] = held1[v][i], w2[i] = held2[v][i];
+        }
+    };
+    auto get_sum = [&](int which, int v, float (&x)[8]) {
+        if constexpr (kWide) {
+            const muon_polar::f32x4 lo = lds_sum[(2 * (which * V + v)) * NT + tid], hi = lds_sum[(2 * (which * V + v) + 1) * NT + tid];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = lo[i], x[4 + i] = hi[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = held_sum[which][v][i];
+        }
+    };
+    auto put_sum = [&](int which, int v, const float (&x)[8]) {
+        if constexpr (kWide) {
+            lds_sum[(2 * (which * V + v)) * NT + tid] = muon_polar::f32x4{x[0], x[1], x[2], x[3]};
+            lds_sum[(2 * (which * V + v) + 1) * NT + tid] = muon_polar::f32x4{x[4], x[5], x[6], x[7]};
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) held_sum[which][v][i] = x[i];
+        }
+    };
+    double scale_total = 0.0;  // a scalar scale's gradient: one sum over all elements, which cancel
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const float zero[8] = {};
+        put_sum(kSumPost, v, zero);
+        put_sum(kSumPre, v, zero);
+        if (kGeneral)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum_scale[v][i] = 0.0f;
+        if constexpr (!kWide) read_weights(v, held1[v], held2[v]);
     }
     const bool has_dh = a.d_normed && a.pre_norm, has_dt = a.d_residual_out != nullptr;
     struct Row {
@@ -230,7 +268,9 @@ __global__ __launch_bounds__(NT, V == 1 && !kGeneral ? 4 : 1) void norms_backwar
         float dot = 0.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            float r[8], dh[8];
+            float r[8], dh[8], w1[8], w2[8], sum_pre[8];
+            weights(v, w1, w2);
+            get_sum(kSumPre, v, sum_pre);
             x.y[v].get(n[v]);
             x.r[v].get(r);
             x.h[v].get(dh);
@@ -243,20 +283,23 @@ __global__ __launch_bounds__(NT, V == 1 && !kGeneral ? 4 : 1) void norms_backwar
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 n[v][i] *= rho1;
-                float u = x.gate * (n[v][i] * w1[v][i]);
+                float u = x.gate * (n[v][i] * w1[i]);
                 if constexpr (kGeneral) u *= gate[v][i];
                 m[v][i] = fmaf(kGeneral ? sc[v][i] : number, r[i], u) * rho2;
-                dm[v][i] = dh[i] * w2[v][i];
+                dm[v][i] = dh[i] * w2[i];
                 dot = fmaf(dm[v][i], m[v][i], dot);
-                sum_pre[v][i] = fmaf(dh[i], m[v][i], sum_pre[v][i]);
+                sum_pre[i] = fmaf(dh[i], m[v][i], sum_pre[i]);
             }
+            put_sum(kSumPre, v, sum_pre);
         }
         const float mean2 = a.pre_norm && !single ? block.sum(dot) * inv_d : 0.0f;
         const float f2 = !a.pre_norm ? 0.0f : single ? rho2 * eps * rho2 * rho2 : rho2;
         float row_dot = 0.0f, row_scale = 0.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            float r[8], dt[8], out[8], dgate[8];
+            float r[8], dt[8], out[8], dgate[8], w1[8], w2[8], sum_post[8];
+            weights(v, w1, w2);
+            get_sum(kSumPost, v, sum_post);
             x.r[v].get(r);
             x.t[v].get(dt);
 #pragma unroll
@@ -265,17 +308,18 @@ __global__ __launch_bounds__(NT, V == 1 && !kGeneral ? 4 : 1) void norms_backwar
                 out[i] = (kGeneral ? sc[v][i] : number) * d_total;
                 row_scale = fmaf(d_total, r[i], row_scale);
                 const float with_n = d_total * n[v][i];
-                dm[v][i] = d_total * w1[v][i];  // dn from here on, but for the token's gate
+                dm[v][i] = d_total * w1[i];  // dn from here on, but for the token's gate
                 float weighed = with_n * x.gate;
                 if constexpr (kGeneral) {
                     sum_scale[v][i] = fmaf(d_total, r[i], sum_scale[v][i]);
-                    dgate[i] = with_n * w1[v][i];
+                    dgate[i] = with_n * w1[i];
                     weighed *= gate[v][i];
                     dm[v][i] *= gate[v][i];
                 }
-                sum_post[v][i] += weighed;
+                sum_post[i] += weighed;
                 row_dot = fmaf(dm[v][i], n[v][i], row_dot);
             }
+            put_sum(kSumPost, v, sum_post);
             Piece<TR> o;
             o.set(out);
             o.store(static_cast<RawR *>(a.d_residual) + row * a.d + col[v], valid[v]);
@@ -300,8 +344,11 @@ __global__ __launch_bounds__(NT, V == 1 && !kGeneral ? 4 : 1) void norms_backwar
     float *mine = part + int64_t(blockIdx.x) * plan.sums * a.d;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        store8_any(mine, kSumPost * a.d + col[v], valid[v], MUON_TRAIN_F32, sum_post[v]);
-        store8_any(mine, kSumPre * a.d + col[v], valid[v], MUON_TRAIN_F32, sum_pre[v]);
+        float sum[8];
+        get_sum(kSumPost, v, sum);
+        store8_any(mine, kSumPost * a.d + col[v], valid[v], MUON_TRAIN_F32, sum);
+        get_sum(kSumPre, v, sum);
+        store8_any(mine, kSumPre * a.d + col[v], valid[v], MUON_TRAIN_F32, sum);
         if constexpr (kGeneral)
             if (plan.sums > kSumScale)
                 store8_any(mine, kSumScale * a.d + col[v], valid[v], MUON_TRAIN_F32, sum_scale[v]);
@@ -409,8 +456,10 @@ __global__ __launch_bounds__(64 * kFinishRuns) void norms_finish_kernel(Args a, 
 // in bf16 161 us with one piece, 169 with two; with an fp32 residual 284 with one (some spilled)
 // and 237 with two, all in fp32 365 and 308; of 5120 (1024 threads would spill more, three in
 // eight of them idle) in bf16 254 and 250, fp32 residual 506 and 299, all in fp32 658 and 383.
-// Past 8192 columns two pieces of 1024 threads have 128 registers and spill: 8192 rows of 16384
-// in bf16 809 us, 38 % of the copy rate.
+// Past 8192 columns two pieces of 1024 threads have 128 registers: their column sums lie in LDS
+// and the weights are read anew for each row (8192 rows of 16384 in bf16 413 us, 75 % of the
+// copy rate, in fp32 659, 94 %; with all of it held, 330 registers spilled, 809 and 1395; a gate
+// of y's shape still spills 100, 939 us and 44 %).
 struct Shape {
     int nt, v;
 };
