@@ -108,6 +108,14 @@ def test_many_sequences_and_rows(gate):
     run_both(*make((1, 5000, 200), F32, F32, gate=gate, scale="vector"))
 
 
+@pytest.mark.parametrize("gate,scale", [("full", "number"), ("token", "vector"), ("sequence", "scalar")])
+@pytest.mark.parametrize("ty,tr", [(B16, B16), (F32, F32)], ids=str)
+@pytest.mark.parametrize("shape", [(2, 300, 1500), (2, 290, 3001), (1, 270, 5120), (2, 140, 9000)], ids=str)
+def test_gates_of_wide_rows(shape, ty, tr, gate, scale):
+    """Each number of threads and pieces of a row, several rows a workgroup."""
+    run_both(*make(shape, ty, tr, gate=gate, scale=scale))
+
+
 def test_gate_over_several_axes():
     run_both(*make((2, 3, 4, 96), F32, F32, gate="sequence"))
     run_both(*make((11, 96), F32, F32, gate="token"))
