@@ -90,8 +90,8 @@ int muon_train_norms_backward(const muon_train_norms_args *args, void *workspace
  *     grad = g·[(1 − λ)·τ·(softmax(z / τ) − p) + λ·(softmax(z) − onehot(label))]
  *
  * with λ = label_weight.  A row whose entries are all absent or −inf has no first term, a
- * row whose label is outside [0, vocab) no second.  An index that occurs twice counts
- * twice.  `grad` may be `logits` itself (same address and row length); otherwise the two
+ * row whose label is outside [0, vocab) no second, whatever its logits are.  An index that
+ * occurs twice counts twice.  `grad` may be `logits` itself (same address and row length); otherwise the two
  * must not overlap. */
 typedef struct muon_train_distill_args {
     int64_t rows, vocab, k; /* k: 1 to 1024 */
@@ -105,7 +105,8 @@ typedef struct muon_train_distill_args {
     int logits_dtype, teacher_dtype, index_bytes; /* index_bytes: 4 or 8 */
     float *loss;  /* [rows] */
     float *stats; /* [rows, 4]: max z, 1 / Σ exp((z − max) / τ), 1 / Σ exp(z − max) (labels),
-                     1 / Σ exp((t − max t) / τ) (0 without entries) */
+                     1 / Σ exp((t − max t) / τ) (0 without entries); 1 / Σ is NaN of a
+                     row that is all −inf */
     void *grad;   /* [rows, vocab], logits' dtype */
 } muon_train_distill_args;
 

@@ -213,13 +213,21 @@ __device__ __forceinline__ void take(Running<kHard> &run, C *x, float c) {
     }
 }
 
-// What the gradient needs of a row: softmax(z / τ) times f_soft plus softmax(z) times f_hard.
+// 1 / a sum of exponentials; of a row that is all −inf, whose softmax is 0 / 0, NaN.
+__device__ __forceinline__ float inverse_sum(float sum) {
+    return sum == 0.0f ? __builtin_nanf("") : 1.0f / sum;
+}
+// What the gradient needs of a row: softmax(z / τ) times f_soft plus softmax(z) times f_hard,
+// 0 for a term that the row does not have.  Logits that are NaN, +inf or all −inf make that
+// factor NaN where the term counts; the exponentials themselves are held to [0, 1], with 0 for
+// NaN (a modifier of the instruction: no time), so that where it does not they add nothing.
 template <bool kHard>
 struct Slope {
     float z_max, c, f_soft, f_hard;
+    __device__ __forceinline__ static float within(float x) { return __builtin_amdgcn_fmed3f(x, 0.0f, 1.0f); }
     __device__ __forceinline__ float operator()(float x) const {
-        float d = f_soft * exp2_hw((x - z_max) * c);
-        if constexpr (kHard) d = fmaf(f_hard, exp2_hw((x - z_max) * kLog2e), d);
+        float d = f_soft * within(exp2_hw((x - z_max) * c));
+        if constexpr (kHard) d = fmaf(f_hard, within(exp2_hw((x - z_max) * kLog2e)), d);
         return d;
     }
 };
@@ -282,8 +290,8 @@ __device__ __forceinline__ void write_row(const Args &a, int64_t row, float kl, 
     a.loss[row] = loss;
     if (a.stats) {
         a.stats[4 * row] = z_max;
-        a.stats[4 * row + 1] = 1.0f / z_sum;
-        a.stats[4 * row + 2] = kHard ? 1.0f / z_hard : 0.0f;
+        a.stats[4 * row + 1] = inverse_sum(z_sum);
+        a.stats[4 * row + 2] = kHard ? inverse_sum(z_hard) : 0.0f;
         a.stats[4 * row + 3] = t_sum != 0.0f ? 1.0f / t_sum : 0.0f;
     }
 }
@@ -398,8 +406,8 @@ __global__ __launch_bounds__(NT, 4) void distill_both_kernel(Args a) {
     const bool taught = sum[1] != 0.0f;
     const float g = a.grad_loss ? a.grad_loss[row] : float(a.grad_value);
     const float soft = taught ? (1.0f - lam) * tau : 0.0f;
-    const Slope<kHard> slope{top[0], c, g * soft * (1.0f / sum[0]),
-                             kHard && y.label >= 0 ? g * lam * (1.0f / sum[2]) : 0.0f};
+    const Slope<kHard> slope{top[0], c, taught ? g * soft * inverse_sum(sum[0]) : 0.0f,
+                             kHard && y.label >= 0 ? g * lam * inverse_sum(sum[2]) : 0.0f};
     Raw *out = static_cast<Raw *>(a.grad) + row * a.ld_grad;
     over_chunks<NT, R, E>(0, vocab, [&](int r, int base, uint32_t own, int valid) {
         float f[E];
@@ -462,7 +470,7 @@ __global__ __launch_bounds__(kGradThreads) void distill_grad_kernel(Args a, int 
     const bool taught = inv_teacher != 0.0f;
     const float g = a.grad_loss ? a.grad_loss[row] : float(a.grad_value);
     const float soft = taught ? (1.0f - lam) * tau : 0.0f;
-    const Slope<kHard> slope{a.stats[4 * row], c, g * soft * a.stats[4 * row + 1],
+    const Slope<kHard> slope{a.stats[4 * row], c, taught ? g * soft * a.stats[4 * row + 1] : 0.0f,
                              kHard && y.label >= 0 ? g * lam * a.stats[4 * row + 2] : 0.0f};
     for (int at = lo; at < hi; at += kStep) {
         C now[kAhead];

@@ -288,3 +288,31 @@ def test_gradient_against_differences():
     slope = (g.double() * way.double()).sum()
     diff = (total(s["z"] + h * way) - total(s["z"] - h * way)) / (2 * h)
     assert abs(diff - slope) <= 1e-3 * abs(slope)
+
+
+@pytest.mark.parametrize("dtype", [F32, B16], ids=str)
+@pytest.mark.parametrize("v", [777, 20011, 200003])
+def test_rows_without_a_term_have_none_of_its_gradient(v, dtype):
+    """A term that a row does not have adds nothing to its gradient, whatever its logits are:
+    without the first none of softmax(z / tau), without the second none of softmax(z)."""
+    s = make(10, v, 6, dtype, labels=True)
+    s["labels"][:] = 3
+    s["index"][:7] = -1  # no entries
+    s["labels"][:4] = -100  # nor a label
+    for row, value in enumerate((-math.inf, math.nan, math.inf)):
+        s["z"][row, 5 if row else slice(None)] = value
+        s["z"][row + 4, 5 if row else slice(None)] = value  # with a label: its term follows the formula
+    s["index"][7] = torch.arange(6)  # entries without weight, no label
+    s["teacher"][7] = -math.inf
+    s["z"][7] = -math.inf
+    s["labels"][7:9] = -100  # row 8: only the first term
+    loss, grad = run_all(s, tau=1.5, lam=0.4)
+    for row in (0, 1, 2, 3, 7):
+        assert loss[row] == 0 and not grad[row].any(), row
+    for row in (4, 5):
+        assert grad[row].isnan().all(), row
+    assert grad[8:].isfinite().all()
+    bare = dict(s, labels=None)
+    _, grad = run_all(bare, tau=1.5)
+    for row in range(8):
+        assert not grad[row].any(), row
