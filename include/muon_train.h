@@ -101,7 +101,7 @@ typedef struct muon_train_distill_args {
     const void *teacher_indices; /* [rows, k], int32 or int64 */
     const int64_t *labels;      /* [rows], or null: no second term */
     const float *grad_loss;     /* [rows], or null: grad_value for every row */
-    double temperature, label_weight, grad_value;
+    double temperature, label_weight, grad_value; /* temperature: normal in fp32, below 1e30 */
     int logits_dtype, teacher_dtype, index_bytes; /* index_bytes: 4 or 8 */
     float *loss;  /* [rows] */
     float *stats; /* [rows, 4]: max z, 1 / Σ exp((z − max) / τ), 1 / Σ exp(z − max) (labels),

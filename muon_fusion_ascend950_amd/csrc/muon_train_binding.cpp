@@ -17,6 +17,8 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
+#include <cfloat>
+
 #include "muon_train.h"
 
 namespace {
@@ -786,8 +788,9 @@ bool check_distill(const at::Tensor &logits, const at::Tensor &teacher_logits,
                       teacher_logits.sizes(), " and ", teacher_indices.sizes());
     const int64_t k = teacher_logits.size(-1);
     TORCH_CHECK_VALUE(k >= 1 && k <= kMaxTop, "K must be 1 to ", kMaxTop, ", got ", k);
-    TORCH_CHECK_VALUE(temperature > 0.0 && temperature < 1e30,
-                      "temperature must be positive, got ", temperature);
+    TORCH_CHECK_VALUE(temperature >= double(FLT_MIN) && temperature < 1e30,
+                      "temperature must be a positive normal float32 number below 1e30, got ",
+                      temperature);
     TORCH_CHECK_VALUE(label_weight >= 0.0 && label_weight <= 1.0,
                       "label_weight must be 0 to 1, got ", label_weight);
     if (!given(labels)) {

@@ -14,6 +14,8 @@
 // bits from every entry of an index that occurs twice).
 #include "train_common.hpp"
 
+#include <cfloat>
+
 namespace muon_train {
 
 namespace {
@@ -501,8 +503,9 @@ int check(const Args *a) {
         return invalid("distill: dtypes must be float32 or bfloat16");
     if (a->index_bytes != 4 && a->index_bytes != 8)
         return invalid("distill: indices must be int32 or int64");
-    if (!(a->temperature > 0.0) || !(a->temperature < 1e30))
-        return invalid("distill: temperature must be positive");
+    // log2(e) / temperature has to be finite in fp32
+    if (!(a->temperature >= double(FLT_MIN)) || !(a->temperature < 1e30))
+        return invalid("distill: temperature must be a positive normal fp32 number below 1e30");
     if (!(a->label_weight >= 0.0 && a->label_weight <= 1.0))
         return invalid("distill: label_weight must be 0 to 1");
     if (a->rows == 0) return MUON_POLAR_OK;

@@ -86,7 +86,8 @@ def distill_topk(logits: torch.Tensor, teacher_logits: torch.Tensor,
 
     logits ``[..., V]``, teacher_logits ``[..., K]`` (K at most 1024) float32 or bfloat16;
     teacher_indices ``[..., K]`` int32 or int64; labels ``[...]`` int64.  Returns float32
-    ``[...]``, differentiable with respect to ``logits``.
+    ``[...]``, differentiable with respect to ``logits``.  temperature: at least float32's
+    smallest normal number, below 1e30.
 
     An entry whose index is outside ``[0, V)`` is absent (rows with fewer than K entries are
     filled with -1), and an absent entry's logit is not looked at.  A row without entries,

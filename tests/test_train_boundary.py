@@ -394,3 +394,20 @@ def test_matmul_workspace_entry():
     args.m = 0
     assert lib.muon_train_fp8_matmul_workspace(ctypes.byref(args), ctypes.byref(size)) == capi.OK and size.value == 0
     assert lib.muon_train_fp8_matmul_in(ctypes.byref(args), None, ctypes.c_size_t(0), None) == capi.OK
+
+
+@pytest.mark.parametrize("temperature", [1e-39, 1e-46, 5e-324, 1e30])
+def test_distill_refuses_temperatures_that_float32_does_not_hold(temperature):
+    """1 / temperature has to be finite in float32."""
+    with FakeTensorMode():
+        for call in (train.distill_topk, train.distill_topk_with_grad):
+            args, kw = _distill_ok(temperature=temperature)
+            with pytest.raises(ValueError, match="temperature"):
+                call(*args, **kw)
+        args, kw = _distill_ok(temperature=1.2e-38)
+        train.distill_topk(*args, **kw)
+    args = DistillArgs(rows=4, vocab=10, k=3, ld_logits=10, ld_grad=10, logits=1 << 20,
+                       teacher_logits=1 << 21, teacher_indices=1 << 22, temperature=temperature,
+                       index_bytes=4, loss=1 << 23)
+    assert capi.load().muon_train_distill_forward(ctypes.byref(args), None) == capi.ERR_INVALID_ARGUMENT
+    assert "temperature" in capi.last_error()
