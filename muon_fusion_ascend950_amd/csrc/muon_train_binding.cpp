@@ -631,6 +631,15 @@ constexpr at::ScalarType kFp8[] = {at::kFloat8_e4m3fn};
 bool wants_grad(const at::Tensor &t) { return t.requires_grad(); }
 bool wants_grad(const OptTensor &t) { return given(t) && t->requires_grad(); }
 OptTensor maybe(const at::Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+// No operator has a derivative in forward mode: a tangent that reaches one is refused here, or
+// it would be lost with the result none the wiser (an operator that is called without a
+// reverse-mode gradient leaves autograd behind).  Level 0 is the only one there is.
+bool has_tangent(const at::Tensor &t) { return t.defined() && t._fw_grad(0).defined(); }
+bool has_tangent(const OptTensor &t) { return t.has_value() && has_tangent(*t); }
+template <class... T>
+void refuse_tangents(const char *what, const T &...t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(t) || ...), what, ": no derivative in forward mode");
+}
 // Gradients that have none of their own: in a pass that keeps its graph, asking them for one
 // is an error.
 variable_list only_once(variable_list grads, const char *what) {
@@ -694,6 +703,7 @@ struct BlockNormsFunction : torch::autograd::Function<BlockNormsFunction> {
         variable_list result(13);
         const bool pre_norm = ctx->saved_data["choices"].toIntVector()[3];
         if (!grads[0].defined() && !(grads[1].defined() && pre_norm)) return result;
+        refuse_tangents("block_norms", grads[0], grads[1]);
         const auto t = ctx->get_saved_variables();
         const auto numbers = ctx->saved_data["numbers"].toDoubleVector();
         const auto choices = ctx->saved_data["choices"].toIntVector();
@@ -751,6 +761,7 @@ std::tuple<at::Tensor, at::Tensor> BlockNorms(const at::Tensor &y, const at::Ten
                           scale->sizes());
     }
     TORCH_CHECK_VALUE(eps >= 0.0, "eps must not be negative, got ", eps);
+    refuse_tangents("block_norms", y, residual, post_weight, gate, scale, pre_weight);
     int64_t wanted = 0;
     if (at::GradMode::is_enabled())
         wanted = int64_t(wants_grad(post_weight)) | wants_grad(gate) << 1 | wants_grad(scale) << 2 |
@@ -817,6 +828,7 @@ struct DistillFunction : torch::autograd::Function<DistillFunction> {
         return loss;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        refuse_tangents("distill_topk", grads[0]);
         const at::AutoDispatchBelowADInplaceOrView below;
         const auto t = ctx->get_saved_variables();
         const auto numbers = ctx->saved_data["numbers"].toDoubleVector();
@@ -832,6 +844,7 @@ at::Tensor DistillTopk(const at::Tensor &logits, const at::Tensor &teacher_logit
                        double temperature, double label_weight) {
     const bool hard = check_distill(logits, teacher_logits, teacher_indices, labels, temperature,
                                     label_weight);
+    refuse_tangents("distill_topk", logits, teacher_logits);
     const OptTensor used = hard ? labels : OptTensor();
     if (at::GradMode::is_enabled() && wants_grad(logits))
         return DistillFunction::apply(logits, teacher_logits.detach(), teacher_indices, used,
@@ -854,6 +867,7 @@ std::tuple<at::Tensor, at::Tensor> DistillTopkWithGrad(
         TORCH_CHECK_VALUE(grad_loss->sizes() == lead, "grad_loss must have shape ", lead, ", got ",
                           grad_loss->sizes());
     }
+    refuse_tangents("distill_topk_with_grad", logits, teacher_logits, grad_loss, out);
     const at::NoGradGuard no_grad;
     at::Tensor grad;
     if (given(out)) {
@@ -887,6 +901,7 @@ struct Fp8LinearFunction : torch::autograd::Function<Fp8LinearFunction> {
         return y;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        refuse_tangents("fp8_linear", grads[0]);
         const at::AutoDispatchBelowADInplaceOrView below;
         const auto t = ctx->get_saved_variables();
         const auto choices = ctx->saved_data["choices"].toIntVector();
@@ -907,6 +922,7 @@ at::Tensor Fp8LinearTrain(const at::Tensor &x, const at::Tensor &weight) {
     TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(1) == x.size(-1),
                       "weight must have shape [N, ", x.size(-1), "], got ", weight.sizes());
     TORCH_CHECK_VALUE(weight.numel() > 0, "weight's dimensions must be positive");
+    refuse_tangents("fp8_linear", x, weight);
     if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight)))
         return Fp8LinearFunction::apply(x, weight,
                                         int64_t(wants_grad(x)) | wants_grad(weight) << 1);
@@ -922,6 +938,7 @@ at::Tensor Fp8LinearServe(const at::Tensor &x, const at::Tensor &values, const a
     TORCH_CHECK_VALUE(cols == x.size(-1), "x must have ", cols, " columns, got shape ", x.sizes());
     TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && wants_grad(x)),
                       "a quantised weight has no gradient: pass the float32 or bfloat16 one");
+    refuse_tangents("fp8_linear", x, scales);
     return MUON_TRAIN_OP("fp8_linear", Fp8Linear).call(x, values, scales);
 }
 

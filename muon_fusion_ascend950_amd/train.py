@@ -9,7 +9,8 @@
 ``muon_update`` starts from the gradients of a model's matrices; these are pieces of the
 forward and backward pass that produce them.  All take ROCm GPU tensors of float32 or
 bfloat16, run on torch's current stream, compute in float32 and round each result once;
-gradients come through autograd.  No reference counterpart: the reference leaves the
+gradients come through autograd, in reverse mode once (a gradient of a gradient and
+forward-mode tangents are refused).  No reference counterpart: the reference leaves the
 training step to its caller (README.md:130).
 """
 
@@ -200,7 +201,8 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> Fp8Blocks:
         scale = max(amax(|block|) * (1 / 448), 2**-126)
         values = (block * (1 / scale)).to(float8_e4m3fn)
 
-    A block that holds an infinity or a NaN has none but NaN back.
+    A block that holds an infinity or a NaN has none but NaN back.  No gradient: ``x`` is
+    taken detached.
     """
     _check_tensor("x", x)
     if x.ndim != 2 or x.shape[1] < 1:

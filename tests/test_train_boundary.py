@@ -411,3 +411,46 @@ def test_distill_refuses_temperatures_that_float32_does_not_hold(temperature):
                        index_bytes=4, loss=1 << 23)
     assert capi.load().muon_train_distill_forward(ctypes.byref(args), None) == capi.ERR_INVALID_ARGUMENT
     assert "temperature" in capi.last_error()
+
+
+# ------------------------------------------------------------------------ forward mode
+def _forward_mode_calls():
+    """Each public call on one differentiable operand, by name."""
+    def index():
+        return _cuda(4, 3, dtype=torch.int64)
+
+    return {
+        "norms y": lambda x: train.block_norms(x, _cuda(4, 64))[0],
+        "norms residual": lambda x: train.block_norms(_cuda(4, 64), x)[0],
+        "norms gate": lambda x: train.block_norms(_cuda(4, 64), _cuda(4, 64), gate=x)[0],
+        "norms weight": lambda x: train.block_norms(_cuda(4, 64), _cuda(4, 64), post_weight=x[0])[0],
+        "norms scale": lambda x: train.block_norms(_cuda(4, 64), _cuda(4, 64), residual_scale=x[0])[0],
+        "distill logits": lambda x: train.distill_topk(x, _cuda(4, 3), index()),
+        "distill teacher": lambda x: train.distill_topk(_cuda(4, 64), x[:, :3], index()),
+        "with_grad logits": lambda x: train.distill_topk_with_grad(x, _cuda(4, 3), index())[1],
+        "with_grad weight": lambda x: train.distill_topk_with_grad(
+            _cuda(4, 64), _cuda(4, 3), index(), grad_loss=x[:, 0])[1],
+        "linear x": lambda x: train.fp8_linear(x, _cuda(8, 64)),
+        "linear weight": lambda x: train.fp8_linear(_cuda(5, 64), x),
+        "serving x": lambda x: train.fp8_linear(x, train.quantize_fp8(_cuda(8, 64), 128)),
+    }
+
+
+@pytest.mark.parametrize("name", _forward_mode_calls())
+def test_forward_mode_is_refused(name):
+    """No operator has a forward-mode derivative; a tangent is refused, never dropped."""
+    import torch.autograd.forward_ad as fwd
+
+    call = _forward_mode_calls()[name]
+    with FakeTensorMode():
+        with fwd.dual_level():
+            x = fwd.make_dual(_cuda(4, 64), _cuda(4, 64))
+            with pytest.raises(NotImplementedError, match="forward"):
+                call(x)
+            call(_cuda(4, 64))  # without a tangent nothing is refused
+        x, t = _cuda(4, 64), _cuda(4, 64)
+        with pytest.raises(NotImplementedError, match="forward"):
+            torch.func.jvp(call, (x,), (t,))
+        if "with_grad" not in name:  # writes into a tensor: no vmap
+            with pytest.raises(NotImplementedError, match="forward"):
+                torch.func.jvp(torch.vmap(call), (_cuda(2, 4, 64),), (_cuda(2, 4, 64),))

@@ -67,3 +67,20 @@ def test_gradients_have_none_of_their_own():
         assert torch.equal(plain, kept)
         with pytest.raises(RuntimeError, match="no gradient of its own"):
             kept.sum().backward()
+
+
+def test_a_gradient_has_no_forward_mode_derivative():
+    """Differentiating a backward pass in forward mode is refused, not answered with zeros."""
+    import torch.autograd.forward_ad as fwd
+
+    gen = torch.Generator().manual_seed(2)
+    x = torch.randn(20, 160, generator=gen).cuda().requires_grad_(True)
+    w = torch.randn(130, 160, generator=gen).cuda()
+    teacher = torch.randn(20, 3, generator=gen).cuda()
+    index = torch.randint(0, 130, (20, 3), generator=gen).cuda()
+    for out in (train.block_norms(x, x)[1], train.fp8_linear(x, w), train.distill_topk(x, teacher, index)):
+        with fwd.dual_level():
+            grad = fwd.make_dual(torch.ones_like(out), torch.ones_like(out))
+            with pytest.raises(NotImplementedError, match="forward"):
+                torch.autograd.grad(out, x, grad, retain_graph=True)
+        torch.autograd.grad(out, x, torch.ones_like(out))
