@@ -95,12 +95,15 @@ struct Norms {
                         "block_norms: post_weight and pre_weight must have one dtype");
         }
         a.gate_kind = static_cast<int>(gate_kind);
-        a.rows_per_sequence = rows_per_sequence;
+        // sequences of no tokens: no rows, whatever number of gate vectors
+        const bool no_tokens = gate_kind == MUON_TRAIN_GATE_SEQUENCE && rows_per_sequence == 0 && a.rows == 0;
+        a.rows_per_sequence = no_tokens ? 1 : rows_per_sequence;
         if (gate_kind != MUON_TRAIN_GATE_NONE) {
             TORCH_CHECK(given(gate_), "block_norms: gate is missing");
-            TORCH_CHECK(gate_kind != MUON_TRAIN_GATE_SEQUENCE || rows_per_sequence > 0,
+            TORCH_CHECK(gate_kind != MUON_TRAIN_GATE_SEQUENCE || a.rows_per_sequence > 0,
                         "block_norms: rows_per_sequence must be positive");
             const int64_t numel = gate_kind == MUON_TRAIN_GATE_CHANNEL ? a.d
+                                  : no_tokens                          ? gate_->numel()
                                   : gate_kind == MUON_TRAIN_GATE_SEQUENCE
                                       ? a.rows / rows_per_sequence * a.d
                                   : gate_kind == MUON_TRAIN_GATE_TOKEN ? a.rows
@@ -179,6 +182,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
     };
     at::Tensor d_post = grad(n.post, 1), d_gate = grad(n.gate, 2), d_scale = grad(n.scale, 4),
                d_pre = grad(n.pre, 8);
+    if (n.a.rows == 0 && d_gate.numel() > 0) d_gate.zero_();  // of sequences without tokens
     n.a.d_y = dy.data_ptr();
     n.a.d_residual = dr.data_ptr();
     if ((wanted & 1) && n.post.defined()) n.a.d_post_weight = d_post.data_ptr();

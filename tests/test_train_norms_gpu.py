@@ -269,3 +269,18 @@ def test_captured_in_a_graph():
             graph.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(held, call(new)))
+
+
+@pytest.mark.parametrize("shape", [(3, 0, 40), (2, 5, 0, 40), (0, 4, 40)], ids=str)
+def test_sequences_without_tokens(shape):
+    """A gate vector for each sequence of none: nothing comes out, its gradient is zero."""
+    y, r = (torch.empty(shape, device="cuda", requires_grad=True) for _ in range(2))
+    gate = torch.ones(shape[0], *(1 for _ in shape[1:-1]), 40, device="cuda", requires_grad=True)
+    weight = torch.ones(40, device="cuda", requires_grad=True)
+    with torch.no_grad():
+        out, h = mf.train.block_norms(y, r, gate=gate, post_weight=weight)
+    assert out.shape == h.shape == shape
+    out, h = mf.train.block_norms(y, r, gate=gate, post_weight=weight)
+    (out.sum() + h.sum()).backward()
+    for t in (y, r, gate, weight):
+        assert t.grad.shape == t.shape and not t.grad.any()
