@@ -21,13 +21,27 @@ using muon_polar::u32x4;
 inline int invalid(const char *msg) {
     return muon_polar::report(MUON_POLAR_ERR_INVALID_ARGUMENT, msg);
 }
-inline int launched(const char *what) {
-    const hipError_t e = hipGetLastError();
-    if (e == hipSuccess) return MUON_POLAR_OK;
-    char msg[256];
-    snprintf(msg, sizeof msg, "%s: %s", what, hipGetErrorString(e));
-    return muon_polar::report(MUON_POLAR_ERR_HIP, msg);
-}
+// The launches of one call.  Each gives its own status: hipGetLastError would also give an
+// error that some earlier HIP call of the thread left behind.
+struct Launches {
+    hipStream_t stream;
+    hipError_t status = hipSuccess;
+    template <class... P, class... A>
+    void operator()(void (*kernel)(P...), dim3 grid, int threads, const A &...a) {
+        if (status != hipSuccess) return;
+        auto launch = [&](P... p) {
+            void *args[] = {const_cast<void *>(static_cast<const void *>(&p))...};
+            status = hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, dim3(threads), args, 0, stream);
+        };
+        launch(a...);
+    }
+    int result(const char *what) const {
+        if (status == hipSuccess) return MUON_POLAR_OK;
+        char msg[256];
+        snprintf(msg, sizeof msg, "%s: %s", what, hipGetErrorString(status));
+        return muon_polar::report(MUON_POLAR_ERR_HIP, msg);
+    }
+};
 
 // Whether two buffers meet (a null one meets none).
 inline bool meet(const void *a, int64_t a_bytes, const void *b, int64_t b_bytes) {

@@ -540,21 +540,21 @@ int64_t row_chunks(const Args &a) {
 }
 
 template <class T, bool kHard>
-void launch_loss(const Args &a, int cus, hipStream_t stream) {
+void launch_loss(const Args &a, int cus, Launches &launch) {
     const dim3 grid(static_cast<uint32_t>(a.rows));
     const int nt = row_threads(a, row_chunks<T>(a), cus);
-    if (nt == 256) distill_loss_kernel<T, 256, kHard><<<grid, nt, 0, stream>>>(a);
-    else if (nt == 512) distill_loss_kernel<T, 512, kHard><<<grid, nt, 0, stream>>>(a);
-    else distill_loss_kernel<T, 1024, kHard><<<grid, nt, 0, stream>>>(a);
+    if (nt == 256) launch(distill_loss_kernel<T, 256, kHard>, grid, nt, a);
+    else if (nt == 512) launch(distill_loss_kernel<T, 512, kHard>, grid, nt, a);
+    else launch(distill_loss_kernel<T, 1024, kHard>, grid, nt, a);
 }
 template <class T, bool kHard>
-void launch_both(const Args &a, int cus, hipStream_t stream) {
+void launch_both(const Args &a, int cus, Launches &launch) {
     const int64_t chunks = row_chunks<T>(a);
     const int nt = row_threads(a, chunks, cus);
     const dim3 grid(static_cast<uint32_t>(a.rows));
     auto go = [&](auto threads, auto r, auto l) {
-        distill_both_kernel<T, decltype(threads)::value, decltype(r)::value, decltype(l)::value, kHard>
-            <<<grid, nt, 0, stream>>>(a);
+        launch(distill_both_kernel<T, decltype(threads)::value, decltype(r)::value, decltype(l)::value, kHard>,
+               grid, nt, a);
     };
     constexpr integral_constant<int, 0> none{};
     if (nt == 256 && chunks <= 256 * 4) go(integral_constant<int, 256>{}, integral_constant<int, 4>{}, none);
@@ -568,7 +568,7 @@ void launch_both(const Args &a, int cus, hipStream_t stream) {
 // Gradient alone: rows are cut where there are too few to fill the card, into parts of 16
 // KiB at least.
 template <class T, bool kHard>
-void launch_grad(const Args &a, int cus, hipStream_t stream) {
+void launch_grad(const Args &a, int cus, Launches &launch) {
     const int64_t least = 16384 / int64_t(sizeof(typename T::Raw));
     int64_t parts = (8 * int64_t(cus) + a.rows - 1) / a.rows;
     const int64_t most = (a.vocab + least - 1) / least;
@@ -576,15 +576,15 @@ void launch_grad(const Args &a, int cus, hipStream_t stream) {
     int64_t width = (a.vocab + parts - 1) / parts;
     width = (width + 7) / 8 * 8;  // parts begin where 16-byte chunks do
     const dim3 grid(static_cast<uint32_t>(a.rows), static_cast<uint32_t>((a.vocab + width - 1) / width));
-    distill_grad_kernel<T, kHard><<<grid, kGradThreads, 0, stream>>>(a, static_cast<int>(width));
+    launch(distill_grad_kernel<T, kHard>, grid, kGradThreads, a, static_cast<int>(width));
 }
 #define MUON_TRAIN_LAUNCH(which)                                                              \
     do {                                                                                      \
         const bool hard = args->labels != nullptr;                                            \
         if (args->logits_dtype == MUON_TRAIN_BF16)                                            \
-            hard ? which<Bf16, true>(*args, cus, stream) : which<Bf16, false>(*args, cus, stream); \
+            hard ? which<Bf16, true>(*args, cus, launch) : which<Bf16, false>(*args, cus, launch); \
         else                                                                                  \
-            hard ? which<F32, true>(*args, cus, stream) : which<F32, false>(*args, cus, stream);   \
+            hard ? which<F32, true>(*args, cus, launch) : which<F32, false>(*args, cus, launch);   \
     } while (0)
 
 }  // namespace
@@ -599,11 +599,12 @@ extern "C" int muon_train_distill_forward(const muon_train_distill_args *args, h
     if (!args->loss) return invalid("distill: null output");
     const int cus = compute_units();
     if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "distill: no device");
+    Launches launch{stream};
     if (args->grad)
         MUON_TRAIN_LAUNCH(launch_both);
     else
         MUON_TRAIN_LAUNCH(launch_loss);
-    return launched("distill_forward");
+    return launch.result("distill_forward");
 }
 
 extern "C" int muon_train_distill_backward(const muon_train_distill_args *args, hipStream_t stream) {
@@ -612,6 +613,7 @@ extern "C" int muon_train_distill_backward(const muon_train_distill_args *args, 
     if (!args->grad || !args->stats) return invalid("distill: null output");
     const int cus = compute_units();
     if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "distill: no device");
+    Launches launch{stream};
     MUON_TRAIN_LAUNCH(launch_grad);
-    return launched("distill_backward");
+    return launch.result("distill_backward");
 }

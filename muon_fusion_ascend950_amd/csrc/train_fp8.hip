@@ -839,22 +839,22 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(DecodeArgs a) 
 // 32 columns a workgroup where that still fills the card (a lane's work on x then serves
 // twice the weight), else 16.
 template <class X>
-void launch_few_rows(const DecodeArgs &a, int cus, hipStream_t stream) {
+void launch_few_rows(const DecodeArgs &a, int cus, Launches &launch) {
     const bool exact = a.c_dtype == MUON_TRAIN_F32;
     const int threads = 64 * kFewWaves;
     if (a.n >= 32 * int64_t(cus)) {
         const dim3 grid(static_cast<uint32_t>((a.n + 31) / 32));
-        if (exact) few_rows_kernel<X, true, 2><<<grid, threads, 0, stream>>>(a);
-        else few_rows_kernel<X, false, 2><<<grid, threads, 0, stream>>>(a);
+        if (exact) launch(few_rows_kernel<X, true, 2>, grid, threads, a);
+        else launch(few_rows_kernel<X, false, 2>, grid, threads, a);
     } else {
         const dim3 grid(static_cast<uint32_t>((a.n + 15) / 16));
-        if (exact) few_rows_kernel<X, true, 1><<<grid, threads, 0, stream>>>(a);
-        else few_rows_kernel<X, false, 1><<<grid, threads, 0, stream>>>(a);
+        if (exact) launch(few_rows_kernel<X, true, 1>, grid, threads, a);
+        else launch(few_rows_kernel<X, false, 1>, grid, threads, a);
     }
 }
 
 template <int BM, int BN, int WM, int WN, int D>
-void launch_tiles(const MatmulArgs &g, bool exact, int parts, int cus, hipStream_t stream) {
+void launch_tiles(const MatmulArgs &g, bool exact, int parts, int cus, Launches &launch) {
     using Geo = Geometry<BM, BN, WM, WN, D>;
     const int tm = static_cast<int>((g.m + BM - 1) / BM), tn = static_cast<int>((g.n + BN - 1) / BN);
     const bool row_b = g.b.block_rows == 1;
@@ -863,8 +863,8 @@ void launch_tiles(const MatmulArgs &g, bool exact, int parts, int cus, hipStream
     const int64_t resident = int64_t(cus) * (160 * 1024 / (D * Geo::kSlot));
     const dim3 grid(static_cast<uint32_t>(Geo::kTwoSlots && !exact && !row_b && tiles > resident ? resident : tiles * parts));
     auto go = [&](auto e, auto r) {
-        matmul_kernel<BM, BN, WM, WN, D, decltype(e)::value, decltype(r)::value>
-            <<<grid, Geo::kThreads, 0, stream>>>(g, tm, tn, parts);
+        launch(matmul_kernel<BM, BN, WM, WN, D, decltype(e)::value, decltype(r)::value>, grid, Geo::kThreads,
+               g, tm, tn, parts);
     };
     using std::bool_constant;
     if (exact && row_b) go(bool_constant<true>{}, bool_constant<true>{});
@@ -922,21 +922,22 @@ extern "C" int muon_train_fp8_quantize(const muon_train_fp8_quantize_args *args,
         meet(a.values, v_bytes, a.values_t, t_bytes))
         return invalid("fp8: x and values must not overlap");
     const int t = static_cast<int>(tc);
+    Launches launch{stream};
     if (a.block_rows == 1 && !a.values_t && tr * tc < 512) {
         const dim3 few(static_cast<uint32_t>((a.rows + 15) / 16 * tc));
-        if (a.x_dtype == MUON_TRAIN_BF16) quantize_rows_kernel<Bf16><<<few, kQuantThreads, 0, stream>>>(a, t);
-        else quantize_rows_kernel<F32><<<few, kQuantThreads, 0, stream>>>(a, t);
-        return launched("fp8_quantize");
+        if (a.x_dtype == MUON_TRAIN_BF16) launch(quantize_rows_kernel<Bf16>, few, kQuantThreads, a, t);
+        else launch(quantize_rows_kernel<F32>, few, kQuantThreads, a, t);
+        return launch.result("fp8_quantize");
     }
     const dim3 grid(static_cast<uint32_t>(tr * tc));
     if (a.x_dtype == MUON_TRAIN_BF16) {
-        if (a.block_rows == 1) quantize_kernel<Bf16, 1><<<grid, kQuantThreads, 0, stream>>>(a, t);
-        else quantize_kernel<Bf16, kBlock><<<grid, kQuantThreads, 0, stream>>>(a, t);
+        if (a.block_rows == 1) launch(quantize_kernel<Bf16, 1>, grid, kQuantThreads, a, t);
+        else launch(quantize_kernel<Bf16, kBlock>, grid, kQuantThreads, a, t);
     } else {
-        if (a.block_rows == 1) quantize_kernel<F32, 1><<<grid, kQuantThreads, 0, stream>>>(a, t);
-        else quantize_kernel<F32, kBlock><<<grid, kQuantThreads, 0, stream>>>(a, t);
+        if (a.block_rows == 1) launch(quantize_kernel<F32, 1>, grid, kQuantThreads, a, t);
+        else launch(quantize_kernel<F32, kBlock>, grid, kQuantThreads, a, t);
     }
-    return launched("fp8_quantize");
+    return launch.result("fp8_quantize");
 }
 
 namespace muon_train {
@@ -1020,11 +1021,12 @@ int matmul(const MatmulArgs &g, float *workspace, size_t bytes, hipStream_t stre
     if (st != MUON_POLAR_OK || g.m == 0 || g.n == 0) return st;
     const int cus = compute_units();
     if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "fp8: no device");
+    Launches launch{stream};
     if (few_rows(g)) {
         const DecodeArgs d{g.n, g.a.ld, int(g.m), int(g.k), int(g.k / kBlock), g.a.values, g.a.scales,
                            g.a.scale_col, g.b, g.c, g.ldc, g.c_dtype};
-        launch_few_rows<Held>(d, cus, stream);
-        return launched("fp8_matmul");
+        launch_few_rows<Held>(d, cus, launch);
+        return launch.result("fp8_matmul");
     }
     if (tiles(g, 64) > INT32_MAX) return invalid("fp8: matrix too large");
     const bool exact = g.c_dtype == MUON_TRAIN_F32;
@@ -1035,17 +1037,17 @@ int matmul(const MatmulArgs &g, float *workspace, size_t bytes, hipStream_t stre
         part.c = workspace;
         part.ldc = split_pitch(g);
         part.c_dtype = MUON_TRAIN_F32;
-        launch_tiles<64, 64, 32, 32, 4>(part, exact, parts, cus, stream);
+        launch_tiles<64, 64, 32, 32, 4>(part, exact, parts, cus, launch);
         const int64_t quads = g.m * (split_pitch(g) / 4);
-        join_kernel<<<static_cast<uint32_t>((quads + 255) / 256), 256, 0, stream>>>(g, workspace, split_pitch(g), parts);
+        launch(join_kernel, dim3(static_cast<uint32_t>((quads + 255) / 256)), 256, g, workspace, split_pitch(g), parts);
     } else if (side == 64) {
-        launch_tiles<64, 64, 32, 32, 4>(g, exact, 1, cus, stream);
+        launch_tiles<64, 64, 32, 32, 4>(g, exact, 1, cus, launch);
     } else if (side == 128) {
-        launch_tiles<128, 128, 64, 64, 2>(g, exact, 1, cus, stream);
+        launch_tiles<128, 128, 64, 64, 2>(g, exact, 1, cus, launch);
     } else {
-        launch_tiles<256, 256, 128, 64, 2>(g, exact, 1, cus, stream);
+        launch_tiles<256, 256, 128, 64, 2>(g, exact, 1, cus, launch);
     }
-    return launched("fp8_matmul");
+    return launch.result("fp8_matmul");
 }
 
 }  // namespace
@@ -1098,7 +1100,8 @@ extern "C" int muon_train_fp8_decode(const muon_train_fp8_decode_args *args, hip
     if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "fp8: no device");
     const DecodeArgs d{g.n, g.ld_x, int(g.m), int(g.cols), int(blocks), g.x, nullptr, 0,
                        g.w, g.c, g.ldc, g.c_dtype};
-    if (g.x_dtype == MUON_TRAIN_BF16) launch_few_rows<Bf16>(d, cus, stream);
-    else launch_few_rows<F32>(d, cus, stream);
-    return launched("fp8_decode");
+    Launches launch{stream};
+    if (g.x_dtype == MUON_TRAIN_BF16) launch_few_rows<Bf16>(d, cus, launch);
+    else launch_few_rows<F32>(d, cus, launch);
+    return launch.result("fp8_decode");
 }

@@ -615,13 +615,14 @@ extern "C" int muon_train_norms_forward(const muon_train_norms_args *args, hipSt
     // as many workgroups as stay resident: each keeps its weights over its rows
     const int64_t resident = int64_t(cus) * (2048 / s.nt);
     const dim3 grid(static_cast<uint32_t>(a.rows < resident ? a.rows : resident));
+    Launches launch{stream};
     with_types(a, [&](auto ty, auto tr) {
         with_forward_shape(s, [&](auto nt, auto v) {
-            norms_forward_kernel<decltype(ty), decltype(tr), decltype(nt)::value, decltype(v)::value>
-                <<<grid, s.nt, 0, stream>>>(a);
+            launch(norms_forward_kernel<decltype(ty), decltype(tr), decltype(nt)::value, decltype(v)::value>,
+                   grid, s.nt, a);
         });
     });
-    return launched("norms_forward");
+    return launch.result("norms_forward");
 }
 
 extern "C" int muon_train_norms_workspace(const muon_train_norms_args *args, size_t *bytes) {
@@ -651,20 +652,21 @@ extern "C" int muon_train_norms_backward(const muon_train_norms_args *args, void
         return invalid("norms: workspace must be 8-byte aligned");
     double *part_scale = static_cast<double *>(workspace);
     float *part = reinterpret_cast<float *>(part_scale + p.groups);
+    Launches launch{stream};
     if (a.rows > 0) {
         with_types(a, [&](auto ty, auto tr) {
             auto go = [&](auto is_general) {
                 constexpr bool kGeneral = decltype(is_general)::value;
                 constexpr bool kOnePiece = std::is_same_v<decltype(ty), Bf16> && std::is_same_v<decltype(tr), Bf16> && !kGeneral;
                 with_backward_shape<kOnePiece>({p.nt, p.v}, [&](auto nt, auto v) {
-                    norms_backward_kernel<decltype(ty), decltype(tr), decltype(nt)::value, decltype(v)::value, kGeneral>
-                        <<<static_cast<uint32_t>(p.groups), p.nt, 0, stream>>>(a, p, part, part_scale);
+                    launch(norms_backward_kernel<decltype(ty), decltype(tr), decltype(nt)::value, decltype(v)::value, kGeneral>,
+                           dim3(static_cast<uint32_t>(p.groups)), p.nt, a, p, part, part_scale);
                 });
             };
             if (general(a)) go(std::true_type{});
             else go(std::false_type{});
         });
-        st = launched("norms_backward");
+        st = launch.result("norms_backward");
         if (st != MUON_POLAR_OK) return st;
     }
     const bool scalar = a.scale_kind == MUON_TRAIN_SCALE_SCALAR && a.d_scale;
@@ -672,6 +674,6 @@ extern "C" int muon_train_norms_backward(const muon_train_norms_args *args, void
                                           a.gate_kind == MUON_TRAIN_GATE_SEQUENCE);
     if (!a.d_post_weight && !a.d_pre_weight && !a.d_scale && !shared_gate) return MUON_POLAR_OK;
     const dim3 grid(static_cast<uint32_t>((a.d + 63) / 64), p.sums + (scalar ? 1 : 0));
-    norms_finish_kernel<<<grid, 64 * kFinishRuns, 0, stream>>>(a, p, part, part_scale);
-    return launched("norms_finish");
+    launch(norms_finish_kernel, grid, 64 * kFinishRuns, a, p, part, part_scale);
+    return launch.result("norms_finish");
 }

@@ -84,3 +84,29 @@ def test_a_gradient_has_no_forward_mode_derivative():
             with pytest.raises(NotImplementedError, match="forward"):
                 torch.autograd.grad(out, x, grad, retain_graph=True)
         torch.autograd.grad(out, x, torch.ones_like(out))
+
+
+def test_an_error_of_an_earlier_call_is_not_the_operators():
+    """An error that another HIP call of this thread left behind is its caller's to read: the
+    operators report what became of their own launches."""
+    import ctypes
+
+    gen = torch.Generator().manual_seed(3)
+    x = torch.randn(40, 256, generator=gen).cuda()
+    w = torch.randn(300, 256, generator=gen).cuda()
+    teacher = torch.randn(40, 3, generator=gen).cuda()
+    index = torch.randint(0, 256, (40, 3), generator=gen).cuda()
+    weight = train.quantize_fp8(w, 128)
+    calls = [lambda: train.quantize_fp8(x), lambda: train.fp8_linear(x, weight), lambda: train.fp8_linear(x[:2], weight),
+             lambda: train.fp8_linear(x, w), lambda: train.block_norms(x, x),
+             lambda: train.distill_topk(x, teacher, index), lambda: train.distill_topk_with_grad(x, teacher, index)]
+    for call in calls:
+        call()
+    with open("/proc/self/maps") as maps:
+        hip = ctypes.CDLL(next(line.split()[-1] for line in maps if "libamdhip64.so" in line))
+    try:
+        for call in calls:
+            assert hip.hipSetDevice(1 << 20) != 0
+            call()
+    finally:
+        hip.hipGetLastError()
