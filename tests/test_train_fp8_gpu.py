@@ -350,3 +350,55 @@ def test_few_tokens_of_long_rows(m, n, k, dtype):
     got = mf.train.fp8_linear(x.cuda(), q)
     check(got, value(x, 1) @ value(w, 128).t(), F32_SUM)
     assert torch.equal(got, mf.train.fp8_matmul(mf.train.quantize_fp8(x.cuda()), q, dtype))
+
+
+def kernel_names(f):
+    """Names of the kernels that `f` launches, from a graph of them."""
+    import ctypes
+
+    class Params(ctypes.Structure):
+        _fields_ = [("block", ctypes.c_uint32 * 3), ("extra", ctypes.c_void_p), ("func", ctypes.c_void_p),
+                    ("grid", ctypes.c_uint32 * 3), ("params", ctypes.c_void_p), ("shared", ctypes.c_uint32)]
+
+    f()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        f()
+    with open("/proc/self/maps") as maps:
+        hip = ctypes.CDLL(next(line.split()[-1] for line in maps if "libamdhip64.so" in line))
+    hip.hipKernelNameRefByPtr.restype = ctypes.c_char_p
+    handle, count = ctypes.c_void_p(graph.raw_cuda_graph()), ctypes.c_size_t(0)
+    assert hip.hipGraphGetNodes(handle, None, ctypes.byref(count)) == 0
+    nodes = (ctypes.c_void_p * count.value)()
+    assert hip.hipGraphGetNodes(handle, nodes, ctypes.byref(count)) == 0
+    names = []
+    for node in nodes:
+        p = Params()
+        assert hip.hipGraphKernelNodeGetParams(ctypes.c_void_p(node), ctypes.byref(p)) == 0
+        names.append(hip.hipKernelNameRefByPtr(ctypes.c_void_p(p.func), None).decode())
+    return names
+
+
+TILED = [(2000, 4000, 640, 128), (4100, 4610, 256, 128), (4500, 4700, 512, 256), (4608, 4608, 256, 256)]
+TILED_F32 = [(2000, 4000, 640, 128), (4000, 4090, 384, 256), (4096, 4096, 256, 256)]
+
+
+@pytest.mark.parametrize("m,n,k,side,dtype", [(*s, B16) for s in TILED] + [(*s, F32) for s in TILED_F32], ids=str)
+@pytest.mark.parametrize("b_rows", [1, 128])
+def test_scales_of_large_tiles(m, n, k, side, dtype, b_rows):
+    """Ones and zeros of both signs, scales that are powers of two drawn for each row, column
+    block and block of K: whole and ragged tiles, several a workgroup, two steps and more.  Every
+    sum is a multiple of 2^-4 below 2^15: exact in fp32, rounded once to bf16."""
+    gen = torch.Generator().manual_seed(m + k + b_rows)
+    blocks, nb = -(-k // 128), n if b_rows == 1 else -(-n // 128)
+    a = torch.randint(-1, 2, (m, k), generator=gen).float()
+    b = torch.randint(-1, 2, (n, k), generator=gen).float()
+    sa = torch.exp2(torch.randint(-2, 3, (m, blocks), generator=gen).float())
+    sb = torch.exp2(torch.randint(-2, 3, (nb, blocks), generator=gen).float())
+    qa = mf.train.Fp8Blocks(a.to(F8).cuda(), sa.cuda())
+    qb = mf.train.Fp8Blocks(b.to(F8).cuda(), sb.cuda())
+    want = (qa.dequantize().double() @ qb.dequantize().double().t()).to(dtype)
+    names = kernel_names(lambda: mf.train.fp8_matmul(qa, qb, dtype))
+    assert any(f"matmul_kernelILi{side}ELi{side}E" in name for name in names), names
+    for _ in range(2):
+        assert torch.equal(mf.train.fp8_matmul(qa, qb, dtype), want)
