@@ -68,9 +68,7 @@ struct Chunk {
         }
     }
     __device__ __forceinline__ void store(typename T::Raw *p, int valid) const {
-        if (valid >= kElems) {
-            __builtin_memcpy(p, &v, 16);
-        } else {
+        if (valid < kElems) {
 #pragma unroll
             for (int i = 0; i < kElems; ++i)
                 if (i < valid) {
@@ -79,6 +77,8 @@ struct Chunk {
                     else
                         p[i] = __uint_as_float(v[i]);
                 }
+        } else {
+            __builtin_memcpy(p, &v, 16);
         }
     }
 };
