@@ -142,7 +142,8 @@ typedef struct muon_train_fp8_quantize_args {
 int muon_train_fp8_quantize(const muon_train_fp8_quantize_args *args, hipStream_t stream);
 
 /* c[m][n] = Σ_blocks a_scale·b_scale·Σ_{k in block} a[m][k]·b[n][k], both operands with k
- * running along their rows: products of values and their sums in fp32, rounded once. */
+ * running along their rows: products of values and their sums in fp32, rounded once.  a_scale
+ * times b_scale may leave fp32's range where the result does not. */
 typedef struct muon_train_fp8_operand {
     const void *values; /* [rows, k], 16-byte aligned */
     const float *scales;

@@ -202,9 +202,35 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(QuantArgs 
 // -------------------------------------------------------------------------- products
 // v_mfma_f32_16x16x128_f8f6f4 on e4m3 values: lane l supplies 32 consecutive values (k-part
 // l / 16 of the 128) of row l % 16 of A and of column l % 16 of B, and receives
-// D[4·(l / 16) + j][l % 16], j = 0 .. 3.
-__device__ __forceinline__ f32x4 mfma_fp8(i32x8 a, i32x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+// D[4·(l / 16) + j][l % 16], j = 0 .. 3.  Each row's values count times 2^(e − 127) of its lane's
+// exponent e, 0 to 254, which is byte kB of eb for b.
+template <int kB = 0>
+__device__ __forceinline__ f32x4 mfma_fp8(i32x8 a, uint32_t ea, i32x8 b, uint32_t eb) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0,
+                                                            static_cast<int>(ea), kB, static_cast<int>(eb));
+}
+
+// The product of two scales may leave fp32's range where the result does not: large ones at
+// blocks whose values meet zeros would be infinity times 0, small ones would lose the sums they
+// multiply.  Such scales are taken apart, s = mantissa·2^(exponent − 127): the exponents go into
+// the MFMA, whose sums then have their results' size, and the mantissas' product onto those.  The
+// bits are the ones that one factor gives where it is in range.  Exponents are kept within
+// 2^±100, the rest left to the mantissa: zeros, infinities, NaN and subnormal scales pass through
+// it, and values times 2^(exponent − 127) are normal numbers in bf16 too.
+struct Apart {
+    uint32_t exponent;
+    float mantissa;
+};
+__device__ __forceinline__ Apart apart(float s) {
+    const float within = __builtin_amdgcn_fmed3f(__builtin_fabsf(s), 0x1p-100f, 0x1p100f);
+    const uint32_t e = __float_as_uint(within) >> 23;
+    return {e, __builtin_amdgcn_ldexpf(s, 127 - static_cast<int>(e))};
+}
+// Scales whose products with each other stay in range whatever pairs meet: 2^-63 to 2^63, by
+// their bits.  Any other (a negative one too) has its step take them apart.
+constexpr uint32_t kNearLow = (127u - 63) << 23, kNearHigh = (127u + 63) << 23;
+__device__ __forceinline__ bool far(float s) {
+    return __float_as_uint(s) - kNearLow > kNearHigh - kNearLow;
 }
 
 using MatmulArgs = muon_train_fp8_matmul_args;
@@ -216,29 +242,35 @@ using MatmulArgs = muon_train_fp8_matmul_args;
 // values, which bf16 holds exactly: 1e-7, at half the rate.
 using bf16x2 = __bf16 __attribute__((ext_vector_type(2)));
 using muon_polar::bf16x8;
-__device__ __forceinline__ bf16x8 to_bf16(uint32_t lo, uint32_t hi) {
-    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
-    const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
-    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
-    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+__device__ __forceinline__ bf16x8 to_bf16(uint32_t lo, uint32_t hi, float power) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, power, false);
+    const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, power, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, power, false);
+    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, power, true);
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
-// 16 rows of 128 K-values of an operand as a lane holds them.
+// 16 rows of 128 K-values of an operand as a lane holds them, times 2^(e − 127) of its row's
+// exponent: `exponent` is e as the instruction at hand takes it, kNone that of 1.
 template <bool kExact>
 struct Frag {
     i32x8 v;
-    __device__ __forceinline__ void set(i32x8 x) { v = x; }
+    uint32_t e;
+    static constexpr uint32_t kNone = 127;
+    __device__ __forceinline__ static uint32_t exponent(uint32_t e) { return e; }
+    __device__ __forceinline__ void set(i32x8 x, uint32_t exponent) { v = x, e = exponent; }
 };
 template <>
 struct Frag<true> {
     bf16x8 v[4];
-    __device__ __forceinline__ void set(i32x8 x) {
+    static constexpr uint32_t kNone = 127u << 23;
+    __device__ __forceinline__ static uint32_t exponent(uint32_t e) { return e << 23; }
+    __device__ __forceinline__ void set(i32x8 x, uint32_t exponent) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = to_bf16(x[2 * i], x[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) v[i] = to_bf16(x[2 * i], x[2 * i + 1], __uint_as_float(exponent));
     }
 };
 __device__ __forceinline__ f32x4 multiply(const Frag<false> &a, const Frag<false> &b) {
-    return mfma_fp8(a.v, b.v, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+    return mfma_fp8(a.v, a.e, b.v, b.e);
 }
 __device__ __forceinline__ f32x4 multiply(const Frag<true> &a, const Frag<true> &b) {
     f32x4 t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -285,6 +317,58 @@ __device__ __forceinline__ void wait_dma_barrier(int behind) {
                  : "s"(behind), "n"(kLate)
                  : "memory", "scc");
 }
+
+// Of a pipelined step's scales, a's blocks' f and b's sb: if one of them is far, mantissas in their
+// place and the exponents, one a byte; otherwise exponents of 127, which change nothing.  What
+// apart() does, in one statement: where 8192 x 14336 x 4096 took 389 us with products of scales it
+// took 407 with a branch of the program's own, and where it took 434, 440 with this one.
+#define MUON_TRAIN_APART(scale, into)                    \
+    "v_max_f32 " into ", |" scale "|, %[low]\n\t"        \
+    "v_min_f32 " into ", %[high], " into "\n\t"          \
+    "v_lshrrev_b32 " into ", 23, " into "\n\t"           \
+    "v_sub_u32 %[t], 0x7f, " into "\n\t"                 \
+    "v_ldexp_f32 " scale ", " scale ", %[t]\n\t"
+#define MUON_TRAIN_APART4(f0, f1, f2, f3, exponents)                                           \
+    MUON_TRAIN_APART(f0, exponents)                                                           \
+    MUON_TRAIN_APART(f1, "%[eb]") "v_lshl_or_b32 " exponents ", %[eb], 8, " exponents "\n\t"  \
+    MUON_TRAIN_APART(f2, "%[eb]") "v_lshl_or_b32 " exponents ", %[eb], 16, " exponents "\n\t" \
+    MUON_TRAIN_APART(f3, "%[eb]") "v_lshl_or_b32 " exponents ", %[eb], 24, " exponents "\n\t"
+// The two wait states at the end are for an MFMA that reads the exponents next.
+#define MUON_TRAIN_APART_END MUON_TRAIN_APART("%[sb]", "%[eb]") ".Lnear%=:\n\ts_nop 1"
+__device__ __forceinline__ void take_scales_apart(int any_far, float (&f)[8], float &sb, uint32_t (&ea)[2],
+                                                  uint32_t &eb) {
+    uint32_t t;
+    asm volatile("v_mov_b32 %[ea0], 0x7f7f7f7f\n\t"
+                 "v_mov_b32 %[ea1], 0x7f7f7f7f\n\t"
+                 "v_mov_b32 %[eb], 0x7f\n\t"
+                 "s_cmp_eq_u32 %[far], 0\n\t"
+                 "s_cbranch_scc1 .Lnear%=\n\t"
+                 MUON_TRAIN_APART4("%[f0]", "%[f1]", "%[f2]", "%[f3]", "%[ea0]")
+                 MUON_TRAIN_APART4("%[f4]", "%[f5]", "%[f6]", "%[f7]", "%[ea1]")
+                 MUON_TRAIN_APART_END
+                 : [ea0] "=&v"(ea[0]), [ea1] "=&v"(ea[1]), [eb] "=&v"(eb), [t] "=&v"(t), [f0] "+v"(f[0]),
+                   [f1] "+v"(f[1]), [f2] "+v"(f[2]), [f3] "+v"(f[3]), [f4] "+v"(f[4]), [f5] "+v"(f[5]),
+                   [f6] "+v"(f[6]), [f7] "+v"(f[7]), [sb] "+v"(sb)
+                 : [far] "s"(__builtin_amdgcn_readfirstlane(any_far)), [low] "s"(0x1p-100f), [high] "s"(0x1p100f)
+                 : "scc");
+}
+__device__ __forceinline__ void take_scales_apart(int any_far, float (&f)[4], float &sb, uint32_t (&ea)[1],
+                                                  uint32_t &eb) {
+    uint32_t t;
+    asm volatile("v_mov_b32 %[ea0], 0x7f7f7f7f\n\t"
+                 "v_mov_b32 %[eb], 0x7f\n\t"
+                 "s_cmp_eq_u32 %[far], 0\n\t"
+                 "s_cbranch_scc1 .Lnear%=\n\t"
+                 MUON_TRAIN_APART4("%[f0]", "%[f1]", "%[f2]", "%[f3]", "%[ea0]")
+                 MUON_TRAIN_APART_END
+                 : [ea0] "=&v"(ea[0]), [eb] "=&v"(eb), [t] "=&v"(t), [f0] "+v"(f[0]), [f1] "+v"(f[1]),
+                   [f2] "+v"(f[2]), [f3] "+v"(f[3]), [sb] "+v"(sb)
+                 : [far] "s"(__builtin_amdgcn_readfirstlane(any_far)), [low] "s"(0x1p-100f), [high] "s"(0x1p100f)
+                 : "scc");
+}
+#undef MUON_TRAIN_APART
+#undef MUON_TRAIN_APART4
+#undef MUON_TRAIN_APART_END
 
 // Four consecutive results of a row, the first `count` of them inside the matrix.
 __device__ __forceinline__ void store4(void *c, int64_t at, int count, int dtype, f32x4 v) {
@@ -456,9 +540,7 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
     auto fragment = [&](const uint8_t *panel) {
         const i32x4 lo = *reinterpret_cast<const i32x4 *>(panel + lane_at);
         const i32x4 hi = *reinterpret_cast<const i32x4 *>(panel + (lane_at ^ 64));
-        Frag<kExact> f;
-        f.set(i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
-        return f;
+        return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     };
 
     f32x4 acc[SM][SN] = {};
@@ -541,9 +623,14 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
         // which the DMA was issued, for both.
         constexpr int kQ = SM * SN, kLag = 2, kBar = (SM - 2) * SN, kLast = (SM - 1) * SN;
         static_assert(D == 2 && SM % 4 == 0 && kQ % 4 == 0 && kLag < SN, "schedule");
-        Frag<false> fa[4], fb[SN];
+        i32x8 fa[4], fb[SN];
         f32x4 t[4];
-        float f[SM], sb = 0.0f, factor = 0.0f;  // a's scales, b's, their product for the block at hand
+        float f[SM], sb = 0.0f;  // a's scales and b's
+        // exponents, four blocks of a's to a register, and the scales' product for the block that
+        // is multiplied and the one that is added up
+        uint32_t ea[SM / 4], eb = 127;
+        float next_factor = 0.0f, factor = 0.0f;
+        int any_far = 0;
         auto base_of = [&](int s) { return smem + s * Geo::kSlot; };
         auto read_a = [&](const uint8_t *base, auto ic) {
             constexpr int i = decltype(ic)::value;
@@ -558,9 +645,18 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
             static_for<SM>([&](auto ic) { f[ic] = scale_m[16 * ic]; });
             sb = *(reinterpret_cast<const float *>(base + Geo::kPanels) + BM + wn);
         };
+        auto look = [&] {  // whether one of the scales at hand is far
+            uint32_t low = __float_as_uint(sb), high = low;
+            static_for<SM>([&](auto ic) {
+                const uint32_t bits = __float_as_uint(f[ic]);
+                low = bits < low ? bits : low;
+                high = umax(high, bits);
+            });
+            any_far = __builtin_amdgcn_ballot_w64(low < kNearLow || high > kNearHigh) != 0 ? 1 : 0;
+        };
         auto add = [&](auto qc) {
             constexpr int q = decltype(qc)::value, i = q / SN, j = q % SN;
-            if constexpr (j == 0) factor = f[i] * sb;
+            if constexpr (j == 0) factor = next_factor;
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(t[q % 4][e], factor, acc[i][j][e]);
         };
@@ -578,6 +674,7 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
         static_for<kLoads + 1>([&](auto d) { issue(d, 1, 1); });
         muon_polar::wait_vm_barrier<kLoads + 1>();
         read_scales(base_of(0));
+        look();
         static_for<3>([&](auto ic) { read_a(base_of(0), ic); });
         static_for<SN>([&](auto jc) { read_b(base_of(0), jc); });
         clear();
@@ -590,14 +687,17 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
                 const int from = phase == 0 ? 2 : 0, to = phase == 0 ? steps : 2;
                 for (int ahead = from; ahead < to; ++ahead, slot ^= 1) {
                     const uint8_t *base = base_of(slot), *after = base_of(slot ^ 1);
+                    take_scales_apart(any_far, f, sb, ea, eb);
                     static_for<kQ>([&](auto qc) {
                         constexpr int q = decltype(qc)::value, i = q / SN, j = q % SN;
                         if constexpr (q == kBar) {
                             wait_dma_barrier<2 * SM>(stored);
                             stored = 0;
                         }
-                        t[q % 4] = multiply(fb[j], fa[i % 4]);
+                        if constexpr (j == 0) next_factor = f[i] * sb;
+                        t[q % 4] = mfma_fp8<i % 4>(fb[j], eb, fa[i % 4], ea[i / 4]);
                         __builtin_amdgcn_sched_barrier(0);
+                        if constexpr (q == kQ - 1) look();
                         // that of kLag before, at first the last step's
                         add(std::integral_constant<int, (q + kQ - kLag) % kQ>{});
                         if constexpr (j == 0 && i + 3 < SM)
@@ -608,7 +708,7 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
                             if constexpr (q == kLast) read_a(after, std::integral_constant<int, 2>{});
                             if constexpr (q >= kLast) read_b(after, std::integral_constant<int, j>{});
                             // the last block's factor is formed: the scales give way
-                            if constexpr (q == kLast + kLag) read_scales(after);
+                            if constexpr (q == kLast) read_scales(after);
                             // kLoads + 1 DMA instructions over the 2·SN MFMAs
                             static_for<kLoads + 1>([&](auto dc) {
                                 constexpr int d = decltype(dc)::value;
@@ -633,28 +733,71 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
         int slot = 0;
         for (int k = first; k < steps; ++k) {
             muon_polar::wait_vm_barrier<(D - 2) * (kLoads + 1)>();
+            using Operand = Frag<kExact>;
             const int next = slot == 0 ? D - 1 : slot - 1;  // the slot that step k - 1 left
             const uint8_t *base = smem + slot * Geo::kSlot;
             const float *scale_m = reinterpret_cast<const float *>(base + Geo::kPanels) + wm + r;
             const float *scale_n = reinterpret_cast<const float *>(base + Geo::kPanels) + BM + wn;
-            Frag<kExact> fb[SN];
+            // Scales are taken apart in every step, or (kLook) only where one of the wave's rows has a
+            // far one.  With a scale a row on both sides that is 16 mantissas a lane of b's: 8192 x
+            // 14336 x 8192 978 us with products of scales, 1166 with all apart, 1017 looking first;
+            // 64 x 64 tiles, whose steps are short, lose more by looking (32 x 4096 x 14336 15.0 us,
+            // 15.4, 18.5).  fp32 results have no registers left for a's exponents beside the rest.
+            constexpr bool kLook = kRowB && Geo::kTwoSlots, kLookA = kLook && !kExact;
+            uint32_t ea[SM], eb[SN];
+            float sm[SM], sb = 1.0f;
             f32x4 sn[SN];
+            if constexpr (kLookA)
 #pragma unroll
-            for (int j = 0; j < SN; ++j) {
-                fb[j] = fragment(base + (BM + wn + 16 * j) * kBlock);
-                if constexpr (kRowB) sn[j] = *reinterpret_cast<const f32x4 *>(scale_n + 16 * j + 4 * part);
+                for (int i = 0; i < SM; ++i) ea[i] = Operand::kNone, sm[i] = scale_m[16 * i];
+            if constexpr (kRowB)
+#pragma unroll
+                for (int j = 0; j < SN; ++j) {
+                    eb[j] = Operand::kNone;
+                    sn[j] = *reinterpret_cast<const f32x4 *>(scale_n + 16 * j + 4 * part);
+                }
+            bool any_far = !kLook || far(scale_n[lane % WN]);
+            if constexpr (kLookA)
+#pragma unroll
+                for (int m = 0; m < WM; m += 64) any_far |= far(scale_m[(m + lane) % WM - r]);
+            if (!kLook || __builtin_amdgcn_ballot_w64(any_far)) {
+                if constexpr (kLookA)
+#pragma unroll
+                    for (int i = 0; i < SM; ++i) {
+                        const Apart p = apart(sm[i]);
+                        ea[i] = Operand::exponent(p.exponent), sm[i] = p.mantissa;
+                    }
+#pragma unroll
+                for (int j = 0; j < SN; ++j) {
+                    // kRowB: of the row of b that a lane supplies the exponent, of the four that it
+                    // receives the mantissas
+                    const Apart p = apart(scale_n[kRowB ? 16 * j + r : 0]);
+                    eb[j] = Operand::exponent(p.exponent);
+                    if constexpr (kRowB)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sn[j][e] = apart(sn[j][e]).mantissa;
+                    else
+                        sb = p.mantissa;
+                }
             }
-            const float sb = kRowB ? 1.0f : scale_n[0];
+            Operand fb[SN];
+#pragma unroll
+            for (int j = 0; j < SN; ++j) fb[j].set(fragment(base + (BM + wn + 16 * j) * kBlock), eb[j]);
 #pragma unroll
             for (int i = 0; i < SM; ++i) {
-                const Frag<kExact> fa = fragment(base + (wm + 16 * i) * kBlock);
-                const float sm = scale_m[16 * i] * sb;
+                Operand fa;
+                if constexpr (!kLookA) {
+                    const Apart p = apart(scale_m[16 * i]);
+                    ea[i] = Operand::exponent(p.exponent), sm[i] = p.mantissa;
+                }
+                fa.set(fragment(base + (wm + 16 * i) * kBlock), ea[i]);
+                const float f = kRowB ? sm[i] : sm[i] * sb;
 #pragma unroll
                 for (int j = 0; j < SN; ++j) {
                     const f32x4 t = multiply(fb[j], fa);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        acc[i][j][e] = fmaf(t[e], kRowB ? sm * sn[j][e] : sm, acc[i][j][e]);
+                        acc[i][j][e] = fmaf(t[e], kRowB ? f * sn[j][e] : f, acc[i][j][e]);
                 }
 #pragma unroll
                 for (int d = i * (kLoads + 1) / SM; d < (i + 1) * (kLoads + 1) / SM; ++d)
@@ -810,14 +953,16 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(DecodeArgs a) 
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (kb + u < end) {
+                const Apart x_scale = apart(sx[u]);
                 Frag<kExact> fx;
-                fx.set(whole(xlo[u], xhi[u]));
+                fx.set(whole(xlo[u], xhi[u]), Frag<kExact>::exponent(x_scale.exponent));
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
+                    const Apart w_scale = apart(sw[t][(kb + u) * a.w.scale_col]);
                     Frag<kExact> fw;
-                    fw.set(whole(lo[u][t], hi[u][t]));
+                    fw.set(whole(lo[u][t], hi[u][t]), Frag<kExact>::exponent(w_scale.exponent));
                     const f32x4 p = multiply(fw, fx);
-                    const float s = sx[u] * sw[t][(kb + u) * a.w.scale_col];
+                    const float s = x_scale.mantissa * w_scale.mantissa;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(p[e], s, acc[t][e]);
                 }

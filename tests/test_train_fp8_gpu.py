@@ -402,3 +402,70 @@ def test_scales_of_large_tiles(m, n, k, side, dtype, b_rows):
     assert any(f"matmul_kernelILi{side}ELi{side}E" in name for name in names), names
     for _ in range(2):
         assert torch.equal(mf.train.fp8_matmul(qa, qb, dtype), want)
+
+
+# few rows, 64 x 64 tiles, those split along K, 128 x 128 and 256 x 256
+FAR = [(3, 70, 384), (70, 90, 384), (32, 300, 5120), (2000, 4000, 384)]
+
+
+def far_scales(kind, m, n, k, b_rows, gen):
+    """Values and scales whose products s_a * s_b leave float32 where the results do not."""
+    blocks, nb = k // 128, n if b_rows == 1 else -(-n // 128)
+
+    def scales(rows, exponents):
+        e = torch.tensor([exponents[i % len(exponents)] for i in range(blocks)])
+        return (1 + torch.rand(rows, blocks, generator=gen)) * torch.exp2(e.float())
+
+    a = torch.randint(0, 2, (m, k), generator=gen).float()
+    b = torch.randint(0, 2, (n, k), generator=gen).float()
+    if kind == "small":  # s_a * s_b about 2^-144, results from 2^-122 on
+        return 256 * a, 256 * b, scales(m, [-72]), scales(nb, [-73])
+    if kind == "large":  # s_a * s_b about 2^131, results about 2^125
+        return a * 2.0 ** -9, b * 2.0 ** -6, scales(m, [119]), scales(nb, [11])
+    # blocks of zero sums with s_a * s_b about 2^202, beside others
+    a[:, ::2] = torch.where((torch.arange(0, k, 2) // 128 % 2 == 0), 0.0, a[:, ::2])
+    b[:, 1::2] = torch.where((torch.arange(1, k, 2) // 128 % 2 == 0), 0.0, b[:, 1::2])
+    return a, b, scales(m, [101, 70]), scales(nb, [100, -72])
+
+
+@pytest.mark.parametrize("kind", ["small", "large", "zero"])
+@pytest.mark.parametrize("m,n,k,dtype", [(*s, d) for s in FAR for d in (F32, B16)] +
+                         [(4000, 4090, 384, F32), (4500, 4700, 384, B16)], ids=str)
+@pytest.mark.parametrize("b_rows", [1, 128])
+def test_scales_far_apart(kind, m, n, k, dtype, b_rows):
+    """Products of two scales under and over float32's range, of results inside it.  A block's
+    sum has one rounding, its scales two, the sum of blocks one each: the bounds above."""
+    gen = torch.Generator().manual_seed(m + n + k)
+    a, b, sa, sb = far_scales(kind, m, n, k, b_rows, gen)
+    qa = mf.train.Fp8Blocks(a.to(F8).cuda(), sa.cuda())
+    qb = mf.train.Fp8Blocks(b.to(F8).cuda(), sb.cuda())
+
+    def exact(q, values, rows):
+        s = q.scales.double().repeat_interleave(rows, 0)[: values.shape[0]]
+        return values.cuda().double() * s.repeat_interleave(128, 1)
+
+    want = exact(qa, a, 1) @ exact(qb, b, b_rows).t()
+    assert torch.isfinite(want.to(dtype)).all()
+    check(mf.train.fp8_matmul(qa, qb, dtype), want, F32_SUM, kind)
+
+
+@pytest.mark.parametrize("rows", [2, 300])
+@pytest.mark.parametrize("dtype", [F32, B16], ids=str)
+def test_linear_of_values_far_apart(rows, dtype):
+    """Large values that meet zeros, and the smallest beside them, forward and both gradients."""
+    gen = torch.Generator().manual_seed(rows)
+    x, w, dy = randn(gen, rows, 384, dtype=dtype), randn(gen, 200, 384), randn(gen, rows, 200, dtype=dtype)
+    x[:, :128], w[:, :128] = 0.0, 0.0
+    x[:, 0], w[:, 1] = 2.0 ** 120, 2.0 ** 40
+    x[:, 256:], w[:, 256:] = x[:, 256:] * 2.0 ** -70, w[:, 256:] * 2.0 ** -72
+    dy[:, 128:] = 0.0
+    dy[0], dy[1:, 0] = 0.0, 2.0 ** 40  # the weight's gradient sums over rows
+    x[1:, 0] = 0.0
+    check(mf.train.fp8_linear(x.cuda(), mf.train.quantize_fp8(w.cuda(), 128)),
+          value(x, 1) @ value(w, 128).t(), F32_SUM, "held")
+    xg, wg = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    y = mf.train.fp8_linear(xg, wg)
+    check(y, value(x, 1) @ value(w, 128).t(), F32_SUM, "y")
+    dx, dw = torch.autograd.grad(y, (xg, wg), dy.cuda())
+    check(dx, value(dy, 1) @ value(w, 128), F32_SUM, "dx")
+    check(dw, value(dy.t(), 1) @ value(x.t(), 1).t(), F32_SUM, "dw")
