@@ -235,11 +235,14 @@ __device__ __forceinline__ bool far(float s) {
 
 using MatmulArgs = muon_train_fp8_matmul_args;
 
-// The fp8 MFMAs do not keep 32 bits of the products they add: measured against 64 bits,
-// results are off by 1.5e-5 to 2.7e-5 of their 2-norm, in chains of 16x16x32 as in single
-// 16x16x128 instructions.  Beside bf16's rounding (2^-9) that is nothing, and results that
-// leave as bf16 take them.  Results kept in fp32 (kExact) take the bf16 MFMA on the same
-// values, which bf16 holds exactly: 1e-7, at half the rate.
+// The fp8 MFMAs do not keep 32 bits of the products they add: of each eight (consecutive k) what
+// lies below 2^-13 of the largest is cut off, the eights are added in full (one product 2^-k of
+// another beside it: whole at k = 10, gone at k = 14; eight places further whole at k = 18).
+// Against 64 bits results are off by 1.5e-5 (normal values) to 7e-5 (log-uniform ones) of their
+// 2-norm, in chains of 16x16x32 as in single 16x16x128 instructions, at most 7·2^-13 of the sum
+// of magnitudes.  bf16's rounding is 2^-8, the values' own 2^-4: results that leave as bf16 take
+// them.  Results kept in fp32 (kExact) take the bf16 MFMA on the same values, which bf16 holds
+// exactly: 1e-7, at half the rate.
 using bf16x2 = __bf16 __attribute__((ext_vector_type(2)));
 using muon_polar::bf16x8;
 __device__ __forceinline__ bf16x8 to_bf16(uint32_t lo, uint32_t hi, float power) {

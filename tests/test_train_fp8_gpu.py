@@ -469,3 +469,23 @@ def test_linear_of_values_far_apart(rows, dtype):
     dx, dw = torch.autograd.grad(y, (xg, wg), dy.cuda())
     check(dx, value(dy, 1) @ value(w, 128), F32_SUM, "dx")
     check(dw, value(dy.t(), 1) @ value(x.t(), 1).t(), F32_SUM, "dw")
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 70, 1000), (70, 90, 1000), (32, 300, 5000), (2000, 4000, 400), (4500, 4700, 400)],
+                         ids=str)
+@pytest.mark.parametrize("b_rows", [1, 128])
+def test_what_bf16_results_keep_of_a_sum(m, n, k, b_rows):
+    """Element by element, with outliers among the values: eight products at a time are cut off
+    below 2^-13 of their largest, so a sum is off by at most 7 * 2^-13 of the sum of magnitudes,
+    and the sum of blocks in fp32 by 2^-20 of it; the result is the rounding of such a sum."""
+    gen = torch.Generator().manual_seed(m + k)
+    a, b = randn(gen, m, k), randn(gen, n, k)
+    a[:, ::11], b[:, ::13] = a[:, ::11] * 100, b[:, ::13] * 30
+    qa, qb = mf.train.quantize_fp8(a.cuda()), mf.train.quantize_fp8(b.cuda(), b_rows)
+    va, vb = value(a, 1).cuda(), value(b, b_rows).cuda()
+    exact, size = va @ vb.t(), va.abs() @ vb.abs().t()
+    off = (7 * 2.0 ** -13 + 2.0 ** -20) * size
+    got = mf.train.fp8_matmul(qa, qb)
+    assert (got >= (exact - off).to(B16)).all() and (got <= (exact + off).to(B16)).all()
+    off = (mf.train.fp8_matmul(qa, qb, F32).double() - exact).abs()
+    assert (off <= 2.0 ** -18 * size).all()  # at most 80 sums and roundings of 2^-24 behind another
