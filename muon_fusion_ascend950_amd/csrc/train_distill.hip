@@ -5,7 +5,8 @@
 // (up to 256 KiB: 1024 threads with 16 pieces of 16 bytes each); maximum and sum of
 // exponentials are taken from there, and the gradient is written from there: the logits
 // cross memory once in and once out, which is what bounds the pass.  Of a longer row the
-// threads take the rest with a running maximum and sum, and read it again for the gradient.
+// threads take the rest with a running maximum and sum, keep the next 128 KiB in LDS, and read
+// what lies past that again for the gradient.
 // Loss alone, and the gradient from a forward pass's stats, hold no row: it streams by.
 //
 // The gradient is the softmax everywhere but at the teacher's indices and the label.  All
@@ -236,7 +237,7 @@ struct Slope {
 
 // Entries of a row in LDS, (index, bits of the amount), read sixteen at a time by whoever looks
 // for an element's: one by one, each read waited for, an entry took 100 clocks of every
-// workgroup (4096 x 65536, 64 entries 225 us, 1024 entries 1008; so 211 and 456).
+// workgroup (4096 x 65536, 64 entries 225 us, 1024 entries 1008; so 213 and 472).
 using u32x2 = uint32_t __attribute__((ext_vector_type(2)));
 constexpr int kEntryGroup = 16;
 struct Entries {
@@ -355,8 +356,8 @@ __global__ __launch_bounds__(NT) void distill_loss_kernel(Args a) {
 
 // Loss and gradient: NT threads hold R chunks each of the row in registers, 16 waves a
 // compute unit whatever NT is, and L chunks more each in LDS: rows
-// up to 384 KiB are read once (4096 rows of 160000 in bf16: 731 -> 703 us, of 98304 in fp32 at
-// 2048 rows 332 -> 314), longer ones twice past that.
+// up to 384 KiB are read once (4096 rows of 160000 in bf16, with labels 656 -> 642 us, without 556
+// -> 549; 2048 rows of 98304 in fp32 344 -> 322), longer ones twice past that.
 template <class T, int NT, int R, int L, bool kHard>
 __global__ __launch_bounds__(NT, 4) void distill_both_kernel(Args a) {
     using Raw = typename T::Raw;

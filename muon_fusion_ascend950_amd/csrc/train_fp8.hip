@@ -473,7 +473,8 @@ __global__ __launch_bounds__((Geometry<BM, BN, WM, WN, D>::kThreads)) void matmu
     using Geo = Geometry<BM, BN, WM, WN, D>;
     constexpr int SM = WM / 16, SN = WN / 16, kLoads = Geo::kLoads;
     // The pipeline's registers leave no room for bf16 fragments (kExact) or a scale for each
-    // column (kRowB: 60 spilled, 8192 x 14336 x 8192 in 1275 us against 1004 without).
+    // column (kRowB: 60 spilled, 8192 x 14336 x 8192 in 1275 us against 1004 without; with scales
+    // taken apart it takes 1017 to 1050).
     constexpr bool kPipelined = Geo::kTwoSlots && !kExact && !kRowB;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[D * Geo::kSlot];
     const int lane = threadIdx.x & 63;
@@ -1119,10 +1120,11 @@ bool few_rows(const MatmulArgs &g) {
 
 // Side of a product's tiles.  A tile takes a compute unit's share of the tiles in turn: the
 // tile whose turns, at the time of one of its own size, end first.  Times as shares of a 256 x
-// 256 tile's, measured at K = 4096 (us a turn): 128 x 128 19.5 of 55, in fp32 32 of 110; 64 x
-// 64 7.7 and 13.3.  On both sides of the borders: 1024 x 2048 in 64s 17.3 us, in 128s 27.3;
-// 1024 x 4096 31.3 and 28.1; 2048 x 4096 in 128s 40.0, in 256s 51.6; 3000 x 4096 59.1 and 53.6
-// (fp32 100 and 111); 4096 x 6144 112 and 105 (fp32 192 and 215).
+// 256 tile's: at 8192 x 4096 x 4096 a turn of 256s takes 62 us, of 128s 20.5, of 64s 7.4 (fp32
+// 113, 32 and 11.3), the smaller ones' more where there are few (64s at 1024 x 2048 10.6).  On
+// both sides of the borders, K = 4096: 1024 x 2048 in 64s 21.1 us, in 128s 28.0; 1024 x 4096
+// 37.1 and 31.0; 2048 x 4096 in 128s 48.3, in 256s 52.3; 3000 x 4096 64.8 and 58.7 (fp32 104.9
+// and 107.0); 4096 x 6144 124 and 107 (fp32 198 and 211).
 int tile_side(const MatmulArgs &g, int cus) {
     if (g.k <= kBlock) return 64;  // a single block of K leaves nothing to pipeline
     const bool exact = g.c_dtype == MUON_TRAIN_F32;
@@ -1135,10 +1137,10 @@ int tile_side(const MatmulArgs &g, int cus) {
 // Parts of K that 64 x 64 tiles are split into where they leave compute units idle.  A tile's
 // unit takes in no more than 58 GB/s (29 bytes a clock) however many loads are under way: two
 // rings of half the steps each, in one workgroup, took 31.7 us against 33.6 at 32 x 4096 x
-// 14336, the parts on other units 15.7 with their joining (fp32 50 -> 19.6).  One workgroup a
+// 14336, the parts on other units 15.6 with their joining (fp32 51 -> 20).  One workgroup a
 // unit: two took 17.4.  A part keeps enough steps to fill its ring, and the join costs what
-// some 16 steps do: 128 x 4096 x 4096 saves 16 of 32 steps, 11.1 and 11.4 us (fp32 16.1 and
-// 14.2); 64 x 4096 x 4096 saves 24, 11.0 and 9.9; 512 x 768 x 2048 would save 8, 7.1 and 8.8.
+// some 16 steps do: 128 x 4096 x 4096 saves 16 of 32 steps, 12.7 and 12.6 us (fp32 17.8 and
+// 15.1); 64 x 4096 x 4096 saves 24, 12.7 and 10.4; 512 x 768 x 2048 would save 8, 8.1 and 9.5.
 int split_parts(const MatmulArgs &g, int cus) {
     constexpr int kSplitSteps = 4, kSplitGain = 16;
     if (few_rows(g) || tile_side(g, cus) != 64) return 1;

@@ -12,8 +12,8 @@
 //     d_y = ρ1·(dn − n·mean(dn·n))
 //
 // Sums over rows (the gradients of weights, of a gate that rows share and of the scale)
-// are kept in registers by the thread that owns the column, over the rows of its
-// workgroup; each workgroup writes them once and a second kernel adds the workgroups'
+// are kept by the thread that owns the column, in registers or (rows past 8192 columns) in
+// LDS, over the rows of its workgroup; each workgroup writes them once and a second kernel adds the workgroups'
 // in index order.  With a gate that all rows of a sequence share, one sum serves two
 // gradients: C = Σ dR·n gives d_w1 = gate·C and d_gate = w1·C.
 #include "train_common.hpp"
@@ -449,16 +449,16 @@ __global__ __launch_bounds__(64 * kFinishRuns) void norms_finish_kernel(Args a, 
     if (in && run == 0 && a.d_post_weight) store_any(a.d_post_weight, c, a.weight_dtype, total);
 }
 
-// Threads and pieces of a row.  Forward: two pieces a thread from 512 columns on, up to 107
-// registers, 20 waves a compute unit.  Backward, which holds more: two pieces and up to 256
+// Threads and pieces of a row.  Forward: one piece a thread up to 512 columns and from 1025 to
+// 2048 (64 registers, 32 waves a compute unit), otherwise two (up to 111, 16 waves).  Backward, which holds more: two pieces and up to 256
 // registers, 8 waves a compute unit; in bf16 with values that rows share one piece, whose 128
 // registers also hold the next row's, 16 waves, as far as 512 threads go.  16384 rows: of 4096
 // in bf16 161 us with one piece, 169 with two; with an fp32 residual 284 with one (some spilled)
 // and 237 with two, all in fp32 365 and 308; of 5120 (1024 threads would spill more, three in
 // eight of them idle) in bf16 254 and 250, fp32 residual 506 and 299, all in fp32 658 and 383.
 // Past 8192 columns two pieces of 1024 threads have 128 registers: their column sums lie in LDS
-// and the weights are read anew for each row (8192 rows of 16384 in bf16 413 us, 75 % of the
-// copy rate, in fp32 659, 94 %; with all of it held, 330 registers spilled, 809 and 1395; a gate
+// and the weights are read anew for each row (8192 rows of 16384 in bf16 388 to 413 us, 75 to 80 %
+// of the copy rate, in fp32 657, 94 %; with all of it held, 330 registers spilled, 809 and 1395; a gate
 // of y's shape still spills 100, 939 us and 44 %).
 struct Shape {
     int nt, v;
@@ -612,7 +612,7 @@ extern "C" int muon_train_norms_forward(const muon_train_norms_args *args, hipSt
     const int cus = compute_units();
     if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "norms: no device");
     const Shape s = forward_shape(a.d);
-    // as many workgroups as stay resident: each keeps its weights over its rows
+    // up to 32 waves a compute unit: each workgroup keeps its weights over its rows
     const int64_t resident = int64_t(cus) * (2048 / s.nt);
     const dim3 grid(static_cast<uint32_t>(a.rows < resident ? a.rows : resident));
     Launches launch{stream};
