@@ -21,6 +21,10 @@ using muon_polar::u32x4;
 inline int invalid(const char *msg) {
     return muon_polar::report(MUON_POLAR_ERR_INVALID_ARGUMENT, msg);
 }
+// A launch has at most 2^32 - 1 threads; one with more came back as done, only the rest past a
+// multiple of 2^32 having run.
+constexpr int64_t kMaxThreads = UINT32_MAX;
+
 // The launches of one call.  Each gives its own status: hipGetLastError would also give an
 // error that some earlier HIP call of the thread left behind.
 struct Launches {
@@ -28,6 +32,7 @@ struct Launches {
     hipError_t status = hipSuccess;
     template <class... P, class... A>
     void operator()(void (*kernel)(P...), dim3 grid, int threads, const A &...a) {
+        if (status == hipSuccess && int64_t(grid.x) * threads > kMaxThreads) status = hipErrorInvalidConfiguration;
         if (status != hipSuccess) return;
         auto launch = [&](P... p) {
             void *args[] = {const_cast<void *>(static_cast<const void *>(&p))...};

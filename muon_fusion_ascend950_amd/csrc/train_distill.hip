@@ -581,11 +581,11 @@ void launch_grad(const Args &a, int cus, Launches &launch) {
 }
 #define MUON_TRAIN_LAUNCH(which)                                                              \
     do {                                                                                      \
-        const bool hard = args->labels != nullptr;                                            \
-        if (args->logits_dtype == MUON_TRAIN_BF16)                                            \
-            hard ? which<Bf16, true>(*args, cus, launch) : which<Bf16, false>(*args, cus, launch); \
+        const bool hard = a.labels != nullptr;                                                \
+        if (a.logits_dtype == MUON_TRAIN_BF16)                                                \
+            hard ? which<Bf16, true>(a, cus, launch) : which<Bf16, false>(a, cus, launch);    \
         else                                                                                  \
-            hard ? which<F32, true>(*args, cus, launch) : which<F32, false>(*args, cus, launch);   \
+            hard ? which<F32, true>(a, cus, launch) : which<F32, false>(a, cus, launch);      \
     } while (0)
 
 }  // namespace
@@ -594,6 +594,38 @@ void launch_grad(const Args &a, int cus, Launches &launch) {
 
 using namespace muon_train;
 
+namespace muon_train {
+namespace {
+
+// Calls f with the arguments of up to kSlice rows after another: of one launch's threads (a row
+// takes 1024 at most).
+template <class F>
+void over_slices(const Args &args, F &&f) {
+    constexpr int64_t kSlice = int64_t(1) << 21;
+    static_assert(kSlice * 1024 <= kMaxThreads, "threads of a launch");
+    const int64_t size = args.logits_dtype == MUON_TRAIN_BF16 ? 2 : 4;
+    const int64_t teacher_size = args.teacher_dtype == MUON_TRAIN_BF16 ? 2 : 4;
+    auto past = [](auto *p, int64_t bytes) {
+        return p ? reinterpret_cast<decltype(p)>(reinterpret_cast<uintptr_t>(p) + static_cast<uintptr_t>(bytes)) : p;
+    };
+    for (int64_t row = 0; row < args.rows; row += kSlice) {
+        Args a = args;
+        a.rows = args.rows - row < kSlice ? args.rows - row : kSlice;
+        a.logits = past(args.logits, row * args.ld_logits * size);
+        a.grad = past(args.grad, row * args.ld_grad * size);
+        a.teacher_logits = past(args.teacher_logits, row * args.k * teacher_size);
+        a.teacher_indices = past(args.teacher_indices, row * args.k * args.index_bytes);
+        a.labels = past(args.labels, row * int64_t(sizeof(int64_t)));
+        a.grad_loss = past(args.grad_loss, row * int64_t(sizeof(float)));
+        a.loss = past(args.loss, row * int64_t(sizeof(float)));
+        a.stats = past(args.stats, row * int64_t(4 * sizeof(float)));
+        f(a);
+    }
+}
+
+}  // namespace
+}  // namespace muon_train
+
 extern "C" int muon_train_distill_forward(const muon_train_distill_args *args, hipStream_t stream) {
     const int st = check(args);
     if (st != MUON_POLAR_OK || args->rows == 0) return st;
@@ -601,10 +633,12 @@ extern "C" int muon_train_distill_forward(const muon_train_distill_args *args, h
     const int cus = compute_units();
     if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "distill: no device");
     Launches launch{stream};
-    if (args->grad)
-        MUON_TRAIN_LAUNCH(launch_both);
-    else
-        MUON_TRAIN_LAUNCH(launch_loss);
+    over_slices(*args, [&](const Args &a) {
+        if (a.grad)
+            MUON_TRAIN_LAUNCH(launch_both);
+        else
+            MUON_TRAIN_LAUNCH(launch_loss);
+    });
     return launch.result("distill_forward");
 }
 
@@ -615,6 +649,6 @@ extern "C" int muon_train_distill_backward(const muon_train_distill_args *args, 
     const int cus = compute_units();
     if (cus <= 0) return muon_polar::report(MUON_POLAR_ERR_HIP, "distill: no device");
     Launches launch{stream};
-    MUON_TRAIN_LAUNCH(launch_grad);
+    over_slices(*args, [&](const Args &a) { MUON_TRAIN_LAUNCH(launch_grad); });
     return launch.result("distill_backward");
 }

@@ -147,7 +147,7 @@ struct BackwardPlan {
 // 4096 in bf16 take 165 us, without 181 to 195 (805 MB: 4.9 TB/s).
 template <class TY, class TR, int NT, int V, bool kGeneral>
 __global__ __launch_bounds__(NT, V == 1 && !kGeneral ? 4 : 1) void norms_backward_kernel(Args a, BackwardPlan plan,
-                                                                           float *part,
+                                                                           int64_t first_group, float *part,
                                                                            double *part_scale) {
     using RawY = typename TY::Raw;
     using RawR = typename TR::Raw;
@@ -165,12 +165,13 @@ __global__ __launch_bounds__(NT, V == 1 && !kGeneral ? 4 : 1) void norms_backwar
     const bool single = a.d == 1;
     const float eps = float(a.eps);
 
-    // rows of this workgroup: first, first + step, .. below end
-    int64_t first = blockIdx.x, step = gridDim.x, end = a.rows;
+    // rows of this workgroup, `group` of all: first, first + step, .. below end
+    const int64_t group = first_group + blockIdx.x;
+    int64_t first = group, step = plan.groups, end = a.rows;
     int64_t sequence = 0;
     if (seq_gate) {
-        sequence = blockIdx.x / plan.groups_per_sequence;
-        first = sequence * a.rows_per_sequence + blockIdx.x % plan.groups_per_sequence;
+        sequence = group / plan.groups_per_sequence;
+        first = sequence * a.rows_per_sequence + group % plan.groups_per_sequence;
         step = plan.groups_per_sequence;
         end = (sequence + 1) * a.rows_per_sequence;
     }
@@ -341,7 +342,7 @@ __global__ __launch_bounds__(NT, V == 1 && !kGeneral ? 4 : 1) void norms_backwar
             o.store(static_cast<RawY *>(a.d_y) + row * a.d + col[v], valid[v]);
         }
     }
-    float *mine = part + int64_t(blockIdx.x) * plan.sums * a.d;
+    float *mine = part + group * plan.sums * a.d;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         float sum[8];
@@ -361,7 +362,7 @@ __global__ __launch_bounds__(NT, V == 1 && !kGeneral ? 4 : 1) void norms_backwar
     if (tid == 0) {
         double t = totals[0];
         for (int w = 1; w < NT / 64; ++w) t += totals[w];
-        part_scale[blockIdx.x] = t;
+        part_scale[group] = t;
     }
 }
 
@@ -659,8 +660,13 @@ extern "C" int muon_train_norms_backward(const muon_train_norms_args *args, void
                 constexpr bool kGeneral = decltype(is_general)::value;
                 constexpr bool kOnePiece = std::is_same_v<decltype(ty), Bf16> && std::is_same_v<decltype(tr), Bf16> && !kGeneral;
                 with_backward_shape<kOnePiece>({p.nt, p.v}, [&](auto nt, auto v) {
-                    launch(norms_backward_kernel<decltype(ty), decltype(tr), decltype(nt)::value, decltype(v)::value, kGeneral>,
-                           dim3(static_cast<uint32_t>(p.groups)), p.nt, a, p, part, part_scale);
+                    // one launch but for gates of very many sequences
+                    const int64_t most = kMaxThreads / p.nt;
+                    for (int64_t g = 0; g < p.groups; g += most) {
+                        const dim3 grid(static_cast<uint32_t>(p.groups - g < most ? p.groups - g : most));
+                        launch(norms_backward_kernel<decltype(ty), decltype(tr), decltype(nt)::value, decltype(v)::value, kGeneral>,
+                               grid, p.nt, a, p, g, part, part_scale);
+                    }
                 });
             };
             if (general(a)) go(std::true_type{});

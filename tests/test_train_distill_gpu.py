@@ -316,3 +316,23 @@ def test_rows_without_a_term_have_none_of_its_gradient(v, dtype):
     _, grad = run_all(bare, tau=1.5)
     for row in range(8):
         assert not grad[row].any(), row
+
+
+def test_more_rows_than_a_launch_takes():
+    """A launch has at most 2^32 - 1 threads, a row up to 1024 of them."""
+    rows, v = (1 << 24) + 5, 3
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    z = torch.randn(rows, v, device="cuda", generator=gen)
+    index = torch.randint(0, v, (rows, 1), device="cuda", generator=gen, dtype=torch.int32)
+    teacher = torch.zeros(rows, 1, device="cuda")
+    labels = torch.randint(-1, v, (rows,), device="cuda", generator=gen)
+    weight = torch.rand(rows, device="cuda", generator=gen)
+    kw = dict(temperature=2.0, labels=labels, label_weight=0.25)
+    want = formula(z, teacher, index, 2.0, labels, 0.25, weight)
+    loss, grad = mf.train.distill_topk_with_grad(z, teacher, index, grad_loss=weight, **kw)
+    check(loss, want[0], BOUND, "loss")
+    check(grad, want[1], BOUND, "gradient")
+    z.requires_grad_(True)
+    alone = mf.train.distill_topk(z, teacher, index, **kw)
+    (auto,) = torch.autograd.grad(alone, z, weight)
+    assert torch.equal(alone, loss) and torch.equal(auto, grad)

@@ -284,3 +284,19 @@ def test_sequences_without_tokens(shape):
     (out.sum() + h.sum()).backward()
     for t in (y, r, gate, weight):
         assert t.grad.shape == t.shape and not t.grad.any()
+
+
+def test_more_sequences_than_a_launch_takes():
+    """A launch has at most 2^32 - 1 threads, a sequence with a gate of its own 64 of them."""
+    b = (1 << 26) + 3
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    # two tokens of one channel that is left as it is: each gradient is a product or a sum of two
+    y, r = (torch.randint(-4, 5, (b, 2, 1), device="cuda", generator=gen).bfloat16() for _ in range(2))
+    gate = torch.randint(1, 5, (b, 1, 1), device="cuda", generator=gen).bfloat16()
+    d_out = torch.randint(-2, 3, (b, 2, 1), device="cuda", generator=gen).bfloat16()
+    leaves = [t.requires_grad_(True) for t in (y, r, gate)]
+    out, _ = mf.train.block_norms(y, r, gate=gate, post_norm=False, pre_norm=False)
+    dy, dr, dgate = torch.autograd.grad(out, leaves, d_out)
+    assert torch.equal(out, r + gate * y) and torch.equal(dr, d_out)
+    assert torch.equal(dy, gate * d_out)
+    assert torch.equal(dgate, (d_out * y).sum(1, keepdim=True))
