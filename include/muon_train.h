@@ -76,7 +76,9 @@ typedef struct muon_train_norms_args {
 } muon_train_norms_args;
 
 int muon_train_norms_forward(const muon_train_norms_args *args, hipStream_t stream);
-/* Bytes of workspace the backward pass of these sizes and kinds needs (host call). */
+/* Bytes of workspace the backward pass of these sizes and kinds needs (host call): 2·d fp32 (3·d
+ * with a scale vector) for each workgroup that the card holds at once, and for each sequence at
+ * least with a sequence gate. */
 int muon_train_norms_workspace(const muon_train_norms_args *args, size_t *bytes);
 int muon_train_norms_backward(const muon_train_norms_args *args, void *workspace,
                               size_t workspace_bytes, hipStream_t stream);

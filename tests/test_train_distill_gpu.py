@@ -336,3 +336,21 @@ def test_more_rows_than_a_launch_takes():
     alone = mf.train.distill_topk(z, teacher, index, **kw)
     (auto,) = torch.autograd.grad(alone, z, weight)
     assert torch.equal(alone, loss) and torch.equal(auto, grad)
+
+
+@pytest.mark.parametrize("dtype", [F32, B16], ids=str)
+@pytest.mark.parametrize("v", [300, 20011, 200003])
+@pytest.mark.parametrize("labels", [False, True])
+def test_rows_whose_softmax_is_nan(v, dtype, labels):
+    """A NaN, +inf or -inf everywhere makes the whole of that row's gradient NaN, no other's."""
+    s = make(7, v, 4, dtype, labels=True)
+    s["labels"][:] = 2
+    if not labels:
+        s["labels"] = None
+    s["z"][1, 9] = math.nan
+    s["z"][2, 9] = math.inf
+    s["z"][3] = -math.inf
+    s["z"][4, s["index"][4, 1]] = -math.inf  # the teacher wants what the student masks
+    loss, grad = run_all(s, tau=2.0, lam=0.3)
+    assert loss[1:4].isnan().all() and loss[4] == math.inf
+    assert grad[1:4].isnan().all() and grad[[0, 4, 5, 6]].isfinite().all()
