@@ -598,7 +598,7 @@ namespace muon_train {
 namespace {
 
 // Calls f with the arguments of up to kSlice rows after another: of one launch's threads (a row
-// takes 1024 at most).
+// takes 1024 at most).  Slices of one size, so that all take the kernel of many rows.
 template <class F>
 void over_slices(const Args &args, F &&f) {
     constexpr int64_t kSlice = int64_t(1) << 21;
@@ -608,9 +608,10 @@ void over_slices(const Args &args, F &&f) {
     auto past = [](auto *p, int64_t bytes) {
         return p ? reinterpret_cast<decltype(p)>(reinterpret_cast<uintptr_t>(p) + static_cast<uintptr_t>(bytes)) : p;
     };
-    for (int64_t row = 0; row < args.rows; row += kSlice) {
+    const int64_t slices = (args.rows + kSlice - 1) / kSlice, each = (args.rows + slices - 1) / slices;
+    for (int64_t row = 0; row < args.rows; row += each) {
         Args a = args;
-        a.rows = args.rows - row < kSlice ? args.rows - row : kSlice;
+        a.rows = args.rows - row < each ? args.rows - row : each;
         a.logits = past(args.logits, row * args.ld_logits * size);
         a.grad = past(args.grad, row * args.ld_grad * size);
         a.teacher_logits = past(args.teacher_logits, row * args.k * teacher_size);
