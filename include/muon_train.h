@@ -149,10 +149,11 @@ int muon_train_fp8_quantize(const muon_train_fp8_quantize_args *args, hipStream_
  * time and cuts each off below 2^-13 of their largest: at most 7·2^-13 of the sum of |a·b|,
  * 1.5e-5 to 7e-5 of a result's 2-norm measured.  a_scale·b_scale may leave fp32's range where
  * the result does not. */
+enum { MUON_TRAIN_FP8_MAX_LD = 1 << 22, MUON_TRAIN_FP8_MAX_SCALES = 1 << 28 };
 typedef struct muon_train_fp8_operand {
     const void *values; /* [rows, k], 16-byte aligned */
     const float *scales;
-    int64_t ld, scale_row, scale_col;
+    int64_t ld, scale_row, scale_col; /* ld at most MAX_LD, scale_col·(k / 128 + 1) MAX_SCALES */
     int block_rows; /* 1 (scale_row must be 1) or 128 */
 } muon_train_fp8_operand;
 typedef struct muon_train_fp8_matmul_args {

@@ -919,6 +919,13 @@ struct Fp8LinearFunction : torch::autograd::Function<Fp8LinearFunction> {
     }
 };
 
+// Whether an operand of a product, rows of `width` values with `scales` scales in each column of
+// blocks, lies within what a product reaches (include/muon_train.h).
+bool reached(int64_t width, int64_t scales) {
+    return blocks(width) * kBlock <= MUON_TRAIN_FP8_MAX_LD &&
+           scales <= MUON_TRAIN_FP8_MAX_SCALES / (blocks(width) + 1);
+}
+
 at::Tensor Fp8LinearTrain(const at::Tensor &x, const at::Tensor &weight) {
     check_tensor("x", x, nullptr, kFloats);
     TORCH_CHECK_VALUE(x.dim() >= 1, "x must have shape [..., K]");
@@ -927,6 +934,13 @@ at::Tensor Fp8LinearTrain(const at::Tensor &x, const at::Tensor &weight) {
                       "weight must have shape [N, ", x.size(-1), "], got ", weight.sizes());
     TORCH_CHECK_VALUE(weight.numel() > 0, "weight's dimensions must be positive");
     refuse_tangents("fp8_linear", x, weight);
+    // what the backward pass would refuse: dy [tokens, N], and both operands transposed
+    const int64_t tokens = rows_of(x), n = weight.size(0), k = weight.size(1);
+    if (at::GradMode::is_enabled())
+        TORCH_CHECK_VALUE((!wants_grad(x) || reached(n, tokens)) &&
+                              (!wants_grad(weight) || (reached(tokens, n) && reached(tokens, k))),
+                          "too many tokens for a backward pass in one call, ", tokens, " of ", k, " to ", n,
+                          " columns");
     if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight)))
         return Fp8LinearFunction::apply(x, weight,
                                         int64_t(wants_grad(x)) | wants_grad(weight) << 1);

@@ -1032,11 +1032,11 @@ int check(const muon_train_fp8_operand &o, int64_t k) {
         return invalid("fp8: values must be 16-byte aligned, row by row");
     if (o.ld < k) return invalid("fp8: rows of values must not overlap");
     // the rows of a tile are reached by 31-bit offsets
-    if (o.ld > (1 << 22)) return invalid("fp8: rows of values lie too far apart");
+    if (o.ld > MUON_TRAIN_FP8_MAX_LD) return invalid("fp8: rows of values lie too far apart");
     if (o.block_rows != 1 && o.block_rows != kBlock) return invalid("fp8: block_rows must be 1 or 128");
     // so are the scales of a tile
     if (o.scale_row < 0 || o.scale_row > (1 << 26) || o.scale_col < 0 ||
-        o.scale_col > (int64_t(1) << 28) / (k / kBlock + 1))
+        o.scale_col > MUON_TRAIN_FP8_MAX_SCALES / (k / kBlock + 1))
         return invalid("fp8: scales lie too far apart");
     if (o.block_rows == 1 && o.scale_row != 1)
         return invalid("fp8: scales of single rows must lie next to each other");

@@ -247,7 +247,8 @@ def fp8_linear(x: torch.Tensor, weight) -> torch.Tensor:
     weight: a float32 or bfloat16 matrix (training: quantised in this call, and with the
     gradients dx = dy @ weight and dweight = dy.T @ x, whose products are in 8 bits too, dy
     and x quantised in blocks of 128 along the axis that each product sums over), or
-    ``Fp8Blocks`` (serving: no gradient).
+    ``Fp8Blocks`` (serving: no gradient).  A call whose weight wants a gradient takes up to 2**22
+    tokens, and tokens * max(N, K) up to about 2**35; one whose x does, tokens * N.
     """
     try:
         if isinstance(weight, Fp8Blocks):

@@ -454,3 +454,22 @@ def test_forward_mode_is_refused(name):
         if "with_grad" not in name:  # writes into a tensor: no vmap
             with pytest.raises(NotImplementedError, match="forward"):
                 torch.func.jvp(torch.vmap(call), (_cuda(2, 4, 64),), (_cuda(2, 4, 64),))
+
+
+@pytest.mark.parametrize("tokens,n,k,wanted", [
+    ((1 << 22) + 1, 64, 64, "weight"),  # a row of the transposed operands
+    (1 << 21, 64, 1 << 14, "weight"), (1 << 21, 1 << 14, 64, "weight"),  # their scales
+    (1 << 21, 1 << 14, 64, "x"),  # the gradient's scales
+])
+def test_fp8_linear_refuses_what_its_backward_pass_could_not_do(tokens, n, k, wanted):
+    """At the call, not in the backward pass that follows it."""
+    with FakeTensorMode():
+        x, w = _cuda(tokens, k, dtype=B16), _cuda(n, k)
+        train.fp8_linear(x, w)  # no gradient wanted
+        (w if wanted == "weight" else x).requires_grad_(True)
+        with pytest.raises(ValueError, match="tokens"):
+            train.fp8_linear(x, w)
+        with torch.no_grad():
+            train.fp8_linear(x, w)
+        less = x[: 1 << 14]
+        assert train.fp8_linear(less, w).requires_grad
